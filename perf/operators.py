@@ -20,36 +20,36 @@ DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 def listed():
     return [
         # one decode step of 64 running requests: one new token each, most of them on a page they have
-        {"name": "slots, decode step", "op": "slots", "b": 64, "page": 64, "cached": "4096:65536", "new": "1:1", "mix": 1},
+        {"name": "slots: decode step", "op": "slots", "b": 64, "page": 64, "cached": "4096:65536", "new": "1:1", "mix": 1},
         # admission of a batch of prompts, a third of them behind a cached prefix, pages of 48 tokens
-        {"name": "slots, prompts admitted", "op": "slots", "b": 301, "page": 48, "cached": "0:5000", "new": "1:2048", "mix": 2},
+        {"name": "slots: prompts admitted", "op": "slots", "b": 301, "page": 48, "cached": "0:5000", "new": "1:2048", "mix": 2},
         # the index lists of one sparse decode step: 64 requests, 2048 positions each
-        {"name": "indices, decode step", "op": "indices", "lens": _text([1] * 64), "ctx": 32768, "topk": 2048, "page": 64, "packed": False},
+        {"name": "indices: decode step", "op": "indices", "lens": _text([1] * 64), "ctx": 32768, "topk": 2048, "page": 64, "packed": False},
         # the index lists of a sparse prefill of three packed sequences
-        {"name": "indices, prefill", "op": "indices", "lens": "5000,1,3191", "ctx": 0, "topk": 2048, "page": 256, "packed": True},
+        {"name": "indices: prefill", "op": "indices", "lens": "5000,1,3191", "ctx": 0, "topk": 2048, "page": 256, "packed": True},
         # short prompts admitted together, grouped heads
-        {"name": "prefill, short prompts", "op": "prefill", "b": 13, "q": "1:300", "ctx": "0:0", "h_q": 16, "h_kv": 2,
+        {"name": "prefill: short prompts", "op": "prefill", "b": 13, "q": "1:300", "ctx": "0:0", "h_q": 16, "h_kv": 2,
          "d_qk": 128, "d_v": 128, "dtype": "bf16", "causal": True, "sink": False, "mix": 3},
         # one latent-attention prompt with the keys and values of every head written out, one tensor-parallel shard
-        {"name": "prefill, one prompt of 8192", "op": "prefill", "b": 1, "q": "8192:8192", "ctx": "0:0", "h_q": 16, "h_kv": 16,
+        {"name": "prefill: one prompt of 8192", "op": "prefill", "b": 1, "q": "8192:8192", "ctx": "0:0", "h_q": 16, "h_kv": 16,
          "d_qk": 192, "d_v": 128, "dtype": "bf16", "causal": True, "sink": False, "mix": 4},
         # packed prompts of uneven lengths, some behind a cached context, grouped heads with sinks
-        {"name": "prefill, packed and chunked", "op": "prefill", "b": 7, "q": "257:4096", "ctx": "0:2048", "h_q": 24, "h_kv": 4,
+        {"name": "prefill: packed and chunked", "op": "prefill", "b": 7, "q": "257:4096", "ctx": "0:2048", "h_q": 24, "h_kv": 4,
          "d_qk": 128, "d_v": 128, "dtype": "fp16", "causal": True, "sink": True, "mix": 5},
         # single tokens over contexts of up to 16384
-        {"name": "prefill, single tokens", "op": "prefill", "b": 8, "q": "1:1", "ctx": "1000:16383", "h_q": 32, "h_kv": 8,
+        {"name": "prefill: single tokens", "op": "prefill", "b": 8, "q": "1:1", "ctx": "1000:16383", "h_q": 32, "h_kv": 8,
          "d_qk": 128, "d_v": 128, "dtype": "bf16", "causal": True, "sink": False, "mix": 6},
         # four samples of one prompt, a tensor-parallel shard of 16 heads
-        {"name": "shared prefix, 4 samples", "op": "shared", "layout": "V32", "b": 4, "s_q": 1, "h_q": 16, "prefix": 2000,
+        {"name": "shared prefix: 4 samples", "op": "shared", "layout": "V32", "b": 4, "s_q": 1, "h_q": 16, "prefix": 2000,
          "suffix": "1:100", "page": 64, "sink": False, "mix": 7},
         # 16 requests behind one system prompt, all heads
-        {"name": "shared prefix, 16 requests", "op": "shared", "layout": "V32", "b": 16, "s_q": 1, "h_q": 64, "prefix": 32768,
+        {"name": "shared prefix: 16 requests", "op": "shared", "layout": "V32", "b": 16, "s_q": 1, "h_q": 64, "prefix": 32768,
          "suffix": "1:1024", "page": 64, "sink": False, "mix": 8},
         # 64 requests, the largest
-        {"name": "shared prefix, 64 requests", "op": "shared", "layout": "V32", "b": 64, "s_q": 1, "h_q": 64, "prefix": 32768,
+        {"name": "shared prefix: 64 requests", "op": "shared", "layout": "V32", "b": 64, "s_q": 1, "h_q": 64, "prefix": 32768,
          "suffix": "64:2048", "page": 64, "sink": False, "mix": 9},
         # two drafted tokens per request, the other cache layout, a sink, an odd number of heads and of tokens
-        {"name": "shared prefix, drafted tokens", "op": "shared", "layout": "MODEL1", "b": 37, "s_q": 2, "h_q": 24, "prefix": 10007,
+        {"name": "shared prefix: drafted tokens", "op": "shared", "layout": "MODEL1", "b": 37, "s_q": 2, "h_q": 24, "prefix": 10007,
          "suffix": "0:500", "page": 256, "sink": True, "mix": 10},
     ]
 
