@@ -354,6 +354,34 @@ int dsv4_kv_store_rows(const Dsv4StoreRowsArgs* r, void* stream) {
   return e ? cuda_fail(e) : DSV4_OK;
 }
 
+int dsv4_build_slot_maps(const Dsv4SlotMapArgs* a, void* stream) {
+  if (!a || !a->cu_new || !a->cu_total || !a->n_taken) return DSV4_ERR_NULL;
+  if (a->b < 0 || a->b > dsv4::SLOT_MAP_MAX_REQUESTS || a->max_pages < 0 || a->page_block_size < 1 ||
+      a->n_slots < 0 || a->n_free < 0)
+    return DSV4_ERR_SHAPE;
+  if ((a->b && (!a->cached_lens || !a->new_lens)) || (a->b && a->max_pages && !a->block_table) ||
+      (a->n_free && !a->free_pages) || (a->n_slots && (!a->slots || !a->positions)))
+    return DSV4_ERR_NULL;
+  if (a->b > 1 && a->stride_table < a->max_pages) return DSV4_ERR_LAYOUT;   // rows would overlap
+  int rc = current_device_is_sm100();
+  if (rc) return rc;
+  cudaError_t e = dsv4::launch_slot_maps(*a, static_cast<cudaStream_t>(stream));
+  return e ? cuda_fail(e) : DSV4_OK;
+}
+
+int dsv4_page_indices(const Dsv4PageIndicesArgs* a, void* stream) {
+  if (!a) return DSV4_ERR_NULL;
+  if (a->n_rows < 0 || a->topk < 0 || a->b < 0 || a->max_pages < 0 || a->page_block_size < 1 ||
+      a->s_q < 1 || a->stride_positions < 0 || a->stride_table < 0)
+    return DSV4_ERR_SHAPE;
+  if (a->n_rows == 0 || a->topk == 0) return DSV4_OK;
+  if (!a->positions || !a->indices || (a->b && a->max_pages && !a->block_table)) return DSV4_ERR_NULL;
+  int rc = current_device_is_sm100();
+  if (rc) return rc;
+  cudaError_t e = dsv4::launch_page_indices(*a, static_cast<cudaStream_t>(stream));
+  return e ? cuda_fail(e) : DSV4_OK;
+}
+
 int dsv4_gather_dequant(const void* kv, int64_t stride_kv_block, int32_t kv_format,
                         int32_t num_blocks, int32_t page_block_size, const int32_t* indices,
                         int32_t n, void* rows_bf16, int32_t method, void* stream) {

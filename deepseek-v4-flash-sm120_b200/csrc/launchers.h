@@ -37,6 +37,11 @@ cudaError_t launch_gather_dequant(const void* kv, int64_t stride, int kv_format,
                                   int page_block, const int32_t* indices, int n, void* rows,
                                   int method, cudaStream_t st);
 
+// Block tables and slot maps (paging.cu).
+constexpr int SLOT_MAP_MAX_REQUESTS = 16384;     // both sums of a request list in shared memory
+cudaError_t launch_slot_maps(const Dsv4SlotMapArgs& a, cudaStream_t st);
+cudaError_t launch_page_indices(const Dsv4PageIndicesArgs& a, cudaStream_t st);
+
 // tcgen05 kernels (sparse_attn_sm100.cu).  `supported` reports whether the
 // tensor-core kernel handles this (format, d_qk) pair.
 bool sm100_attn_supported(int kv_format, int d_qk);

@@ -71,6 +71,20 @@ class StoreRowsArgs(C.Structure):
         (n, i32) for n in ("loc_is_int64", "reserved")]
 
 
+class SlotMapArgs(C.Structure):
+    _fields_ = [(n, i32) for n in ("b", "max_pages", "page_block_size", "n_slots", "n_free",
+                                   "reserved")] + [
+        (n, vp) for n in ("block_table", "cached_lens", "new_lens", "free_pages", "slots",
+                          "positions", "cu_new", "cu_total", "n_taken")] + [("stride_table", i64)]
+
+
+class PageIndicesArgs(C.Structure):
+    _fields_ = [(n, i32) for n in ("n_rows", "topk", "b", "s_q", "max_pages",
+                                   "page_block_size")] + [
+        (n, vp) for n in ("block_table", "positions", "cu_seqlens", "indices")] + [
+        (n, i64) for n in ("stride_table", "stride_positions")]
+
+
 # name -> (restype, argtypes); every symbol include/dsv4_b200.h declares.
 SYMBOLS = {
     "dsv4_abi_version": (C.c_int, []),
@@ -88,6 +102,8 @@ SYMBOLS = {
     "dsv4_sparse_prefill": (C.c_int, [C.POINTER(PrefillArgs), vp]),
     "dsv4_kv_store": (C.c_int, [C.POINTER(StoreArgs), vp]),
     "dsv4_kv_store_rows": (C.c_int, [C.POINTER(StoreRowsArgs), vp]),
+    "dsv4_build_slot_maps": (C.c_int, [C.POINTER(SlotMapArgs), vp]),
+    "dsv4_page_indices": (C.c_int, [C.POINTER(PageIndicesArgs), vp]),
     "dsv4_gather_dequant": (C.c_int, [vp, i64, i32, i32, i32, vp, i32, vp, i32, vp]),
     "dsv4_device_status": (C.c_int, [C.POINTER(C.c_int32), C.c_int]),
     "dsv4_debug_set_timeline": (C.c_int, [vp]),

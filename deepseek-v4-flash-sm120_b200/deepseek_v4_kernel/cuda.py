@@ -286,6 +286,96 @@ def kv_store_rows(k, loc, kv) -> None:
                 "dsv4_kv_store_rows")
 
 
+def _int32_on(name, t, device, dim) -> None:
+    _require(t.dtype == torch.int32 and t.dim() == dim and t.device == device,
+             f"{name} must be {dim}-D int32 on {device}")
+
+
+def build_slot_maps(block_table, cached_lens, new_lens, free_pages, page_block: int, n_slots: int):
+    """Block tables and slot maps of one serving step, from request lengths on the device.
+
+      block_table [b, max_pages] int32, updated IN PLACE with the pages of the new tokens;
+      cached_lens, new_lens [b] int32; free_pages [n_free] int32 page ids, taken from the
+      front in request order; n_slots = capacity for the packed new tokens of all requests
+      -> (slots int64 [n_slots], positions int32 [n_slots], cu_new int32 [b + 1],
+          cu_total int32 [b + 1], n_taken int32 [1])
+
+    slots / positions of the tokens in request order (slots are what `kv_store` and
+    `kv_store_rows` take), -1 behind the last one; a token without a page has slot -1.
+    cu_new / cu_total are the running sums of new_lens and cached_lens + new_lens (the two
+    arrays `dense_prefill_fwd` takes).  n_taken > n_free says that the free list was too
+    short.  No host synchronisation; see dsv4_build_slot_maps in the C header.  No
+    counterpart in the reference, whose serving framework builds these on the host."""
+    _require(block_table.is_cuda, "block_table must be a CUDA tensor")
+    dev = block_table.device
+    _int32_on("block_table", block_table, dev, 2)
+    b, max_pages = block_table.shape
+    for name, t in (("cached_lens", cached_lens), ("new_lens", new_lens)):
+        _int32_on(name, t, dev, 1)
+        _require(t.numel() == b and t.is_contiguous(), f"{name} must be contiguous [{b}]")
+    _int32_on("free_pages", free_pages, dev, 1)
+    _require(free_pages.is_contiguous(), "free_pages must be contiguous")
+    _require(max_pages <= 1 or block_table.stride(1) == 1, "block_table rows must be dense")
+    page_block, n_slots = int(page_block), int(n_slots)
+    _require(1 <= page_block < 2 ** 31 and 0 <= n_slots < 2 ** 31, "page_block >= 1 and n_slots >= 0 expected")
+    _require(b <= 16384, "at most 16384 requests")
+    with torch.cuda.device(dev):
+        slots = torch.empty((n_slots,), dtype=torch.int64, device=dev)
+        ints = torch.empty((n_slots + 2 * (b + 1) + 1,), dtype=torch.int32, device=dev)
+        positions, cu_new, cu_total, n_taken = ints.split([n_slots, b + 1, b + 1, 1])
+        a = N.SlotMapArgs()
+        a.b, a.max_pages, a.page_block_size, a.n_slots = b, max_pages, page_block, n_slots
+        a.n_free = free_pages.numel()
+        a.block_table, a.stride_table = block_table.data_ptr(), block_table.stride(0) if b > 1 else max_pages
+        a.cached_lens, a.new_lens, a.free_pages = cached_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr()
+        a.slots, a.positions = slots.data_ptr(), positions.data_ptr()
+        a.cu_new, a.cu_total, a.n_taken = cu_new.data_ptr(), cu_total.data_ptr(), n_taken.data_ptr()
+        N.check(N.lib.dsv4_build_slot_maps(C.byref(a), torch.cuda.current_stream(dev).cuda_stream),
+                "dsv4_build_slot_maps")
+    return slots, positions, cu_new, cu_total, n_taken
+
+
+def page_indices(block_table, positions, page_block: int, cu_seqlens=None) -> torch.Tensor:
+    """Logical positions -> the physical token indices `sparse_decode_fwd` and the sparse
+    prefills take.
+
+      block_table [b, max_pages] int32; positions [b, s_q, topk] int32 (row [r, s] belongs to
+      request r), or [n, topk] int32 with cu_seqlens [b + 1] int32 giving the packed rows of
+      each request -> int32 indices of the shape of `positions`
+
+    A negative position, one past the table, one on a page with a negative id, and a row of
+    no request give -1."""
+    _require(block_table.is_cuda, "block_table must be a CUDA tensor")
+    dev = block_table.device
+    _int32_on("block_table", block_table, dev, 2)
+    b, max_pages = block_table.shape
+    _int32_on("positions", positions, dev, 3 if cu_seqlens is None else 2)
+    topk = positions.size(-1)
+    _require(topk <= 1 or positions.stride(-1) == 1, "positions must be dense in the last dim")
+    _require(max_pages <= 1 or block_table.stride(1) == 1, "block_table rows must be dense")
+    _require(1 <= int(page_block) < 2 ** 31, "page_block >= 1 expected")
+    if cu_seqlens is None:
+        _require(positions.size(0) == b, f"positions must be [{b}, s_q, topk]")
+        s_q, n_rows = positions.size(1), b * positions.size(1)
+        flat = positions.reshape(n_rows, topk)           # a view for every dense arrangement
+    else:
+        _int32_on("cu_seqlens", cu_seqlens, dev, 1)
+        _require(cu_seqlens.numel() == b + 1 and cu_seqlens.is_contiguous(), f"cu_seqlens must be contiguous [{b + 1}]")
+        s_q, n_rows, flat = 1, positions.size(0), positions
+    with torch.cuda.device(dev):
+        out = torch.empty(positions.shape, dtype=torch.int32, device=dev)
+        a = N.PageIndicesArgs()
+        a.n_rows, a.topk, a.b, a.s_q = n_rows, topk, b, max(s_q, 1)
+        a.max_pages, a.page_block_size = max_pages, int(page_block)
+        a.block_table, a.positions, a.indices = block_table.data_ptr(), flat.data_ptr(), out.data_ptr()
+        a.cu_seqlens = _ptr(cu_seqlens)
+        a.stride_table = block_table.stride(0)
+        a.stride_positions = flat.stride(0) if n_rows > 1 else topk
+        N.check(N.lib.dsv4_page_indices(C.byref(a), torch.cuda.current_stream(dev).cuda_stream),
+                "dsv4_page_indices")
+    return out
+
+
 def gather_dequant(kv, indices, method: int = 0) -> torch.Tensor:
     """Dequantised BF16 rows [n, d_qk] of the tokens named by int32 `indices` [n]."""
     _require(kv.is_cuda and kv.dim() == 4 and indices.dtype == torch.int32, "bad arguments")

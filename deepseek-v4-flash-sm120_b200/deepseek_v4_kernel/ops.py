@@ -68,3 +68,16 @@ def kv_store_rows(k, loc, kv) -> None:
     row per token (latent then RoPE values, possibly a strided view) and its int32 / int64
     slot mapping."""
     _cuda.kv_store_rows(k, loc, kv)
+
+
+def build_slot_maps(block_table, cached_lens, new_lens, free_pages, page_block, n_slots):
+    """Extend block tables (in place) by the pages of this step's new tokens and map the
+    tokens to cache slots, from request lengths on the device: returns (slots, positions,
+    cu_new, cu_total, n_taken)."""
+    return _cuda.build_slot_maps(block_table, cached_lens, new_lens, free_pages, page_block, n_slots)
+
+
+def page_indices(block_table, positions, page_block, cu_seqlens=None) -> torch.Tensor:
+    """Logical positions (an indexer's top-k lists) -> the physical token indices
+    `sparse_decode_fwd` and the sparse prefills take."""
+    return _cuda.page_indices(block_table, positions, page_block, cu_seqlens)

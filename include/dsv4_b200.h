@@ -301,6 +301,57 @@ typedef struct Dsv4StoreRowsArgs {
 
 int dsv4_kv_store_rows(const Dsv4StoreRowsArgs* args, void* cuda_stream);
 
+/* ---------------------------------------------------------------------------
+ * Block tables and slot maps from request lengths.  No counterpart in the reference
+ * (its serving framework builds them on the host); they produce what dsv4_kv_store and
+ * the attention entries take.
+ *
+ * Request r has cached_lens[r] tokens in the cache and appends new_lens[r] (negative
+ * lengths count as 0).  Its pages that do not exist yet are taken from free_pages, in
+ * request order: with old = ceil(cached / P) and first = the number of pages the requests
+ * before it take, entry j >= old of its table row becomes free_pages[first + j - old].
+ * The new tokens of all requests, packed in request order, get slots[t] = page * P + offset
+ * and positions[t] = their place in the request; t beyond the last new token, and tokens
+ * without a page (free list used up, column >= max_pages, a negative page id), get slot -1,
+ * which the KV stores skip; positions are -1 beyond the last token only.  cu_new /
+ * cu_total are the running sums of new_lens / cached + new; they and the positions
+ * saturate at 2^31 - 1, and
+ * n_taken is the number of pages taken: more than n_free means that the list was too short
+ * (the missing entries are -1).  Tokens behind n_slots are not emitted, but their pages are
+ * taken.  Existing table entries are not written.  b <= 16384.                            */
+typedef struct Dsv4SlotMapArgs {
+  int32_t b, max_pages, page_block_size, n_slots, n_free, reserved;
+  int32_t* block_table;         /* [b, max_pages], updated in place               */
+  const int32_t* cached_lens;   /* [b]                                            */
+  const int32_t* new_lens;      /* [b]                                            */
+  const int32_t* free_pages;    /* [n_free]                                       */
+  int64_t* slots;               /* [n_slots]                                      */
+  int32_t* positions;           /* [n_slots]                                      */
+  int32_t* cu_new;              /* [b + 1]                                        */
+  int32_t* cu_total;            /* [b + 1]                                        */
+  int32_t* n_taken;             /* [1]                                            */
+  int64_t stride_table;         /* elements                                       */
+} Dsv4SlotMapArgs;
+
+int dsv4_build_slot_maps(const Dsv4SlotMapArgs* args, void* cuda_stream);
+
+/* Logical positions -> physical token indices, the form dsv4_sparse_decode and
+ * dsv4_sparse_prefill take: indices[i][j] = block_table[r][pos / P] * P + pos % P for
+ * pos = positions[i][j].  Row i belongs to request r = i / s_q, or, when cu_seqlens
+ * [b + 1] is given, to the request with cu_seqlens[r] <= i < cu_seqlens[r + 1].  The result
+ * is -1 for a negative position, a column >= max_pages, a negative page id, an index that
+ * does not fit int32, and a row of no request.  Rows of indices are dense.                */
+typedef struct Dsv4PageIndicesArgs {
+  int32_t n_rows, topk, b, s_q, max_pages, page_block_size;
+  const int32_t* block_table;   /* [b, max_pages]                                 */
+  const int32_t* positions;     /* [n_rows, topk]                                 */
+  const int32_t* cu_seqlens;    /* [b + 1] or null                                */
+  int32_t* indices;             /* [n_rows, topk]                                 */
+  int64_t stride_table, stride_positions;                /* elements              */
+} Dsv4PageIndicesArgs;
+
+int dsv4_page_indices(const Dsv4PageIndicesArgs* args, void* cuda_stream);
+
 /* ===========================================================================
  * TEST HOOKS.  The three entries marked "test hook" below (dsv4_gather_dequant,
  * dsv4_debug_set_timeline, dsv4_umma_selftest) exist for the test-suite and for
