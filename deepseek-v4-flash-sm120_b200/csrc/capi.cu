@@ -320,6 +320,58 @@ int dsv4_sparse_prefill(const Dsv4PrefillArgs* a, void* stream) {
   return e ? cuda_fail(e) : DSV4_OK;
 }
 
+int dsv4_plan_dense_splits(int t_q, int t_k, int b, int h_q, int h_kv, int num_sms) {
+  if (t_q < 1 || t_k < 1 || b < 1 || h_q < 1 || h_kv < 1 || h_q % h_kv || num_sms < 1) return 1;
+  const int64_t ctas = dsv4::dense_ctas(t_q, b, h_q, h_kv);
+  const int64_t tiles = (static_cast<int64_t>(t_k) / b + 127) / 128;   // of a sequence, on average
+  if (ctas >= num_sms || tiles <= 2) return 1;
+  // In tile times: waves of CTAs, each with its own start and end; joining costs once.
+  const double fixed = 3.0, join = 4.0;
+  int best = 1;
+  double best_cost = 1e30;
+  for (int s = 1; s <= dsv4::DENSE_MAX_SPLITS && s <= tiles; ++s) {
+    const int64_t waves = (ctas * s + num_sms - 1) / num_sms;
+    const double cost = waves * ((tiles + s - 1) / s + fixed) + (s > 1 ? join : 0.0);
+    if (cost < best_cost - 1e-9) { best_cost = cost; best = s; }
+  }
+  return best;
+}
+
+int dsv4_dense_prefill(const Dsv4DensePrefillArgs* a, void* stream) {
+  if (!a) return DSV4_ERR_NULL;
+  if (a->b < 0 || a->t_q < 0 || a->t_k < 0 || a->h_q < 1 || a->h_kv < 1 || a->h_q % a->h_kv ||
+      a->n_splits < 1 || a->n_splits > dsv4::DENSE_MAX_SPLITS || !(a->sm_scale > 0.0f) ||
+      !(a->sm_scale <= 3.0e38f) || dsv4::dense_ctas(a->t_q, a->b, a->h_q, a->h_kv) > 0x7fffffff)
+    return DSV4_ERR_SHAPE;
+  if (!((a->d_qk == 64 && a->d_v == 64) || (a->d_qk == 128 && a->d_v == 128) ||
+        (a->d_qk == 192 && a->d_v == 128)))
+    return DSV4_ERR_LAYOUT;
+  if (a->dtype != DSV4_DTYPE_BF16 && a->dtype != DSV4_DTYPE_FP16) return DSV4_ERR_UNSUPPORTED;
+  if (a->b == 0 || a->t_q == 0) return DSV4_OK;
+  if (!a->q || !a->cu_seqlens_q || !a->cu_seqlens_k || !a->out || !a->max_logits || !a->lse ||
+      (a->t_k && (!a->k || !a->v)))
+    return DSV4_ERR_NULL;
+  struct { const void* p; int64_t t, h; int nt, nh; } views[4] = {
+      {a->q, a->stride_q_t, a->stride_q_h, a->t_q, a->h_q},
+      {a->k, a->stride_k_t, a->stride_k_h, a->t_k, a->h_kv},
+      {a->v, a->stride_v_t, a->stride_v_h, a->t_k, a->h_kv},
+      {a->out, a->stride_o_t, a->stride_o_h, a->t_q, a->h_q}};
+  for (const auto& v : views) {
+    if (v.nt == 0) continue;
+    if (!aligned16(v.p)) return DSV4_ERR_ALIGN;
+    if (v.nt > 1 && (v.t < 1 || (v.t & 7) || v.t >= (1ll << 38))) return DSV4_ERR_ALIGN;
+    if (v.nh > 1 && (v.h < 1 || (v.h & 7) || v.h >= (1ll << 38))) return DSV4_ERR_ALIGN;
+  }
+  if (a->n_splits > 1) {
+    if (!a->o_accum || !a->stat_accum) return DSV4_ERR_SCRATCH;
+    if (!aligned16(a->o_accum) || (reinterpret_cast<uintptr_t>(a->stat_accum) & 7u)) return DSV4_ERR_ALIGN;
+  }
+  int rc = current_device_is_sm100();
+  if (rc) return rc;
+  cudaError_t e = dsv4::launch_dense_prefill(*a, static_cast<cudaStream_t>(stream));
+  return e ? cuda_fail(e) : DSV4_OK;
+}
+
 int dsv4_kv_store(const Dsv4StoreArgs* a, void* stream) {
   if (!a || !a->k_nope || !a->k_rope || !a->slots || !a->kv) return DSV4_ERR_NULL;
   if (a->n_tokens < 0 || a->num_blocks < 1 || a->page_block_size < 1) return DSV4_ERR_SHAPE;
@@ -407,6 +459,9 @@ int dsv4_device_status(int32_t* status_out, int reset) {
   int v = 0;
   cudaError_t e = dsv4::read_attn_error(&v, reset != 0);
   if (e) return cuda_fail(e);
+  int d = 0;
+  if ((e = dsv4::read_dense_error(&d, reset != 0))) return cuda_fail(e);
+  if (v == 0) v = d;
   *status_out = v;
   return DSV4_OK;
 }

@@ -1,0 +1,734 @@
+// Dense causal attention over packed sequences with grouped heads (whole prompts, chunks of
+// prompts behind a cached context, single tokens).
+//
+//   O_i = sum_j p_ij V_j / sum_j p_ij,   p_ij = exp(scale Q_i K_j),   j <= i + len_k - len_q
+//
+// One CTA owns two tiles of 128 query rows of one sequence and one group of heads, and walks
+// the sequence's keys in tiles of 128.  A row is a (token, head) pair: the heads that share a
+// key/value head are packed next to each other, so a single token of a group fills as much of
+// a tile as it can, and a tile spans few tokens (little of it is masked).
+//
+//   S_s [128 rows, 128 keys] = Q_s K^T        A, B from shared memory, K-major
+//   O_s [128 rows, d_v]     += P_s V          A = P from TMEM, B = V, MN-major as it was loaded
+//
+// The two tiles (s = 0, 1) take turns: while the tensor core works for one, a warpgroup of
+// softmax threads works for the other.  A softmax thread owns one row (its TMEM lane), so the
+// maximum and the sum of a row need no exchange; P is written over S in TMEM.  O is rescaled
+// only when a row's maximum has grown by more than 2^8 since its reference was set (the sums
+// are 32-bit and P has as many significant bits at any scale), by the same threads, so there
+// is no correction stage.  Q, K and V arrive by TMA; K's ring is recycled in blocks of 64
+// columns and V's in tiles, which is what the 227 KB allow at d_qk = 192.
+//
+// Masked keys: scores are replaced, not added to, so nothing in a masked key's K row counts.
+// A product with weight zero would still let a NaN or an infinity of a masked V row through,
+// so in the tiles that some row sees only in part two idle warps look over V in shared memory
+// before the tensor core may read it: rows no one sees are cleared, and elements that are not
+// finite are cleared and handed by the epilogue to the rows that do see them.
+//
+// Few rows (single tokens over long contexts): the keys are cut into n_splits ranges, each
+// CTA leaves a normalised 32-bit partial, and dense_combine_kernel joins them.
+#include <cuda.h>
+#include <cuda_fp16.h>
+
+#include <mutex>
+
+#include "attn_params.cuh"
+#include "launchers.h"
+#include "sm100_ptx.cuh"
+
+namespace dsv4 {
+
+__device__ int g_dense_error = 0;
+
+namespace {
+
+using namespace ptx;
+
+constexpr int TILE_M = 128, TILE_N = 128;
+constexpr int BLOCK_BYTES = 128 * 128;               // [128 rows][64 16-bit values], swizzled
+constexpr int SOFTMAX_THREADS = 256;                 // two warpgroups, one per row tile
+constexpr int THREADS = SOFTMAX_THREADS + 128;       // + MMA, TMA and two looking-over warps
+// 384 threads start with 168 registers; the third warpgroup hands most of its own over:
+// 128 * 72 + 256 * 216 = 384 * 168.
+constexpr int LAUNCH_REGS = 168, SOFTMAX_REGS = 216, HELPER_REGS = 72;
+static_assert(SOFTMAX_THREADS * SOFTMAX_REGS + 128 * HELPER_REGS <= THREADS * LAUNCH_REGS,
+              "setmaxnreg.inc can only take what setmaxnreg.dec gave back");
+static_assert(THREADS * (LAUNCH_REGS + 8) > 65536, "LAUNCH_REGS is what the launch bound yields");
+constexpr int WARP_MMA = 8, WARP_TMA = 9, WARP_LOOK = 10;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float RESCALE_THRESHOLD = 8.0f;            // log2 units
+constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_O = 256;   // S_s at 128 s, O_s at 256 + 128 s
+
+enum DenseErr { ERR_Q = 11, ERR_K = 12, ERR_V = 13, ERR_P = 14, ERR_S = 15, ERR_O = 16, ERR_SLOT = 17, ERR_LOOK = 18 };
+
+template <int DQK, int DV> struct DCfg {
+  static constexpr int QB = DQK / 64, VB = DV / 64;
+  static constexpr int K_SLOTS = DQK == 192 ? 4 : DQK == 128 ? 6 : 4;   // blocks of 64 columns
+  static constexpr int V_UNITS = DQK == 64 ? 4 : 2;                     // whole tiles
+  static constexpr int Q_BYTES = 2 * QB * BLOCK_BYTES, K_BYTES = K_SLOTS * BLOCK_BYTES;
+  static constexpr int V_UNIT_BYTES = VB * BLOCK_BYTES, V_BYTES = V_UNITS * V_UNIT_BYTES;
+};
+
+struct DenseCtrl {
+  uint64_t q_full[2], s_full[2], p_full[2], o_done[2];
+  uint64_t k_full[6], k_empty[6], v_full[4], v_empty[4];
+  // tiles that are looked over (the last ones) land on v_look instead of v_full, so that the
+  // looking warps count only their own phases; v_clean hands them on
+  uint64_t v_look[4], v_clean[4];
+  uint32_t tmem;
+  int fail, bad;
+};
+
+template <int DQK, int DV> constexpr size_t dense_smem_bytes() {
+  using C = DCfg<DQK, DV>;
+  return 1024 + C::Q_BYTES + C::K_BYTES + C::V_BYTES + sizeof(DenseCtrl);
+}
+static_assert(dense_smem_bytes<192, 128>() <= 232448 && dense_smem_bytes<128, 128>() <= 232448, "227 KB a CTA");
+
+struct DenseParams {
+  CUtensorMap mq, mk, mv;
+  int b, t_q, t_k, h_q, h_kv, causal;
+  int pack, tok_tile;            // heads packed per row tile, tokens per row tile
+  int chunks;                    // head chunks: h_q / pack
+  int slots;                     // row-tile pairs, upper bound over all sequences
+  int n_splits;
+  float sm_scale;
+  const int32_t *cu_q, *cu_k;
+  const float* sink;
+  const void* v;
+  int64_t stride_v_t, stride_v_h, stride_o_t, stride_o_h, stride_ml_t, stride_lse_t;
+  void* out;
+  float *max_logits, *lse;
+  float *o_accum, *stat_accum;   // [split][t][h][d_v], [split][t][h][2] (max logit, log-sum-exp)
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (BF16) {
+    __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&t);
+  } else {
+    __half2 t = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&t);
+  }
+}
+// Which halves of a word are infinite or NaN (bits 15 and 31).
+template <bool BF16>
+__device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
+  return BF16 ? ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u
+              : ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+}
+
+// The part of a sequence that a CTA works on.
+struct Work {
+  int q0, len_q, k0, len_k;      // rows of the packed tensors
+  int t0;                        // first query token of row tile 0, in the sequence
+  int first, count[2];           // key tiles: [first, first + count[s])
+  int look;                      // key tiles from this one on are seen only in part by some row
+  bool any;
+};
+
+// Keys of the sequence that token t sees: [0, reach).
+__device__ __forceinline__ int reach_of(const DenseParams& p, const Work& w, int t) {
+  if (!p.causal) return w.len_k;
+  const int r = t + w.len_k - w.len_q + 1;
+  return r < 0 ? 0 : r < w.len_k ? r : w.len_k;
+}
+
+__device__ __forceinline__ int clamp_to(int v, int lo, int hi) { return min(max(v, lo), hi); }
+
+__device__ __forceinline__ Work find_work(const DenseParams& p, int slot, int split) {
+  Work w;
+  // Sequence s owns the slots from cu_q[s] / span + s on: at least ceil(len / span) of them.
+  const int span = 2 * p.tok_tile;
+  int lo = 0, hi = p.b;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (clamp_to(__ldg(p.cu_q + mid), 0, p.t_q) / span + mid <= slot) lo = mid; else hi = mid;
+  }
+  w.q0 = clamp_to(__ldg(p.cu_q + lo), 0, p.t_q);
+  w.len_q = clamp_to(__ldg(p.cu_q + lo + 1), w.q0, p.t_q) - w.q0;
+  w.k0 = clamp_to(__ldg(p.cu_k + lo), 0, p.t_k);
+  w.len_k = clamp_to(__ldg(p.cu_k + lo + 1), w.k0, p.t_k) - w.k0;
+  const int64_t t0 = static_cast<int64_t>(slot - (w.q0 / span + lo)) * span;
+  w.any = t0 >= 0 && t0 < w.len_q;
+  w.t0 = static_cast<int>(w.any ? t0 : 0);
+  int tiles[2] = {0, 0};
+  if (w.any) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int a = w.t0 + s * p.tok_tile;
+      if (a < w.len_q)
+        tiles[s] = (reach_of(p, w, min(a + p.tok_tile, w.len_q) - 1) + TILE_N - 1) / TILE_N;
+    }
+  }
+  const int total = max(tiles[0], tiles[1]);
+  const int per = (total + p.n_splits - 1) / p.n_splits;
+  w.first = min(split * per, total);
+  const int end = min(w.first + per, total);
+#pragma unroll
+  for (int s = 0; s < 2; ++s) w.count[s] = max(min(tiles[s], end) - w.first, 0);
+  w.look = reach_of(p, w, w.t0) / TILE_N;
+  return w;
+}
+
+// Where a row's results go, and its final factor.
+template <int DV, bool BF16>
+__device__ __forceinline__ void store_stats(const DenseParams& p, int split, int64_t t, int h, float m_raw, float m_ref,
+                                            float l, bool fail, float& factor) {
+  // m_ref: reference in log2 units (-inf: nothing seen); l: sum relative to it
+  const bool none = l == 0.f;                  // (a sum of NaN scores is not zero: it shows)
+  const float lse = none ? -INFINITY : logf(l) + m_ref * LN2;
+  const float ml = none ? -INFINITY : m_raw * p.sm_scale;
+  factor = none ? 0.f : 1.f / l;
+  if (p.n_splits > 1) {
+    float2* dst = reinterpret_cast<float2*>(p.stat_accum + ((static_cast<int64_t>(split) * p.t_q + t) * p.h_q + h) * 2);
+    *dst = make_float2(ml, fail ? NAN : lse);
+    return;
+  }
+  if (p.sink != nullptr && !none) factor *= 1.f / (1.f + expf(p.sink[h] - lse));
+  p.max_logits[t * p.stride_ml_t + h] = ml;
+  p.lse[t * p.stride_lse_t + h] = fail ? NAN : none ? INFINITY : lse;
+}
+
+template <int DQK, int DV, bool BF16>
+__global__ void __launch_bounds__(THREADS, 1)
+dense_attn_kernel(const __grid_constant__ DenseParams p) {
+  using C = DCfg<DQK, DV>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  const uint32_t sQ = base, sK = sQ + C::Q_BYTES, sV = sK + C::K_BYTES;
+  DenseCtrl& ctrl = *reinterpret_cast<DenseCtrl*>(smem_raw + (base - raw) + C::Q_BYTES + C::K_BYTES + C::V_BYTES);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  grid_dependency_wait();
+  // Slots last to first: in a causal sequence the late rows are the long ones.
+  const int chunk = blockIdx.x % p.chunks;
+  const int slot = p.slots - 1 - static_cast<int>(blockIdx.x / p.chunks);
+  const int split = blockIdx.z;
+  const Work w = find_work(p, slot, split);
+  if (!w.any) return;
+  const int head0 = chunk * p.pack;
+  const int kvh = head0 / (p.h_q / p.h_kv);
+  const int n_tiles = max(w.count[0], w.count[1]);
+
+  if (n_tiles == 0) {                     // nothing in this CTA's range: results of empty rows
+    const int rows = 2 * p.tok_tile * p.pack;
+    for (int i = tid; i < rows; i += THREADS) {
+      const int tok = w.t0 + i / p.pack, h = head0 + i % p.pack;
+      if (tok >= w.len_q) continue;
+      const int64_t t = w.q0 + tok;
+      float f;
+      store_stats<DV, BF16>(p, split, t, h, -INFINITY, -INFINITY, 0.f, false, f);
+      if (p.n_splits > 1) {
+        float4* d = reinterpret_cast<float4*>(p.o_accum + ((static_cast<int64_t>(split) * p.t_q + t) * p.h_q + h) * DV);
+        for (int c = 0; c < DV / 4; ++c) d[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+      } else {
+        uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + t * p.stride_o_t + h * p.stride_o_h);
+        for (int c = 0; c < DV / 8; ++c) d[c] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    return;
+  }
+
+  auto bar = [&](uint64_t* x) { return smem_u32(x); };
+  if (warp == WARP_MMA) {
+    if (lane == 0) {
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(bar(&ctrl.q_full[s]), 1);
+        mbar_init(bar(&ctrl.s_full[s]), 1);
+        mbar_init(bar(&ctrl.p_full[s]), 4);
+        mbar_init(bar(&ctrl.o_done[s]), 1);
+      }
+      for (int i = 0; i < 6; ++i) {
+        mbar_init(bar(&ctrl.k_full[i]), 1);
+        mbar_init(bar(&ctrl.k_empty[i]), 1);
+      }
+      for (int i = 0; i < 4; ++i) {
+        mbar_init(bar(&ctrl.v_full[i]), 1);
+        mbar_init(bar(&ctrl.v_empty[i]), 1);
+        mbar_init(bar(&ctrl.v_look[i]), 1);
+        mbar_init(bar(&ctrl.v_clean[i]), 2);
+      }
+      ctrl.fail = 0;
+      ctrl.bad = 0;
+      mbar_init_fence();
+    }
+    __syncwarp();
+    tmem_alloc(smem_u32(&ctrl.tmem), TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = ctrl.tmem;
+  // A role whose bounded wait gives up records it and ends; the others then run into their
+  // own limits, long after every copy and product in flight has finished.
+  auto gave_up = [&](int code) {
+    atomicExch(&g_dense_error, code);
+    *reinterpret_cast<volatile int*>(&ctrl.fail) = 1;
+  };
+
+  if (warp >= WARP_MMA) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(HELPER_REGS));
+    if (warp == WARP_TMA) {
+      // ======================= loads ======================================================
+      if (elect_one()) {
+        const uint32_t q_bytes = static_cast<uint32_t>(p.pack * p.tok_tile) * 128u;
+        auto load_q = [&](int s) {
+          mbar_expect_tx(bar(&ctrl.q_full[s]), q_bytes * C::QB);
+          for (int c = 0; c < C::QB; ++c)
+            tma_load_3d(sQ + (s * C::QB + c) * BLOCK_BYTES, &p.mq, 64 * c, head0,
+                        w.q0 + w.t0 + s * p.tok_tile, bar(&ctrl.q_full[s]));
+        };
+        if (w.count[0] > 0) load_q(0);
+        bool ok = true;
+        int ks = 0, kphase = 0, vu = 0, vphase = 0;
+        for (int i = 0; i < n_tiles && ok; ++i) {
+          const int row = w.k0 + (w.first + i) * TILE_N;
+          for (int c = 0; c < C::QB && ok; ++c) {
+            if (!mbar_wait(bar(&ctrl.k_empty[ks]), kphase ^ 1)) { gave_up(ERR_SLOT); ok = false; break; }
+            mbar_expect_tx(bar(&ctrl.k_full[ks]), BLOCK_BYTES);
+            tma_load_3d(sK + ks * BLOCK_BYTES, &p.mk, 64 * c, kvh, row, bar(&ctrl.k_full[ks]));
+            if (++ks == C::K_SLOTS) { ks = 0; kphase ^= 1; }
+          }
+          if (i == 0 && w.count[1] > 0) load_q(1);
+          if (!ok || !mbar_wait(bar(&ctrl.v_empty[vu]), vphase ^ 1)) { gave_up(ERR_SLOT); break; }
+          const uint32_t landed = bar(w.first + i >= w.look ? &ctrl.v_look[vu] : &ctrl.v_full[vu]);
+          mbar_expect_tx(landed, C::V_UNIT_BYTES);
+          for (int c = 0; c < C::VB; ++c)
+            tma_load_3d(sV + vu * C::V_UNIT_BYTES + c * BLOCK_BYTES, &p.mv, 64 * c, kvh, row, landed);
+          if (++vu == C::V_UNITS) { vu = 0; vphase ^= 1; }
+        }
+      }
+      __syncwarp();
+    } else if (warp == WARP_MMA) {
+      // ======================= products ===================================================
+      const uint32_t idesc_qk = make_idesc_16(BF16, TILE_M, TILE_N, 0, 0);
+      const uint32_t idesc_pv = make_idesc_16(BF16, TILE_M, DV, 0, 1);
+      const uint64_t dQ = make_smem_desc(sQ, 16, 1024, SWZ_128B);
+      const uint64_t dK = make_smem_desc(sK, 16, 1024, SWZ_128B);
+      const uint64_t dV = make_smem_desc(sV, BLOCK_BYTES, 1024, SWZ_128B);   // MN-major
+      const uint32_t elected = elect_one();
+      bool ok = true;
+      uint32_t clean_parity = 0;
+      auto wait = [&](uint64_t* b, int parity, int code) {
+        if (ok && !mbar_wait_warp(bar(b), parity, lane)) {
+          if (lane == 0) gave_up(code);
+          ok = false;
+        }
+      };
+      // S_s of key tile i; `last`: nobody reads the tile's K after this product.
+      auto scores = [&](int s, int i, bool last) {
+        int idx = i * C::QB;
+        int ks = idx % C::K_SLOTS, kphase = (idx / C::K_SLOTS) & 1;
+        if (i == 0) wait(&ctrl.q_full[s], 0, ERR_Q);
+#pragma unroll
+        for (int c = 0; c < C::QB; ++c) {
+          wait(&ctrl.k_full[ks], kphase, ERR_K);
+          if (!ok) return;
+          tc_fence_after_sync();
+#pragma unroll
+          for (int k4 = 0; k4 < 4; ++k4)
+            umma_bf16_elect(tmem + COL_S + 128 * s, dQ + (((s * C::QB + c) * BLOCK_BYTES + k4 * 32) >> 4),
+                            dK + ((ks * BLOCK_BYTES + k4 * 32) >> 4), idesc_qk, (c | k4) != 0, elected);
+          if (last) umma_commit_elect(bar(&ctrl.k_empty[ks]), elected);
+          if (++ks == C::K_SLOTS) { ks = 0; kphase ^= 1; }
+        }
+        umma_commit_elect(bar(&ctrl.s_full[s]), elected);
+      };
+      for (int s = 0; s < 2; ++s)
+        if (w.count[s] > 0 && ok) scores(s, 0, s == 1 || w.count[1] <= 0);
+#pragma unroll 1
+      for (int i = 0; i < n_tiles && ok; ++i) {
+        const int vu = i % C::V_UNITS, vphase = (i / C::V_UNITS) & 1;
+        bool have_v = false;
+#pragma unroll 1
+        for (int s = 0; s < 2 && ok; ++s) {
+          if (i >= w.count[s]) continue;
+          wait(&ctrl.p_full[s], i & 1, ERR_P);
+          if (!have_v) {
+            have_v = true;
+            if (w.first + i >= w.look) {
+              wait(&ctrl.v_clean[vu], (clean_parity >> vu) & 1, ERR_LOOK);
+              clean_parity ^= 1u << vu;
+            } else {
+              wait(&ctrl.v_full[vu], vphase, ERR_V);
+            }
+          }
+          if (!ok) break;
+          tc_fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < TILE_N / 16; ++k)
+            umma_ts_elect(tmem + COL_O + 128 * s, tmem + COL_S + 128 * s + 8 * k,
+                          dV + ((vu * C::V_UNIT_BYTES + k * 2048) >> 4), idesc_pv, (i | k) != 0, elected);
+          umma_commit_elect(bar(&ctrl.o_done[s]), elected);
+          if (s == 1 || i >= w.count[1]) umma_commit_elect(bar(&ctrl.v_empty[vu]), elected);
+          if (i + 1 < w.count[s]) scores(s, i + 1, s == 1 || i + 1 >= w.count[1]);
+        }
+      }
+    } else {
+      // ======================= looking over V =============================================
+      const int t2 = (warp - WARP_LOOK) * 32 + lane;
+      // keys the whole CTA sees (its last row sees the most)
+      const int seen = reach_of(p, w, min(w.t0 + 2 * p.tok_tile, w.len_q) - 1);
+      uint32_t parity = 0;
+      for (int i = max(w.look - w.first, 0); i < n_tiles; ++i) {
+        const int vu = i % C::V_UNITS;
+        if (!mbar_wait_warp(bar(&ctrl.v_look[vu]), (parity >> vu) & 1, lane)) {
+          if (lane == 0) gave_up(ERR_V);
+          break;
+        }
+        parity ^= 1u << vu;
+        const int live = min(seen - (w.first + i) * TILE_N, TILE_N);   // rows of the tile that count
+        uint32_t found = 0;
+        for (int c = t2; c < C::V_UNIT_BYTES / 16; c += 64) {
+          const uint32_t addr = sV + vu * C::V_UNIT_BYTES + c * 16;
+          const int row = (c >> 3) & 127;
+          uint32_t x[4];
+          if (row >= live) {
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory");
+            continue;
+          }
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(addr) : "memory");
+          uint32_t f = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) f |= not_finite2<BF16>(x[k]);
+          if (f) {
+            found = 1;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t h = not_finite2<BF16>(x[k]);
+              if (h & 0x8000u) x[k] &= 0xffff0000u;
+              if (h & 0x80000000u) x[k] &= 0x0000ffffu;
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                         ::"r"(addr), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+          }
+        }
+        if (found) *reinterpret_cast<volatile int*>(&ctrl.bad) = 1;
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(&ctrl.v_clean[vu]));
+      }
+    }
+    grid_launch_dependents();
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    if (warp == WARP_MMA) tmem_dealloc(tmem, TMEM_COLS);
+    return;
+  }
+
+  // ======================= softmax ======================================================
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
+  const int s = warp >> 2;
+  const int row = (warp & 3) * 32 + lane;
+  const int tok = w.t0 + s * p.tok_tile + row / p.pack;
+  const int h = head0 + row % p.pack;
+  const bool live = row < p.pack * p.tok_tile && tok < w.len_q;
+  const int reach = live ? reach_of(p, w, tok) : 0;
+  const int n_mine = w.count[s];
+  const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+  const uint32_t tS = tmem + lanes + COL_S + 128 * s, tO = tmem + lanes + COL_O + 128 * s;
+  const float c = p.sm_scale * LOG2E;
+  // tiles below this one are seen whole by every row of this tile that exists
+  const int whole = reach_of(p, w, w.t0 + s * p.tok_tile) / TILE_N;
+
+  float m_ref = -INFINITY, m_raw = -INFINITY, l = 0.f;
+  bool ok = true;
+#pragma unroll 1
+  for (int i = 0; i < n_mine; ++i) {
+    if (!mbar_wait(bar(&ctrl.s_full[s]), i & 1)) { gave_up(ERR_S); ok = false; break; }
+    tc_fence_after_sync();
+    uint32_t x[TILE_N];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) tmem_ld32(tS + 32 * k, x + 32 * k);
+    tmem_ld_wait();
+    if (w.first + i >= whole) {
+      const int see = reach - (w.first + i) * TILE_N;
+#pragma unroll
+      for (int k = 0; k < TILE_N; ++k) x[k] = k < see ? x[k] : 0xff800000u;
+    }
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int k = 0; k < TILE_N; ++k) mx[k & 3] = fmaxf(mx[k & 3], __uint_as_float(x[k]));
+    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+    m_raw = fmaxf(m_raw, top);
+    const float top2 = top * c;
+    const bool raise = top2 > m_ref + RESCALE_THRESHOLD;       // also the first finite one
+    float alpha = 1.f;
+    if (raise) {
+      alpha = ex2(m_ref - top2);                               // 0 for the first
+      m_ref = top2;
+      l *= alpha;
+    }
+    if (i > 0 && __any_sync(0xffffffffu, raise)) {
+      if (!mbar_wait(bar(&ctrl.o_done[s]), (i - 1) & 1)) { gave_up(ERR_O); ok = false; break; }
+      tc_fence_after_sync();
+#pragma unroll 1
+      for (int k = 0; k < DV / 16; ++k) {
+        uint32_t o[16];
+        tmem_ld16(tO + 16 * k, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int q = 0; q < 16; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * alpha);
+        tmem_st16(tO + 16 * k, o);
+      }
+    }
+    const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      uint32_t pk[32];
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const float a = ex2(fmaf(__uint_as_float(x[64 * q + 2 * k]), c, -ref));
+        const float b = ex2(fmaf(__uint_as_float(x[64 * q + 2 * k + 1]), c, -ref));
+        sum[(2 * k) & 3] += a;
+        sum[(2 * k + 1) & 3] += b;
+        pk[k] = pack2<BF16>(a, b);
+      }
+      tmem_st32(tS + 32 * q, pk);
+    }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    tmem_st_wait();
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(&ctrl.p_full[s]));
+  }
+  grid_launch_dependents();
+
+  // ---- epilogue --------------------------------------------------------------------------
+  if (n_mine > 0 && ok && !mbar_wait(bar(&ctrl.o_done[s]), (n_mine - 1) & 1)) { gave_up(ERR_O); ok = false; }
+  tc_fence_after_sync();
+  const bool fail = !ok || *reinterpret_cast<volatile int*>(&ctrl.fail) != 0;
+  const int64_t t = static_cast<int64_t>(w.q0) + tok;
+  float factor = 0.f;
+  if (live) store_stats<DV, BF16>(p, split, t, h, m_raw, m_ref, l, fail, factor);
+  const bool bad = *reinterpret_cast<volatile int*>(&ctrl.bad) != 0;
+  const int64_t acc = ((static_cast<int64_t>(split) * p.t_q + t) * p.h_q + h) * DV;
+#pragma unroll 1
+  for (int k = 0; k < DV / 32; ++k) {
+    uint32_t o[32];
+    if (n_mine > 0) {
+      tmem_ld32(tO + 32 * k, o);                               // warp-collective
+      tmem_ld_wait();
+    }
+    float f[32];
+#pragma unroll
+    for (int q = 0; q < 32; ++q) f[q] = factor == 0.f && l == 0.f ? 0.f : __uint_as_float(o[q]) * factor;
+    if (bad && live) {
+      // the values that were cleared, for the rows that see them: their weight is positive,
+      // so an infinity stays one (and two of both signs, or a NaN, make a NaN)
+      const int from = max(w.look, w.first) * TILE_N, to = min(reach, (w.first + n_mine) * TILE_N);
+      for (int j = from; j < to; ++j) {
+        const uint16_t* vr = static_cast<const uint16_t*>(p.v) + (w.k0 + j) * p.stride_v_t + kvh * p.stride_v_h + 32 * k;
+#pragma unroll
+        for (int q = 0; q < 32; ++q) {
+          const uint32_t u = vr[q];
+          if (not_finite2<BF16>(u) & 0x8000u) {
+            if constexpr (BF16) f[q] += __uint_as_float(u << 16);
+            else f[q] += __half2float(__ushort_as_half(static_cast<unsigned short>(u)));
+          }
+        }
+      }
+    }
+    if (!live || fail) continue;
+    if (p.n_splits > 1) {
+      float4* d = reinterpret_cast<float4*>(p.o_accum + acc + 32 * k);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) d[q] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
+    } else {
+      uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + t * p.stride_o_t + h * p.stride_o_h + 32 * k);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        d[q] = make_uint4(pack2<BF16>(f[8 * q], f[8 * q + 1]), pack2<BF16>(f[8 * q + 2], f[8 * q + 3]),
+                          pack2<BF16>(f[8 * q + 4], f[8 * q + 5]), pack2<BF16>(f[8 * q + 6], f[8 * q + 7]));
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+}
+
+// Joins the partials of the key ranges: one warp per (token, head), in range order.
+template <int DV, bool BF16>
+__global__ void __launch_bounds__(256)
+dense_combine_kernel(const __grid_constant__ DenseParams p) {
+  constexpr int PER = DV / 32;
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (item >= static_cast<int64_t>(p.t_q) * p.h_q) return;
+  const int64_t t = item / p.h_q;
+  const int h = static_cast<int>(item - t * p.h_q);
+  if (t < __ldg(p.cu_q) || t >= __ldg(p.cu_q + p.b)) return;   // a row of no sequence stays as it is
+  float ml = -INFINITY, top = -INFINITY;
+  for (int s = 0; s < p.n_splits; ++s) {
+    const float2 v = *reinterpret_cast<const float2*>(p.stat_accum + ((static_cast<int64_t>(s) * p.t_q + t) * p.h_q + h) * 2);
+    ml = fmaxf(ml, v.x);
+    top = (v.y != v.y || top != top) ? NAN : fmaxf(top, v.y);  // a failed part shows
+  }
+  float acc[PER], sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) acc[k] = 0.f;
+  if (top != -INFINITY) {
+    for (int s = 0; s < p.n_splits; ++s) {
+      const int64_t at = (static_cast<int64_t>(s) * p.t_q + t) * p.h_q + h;
+      const float e = p.stat_accum[at * 2 + 1];
+      if (e == -INFINITY) continue;
+      const float wgt = expf(e - top);
+      sum += wgt;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) acc[k] = fmaf(wgt, p.o_accum[at * DV + lane * PER + k], acc[k]);
+    }
+  }
+  const bool none = top == -INFINITY;
+  const float lse = none ? -INFINITY : top + logf(sum);
+  float f = none ? 0.f : 1.f / sum;
+  if (p.sink != nullptr && !none) f *= 1.f / (1.f + expf(p.sink[h] - lse));
+  uint32_t* d = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + t * p.stride_o_t + h * p.stride_o_h + lane * PER);
+#pragma unroll
+  for (int k = 0; k < PER / 2; ++k) d[k] = pack2<BF16>(acc[2 * k] * f, acc[2 * k + 1] * f);
+  if (lane == 0) {
+    p.max_logits[t * p.stride_ml_t + h] = ml;
+    p.lse[t * p.stride_lse_t + h] = none ? INFINITY : lse;
+  }
+}
+
+constexpr int MAX_DEVICES = 64;
+std::mutex g_dense_mu;
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's tensor-map encoder, looked up once (the library links no driver library).
+cudaError_t encoder(EncodeTiled* out) {
+  std::lock_guard<std::mutex> lk(g_dense_mu);
+  static EncodeTiled fn = nullptr;
+  if (fn == nullptr) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult st;
+    cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &st);
+    if (e) return e;
+    if (st != cudaDriverEntryPointSuccess || f == nullptr) return cudaErrorNotSupported;
+    fn = reinterpret_cast<EncodeTiled>(f);
+  }
+  *out = fn;
+  return cudaSuccess;
+}
+
+// Map of a [tokens, heads, d] tensor of 16-bit values with boxes of `box_t` tokens, `box_h`
+// heads and 64 values.
+cudaError_t make_map(CUtensorMap* m, bool bf16, const void* ptr, int tokens, int heads, int d, int64_t stride_t,
+                     int64_t stride_h, int box_t, int box_h) {
+  EncodeTiled enc;
+  cudaError_t e = encoder(&enc);
+  if (e) return e;
+  // the stride of a dimension of one element is never used, but has to be a legal one
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(heads > 1 ? stride_h : d) * 2,
+                                 static_cast<cuuint64_t>(tokens > 1 ? stride_t : d) * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_h), static_cast<cuuint32_t>(box_t)};
+  const cuuint32_t ones[3] = {1, 1, 1};
+  const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                         const_cast<void*>(ptr), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+template <int DQK, int DV, bool BF16>
+cudaError_t launch_one(const DenseParams& p, cudaStream_t st) {
+  constexpr size_t smem = dense_smem_bytes<DQK, DV>();
+  static bool configured[MAX_DEVICES] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e) return e;
+  if (dev < 0 || dev >= MAX_DEVICES) return cudaErrorInvalidDevice;
+  {
+    std::lock_guard<std::mutex> lk(g_dense_mu);
+    if (!configured[dev]) {
+      e = cudaFuncSetAttribute(dense_attn_kernel<DQK, DV, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(smem));
+      if (e) return e;
+      configured[dev] = true;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.slots) * p.chunks, 1, p.n_splits);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  cfg.attrs = attr;
+  cfg.numAttrs = add_overlap_attribute(attr);
+  if ((e = cudaLaunchKernelEx(&cfg, dense_attn_kernel<DQK, DV, BF16>, p))) return e;
+  if (p.n_splits == 1) return cudaSuccess;
+  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.t_q) * p.h_q + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, dense_combine_kernel<DV, BF16>, p);
+}
+
+// Heads packed into a row tile: the most heads of a group that divide it and fit.
+int pack_of(int group) {
+  for (int v = group < TILE_M ? group : TILE_M; v > 1; --v)
+    if (group % v == 0) return v;
+  return 1;
+}
+
+}  // namespace
+
+int64_t dense_ctas(int t_q, int b, int h_q, int h_kv) {
+  const int pack = pack_of(h_q / h_kv);
+  return (static_cast<int64_t>(t_q) / (2 * (TILE_M / pack)) + b) * (h_q / pack);
+}
+
+cudaError_t launch_dense_prefill(const Dsv4DensePrefillArgs& a, cudaStream_t st) {
+  DenseParams p;
+  const bool bf16 = a.dtype == DSV4_DTYPE_BF16;
+  p.b = a.b; p.t_q = a.t_q; p.t_k = a.t_k; p.h_q = a.h_q; p.h_kv = a.h_kv; p.causal = a.causal;
+  p.pack = pack_of(a.h_q / a.h_kv);
+  p.tok_tile = TILE_M / p.pack;
+  p.chunks = a.h_q / p.pack;
+  p.slots = a.t_q / (2 * p.tok_tile) + a.b;
+  p.n_splits = a.n_splits;
+  p.sm_scale = a.sm_scale;
+  p.cu_q = a.cu_seqlens_q; p.cu_k = a.cu_seqlens_k; p.sink = a.attn_sink;
+  p.v = a.v; p.stride_v_t = a.stride_v_t; p.stride_v_h = a.stride_v_h;
+  p.out = a.out; p.max_logits = a.max_logits; p.lse = a.lse;
+  p.stride_o_t = a.stride_o_t; p.stride_o_h = a.stride_o_h;
+  p.stride_ml_t = a.stride_ml_t; p.stride_lse_t = a.stride_lse_t;
+  p.o_accum = a.o_accum; p.stat_accum = a.stat_accum;
+  cudaError_t e;
+  if ((e = make_map(&p.mq, bf16, a.q, a.t_q, a.h_q, a.d_qk, a.stride_q_t, a.stride_q_h, p.tok_tile, p.pack))) return e;
+  // a batch without any key still needs legal maps: nothing is loaded through them
+  const bool keys = a.t_k > 0;
+  if ((e = make_map(&p.mk, bf16, keys ? a.k : a.q, keys ? a.t_k : 1, keys ? a.h_kv : 1, a.d_qk,
+                    a.stride_k_t, a.stride_k_h, TILE_N, 1))) return e;
+  if ((e = make_map(&p.mv, bf16, keys ? a.v : a.q, keys ? a.t_k : 1, keys ? a.h_kv : 1, a.d_v,
+                    a.stride_v_t, a.stride_v_h, TILE_N, 1))) return e;
+  if (a.d_qk == 192) return bf16 ? launch_one<192, 128, true>(p, st) : launch_one<192, 128, false>(p, st);
+  if (a.d_qk == 128) return bf16 ? launch_one<128, 128, true>(p, st) : launch_one<128, 128, false>(p, st);
+  return bf16 ? launch_one<64, 64, true>(p, st) : launch_one<64, 64, false>(p, st);
+}
+
+cudaError_t read_dense_error(int* value, bool reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(value, g_dense_error, sizeof(int));
+  if (e) return e;
+  if (reset && *value) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_dense_error, &zero, sizeof(int));
+  }
+  return e;
+}
+
+}  // namespace dsv4

@@ -42,6 +42,12 @@ constexpr int SLOT_MAP_MAX_REQUESTS = 16384;     // both sums of a request list 
 cudaError_t launch_slot_maps(const Dsv4SlotMapArgs& a, cudaStream_t st);
 cudaError_t launch_page_indices(const Dsv4PageIndicesArgs& a, cudaStream_t st);
 
+// Dense attention over packed sequences (dense_attn_sm100.cu).
+constexpr int DENSE_MAX_SPLITS = 64;
+int64_t dense_ctas(int t_q, int b, int h_q, int h_kv);      // CTAs of one key range, at most
+cudaError_t launch_dense_prefill(const Dsv4DensePrefillArgs& a, cudaStream_t st);
+cudaError_t read_dense_error(int* value, bool reset);
+
 // tcgen05 kernels (sparse_attn_sm100.cu).  `supported` reports whether the
 // tensor-core kernel handles this (format, d_qk) pair.
 bool sm100_attn_supported(int kv_format, int d_qk);

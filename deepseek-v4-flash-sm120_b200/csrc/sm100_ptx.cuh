@@ -79,6 +79,20 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, in
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
+// ---- TMA ------------------------------------------------------------------
+// Expect `bytes` of asynchronous copies on `bar` and arrive on it once.
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// One box of a 3-D tensor into this CTA's shared memory.  x times the element size must be a
+// multiple of 16 bytes; what lies outside the tensor reads as zero and counts as copied.
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+
 // ---- fences ---------------------------------------------------------------
 // Generic-proxy shared-memory writes -> visible to the async proxy (tcgen05.mma).
 __device__ __forceinline__ void fence_async_smem() {
@@ -179,6 +193,19 @@ __device__ __forceinline__ void umma_commit(uint32_t bar) {
                ::"r"(bar) : "memory");
 }
 
+// The same product with A taken from TMEM (row = lane, two consecutive 16-bit contraction
+// elements per 32-bit column) and only B from shared memory.
+__device__ __forceinline__ void umma_ts_elect(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b,
+                                              uint32_t idesc, uint32_t accumulate, uint32_t elected) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+
 // Instruction descriptor, kind::f16, BF16 x BF16 -> fp32, dense.
 // bits: [4,6) D format (1 = f32); [7,10) A format (1 = bf16); [10,13) B format;
 // [15] A major (0 = K, 1 = MN); [16] B major; [17,23) N >> 3; [24,29) M >> 4.
@@ -186,6 +213,11 @@ __host__ __device__ constexpr uint32_t make_idesc_bf16(int m, int n, int a_mn, i
   return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(a_mn) << 15) |
          (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// The same for FP16 x FP16 (format 0) or BF16 x BF16 operands.
+__host__ __device__ constexpr uint32_t make_idesc_16(bool bf16, int m, int n, int a_mn, int b_mn) {
+  return make_idesc_bf16(m, n, a_mn, b_mn) & (bf16 ? ~0u : ~((1u << 7) | (1u << 10)));
 }
 
 // Shared-memory matrix descriptor.  Fields (all byte quantities >> 4):
@@ -222,6 +254,28 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         "=r"(r[14]), "=r"(r[15])
       : "r"(taddr) : "memory");
 }
+// 32 consecutive columns.
+#define DSV4_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), \
+    "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define DSV4_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), \
+    "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : DSV4_R8(r, 0), DSV4_R8(r, 8), DSV4_R8(r, 16), DSV4_R8(r, 24)
+      : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+      ::DSV4_W8(r, 0), DSV4_W8(r, 8), DSV4_W8(r, 16), DSV4_W8(r, 24), "r"(taddr) : "memory");
+}
+#undef DSV4_R8
+#undef DSV4_W8
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "

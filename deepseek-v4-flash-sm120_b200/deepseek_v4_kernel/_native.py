@@ -85,6 +85,18 @@ class PageIndicesArgs(C.Structure):
         (n, i64) for n in ("stride_table", "stride_positions")]
 
 
+DTYPE_BF16, DTYPE_FP16 = 0, 1
+
+
+class DensePrefillArgs(C.Structure):
+    _fields_ = [(n, i32) for n in ("b", "t_q", "t_k", "h_q", "h_kv", "d_qk", "d_v", "dtype", "causal",
+                                   "n_splits")] + [("sm_scale", f32), ("reserved", i32)] + [
+        (n, vp) for n in ("q", "k", "v", "cu_seqlens_q", "cu_seqlens_k", "attn_sink", "out",
+                          "max_logits", "lse", "o_accum", "stat_accum")] + [
+        (n, i64) for n in ("stride_q_t", "stride_q_h", "stride_k_t", "stride_k_h", "stride_v_t",
+                           "stride_v_h", "stride_o_t", "stride_o_h", "stride_ml_t", "stride_lse_t")]
+
+
 # name -> (restype, argtypes); every symbol include/dsv4_b200.h declares.
 SYMBOLS = {
     "dsv4_abi_version": (C.c_int, []),
@@ -102,6 +114,8 @@ SYMBOLS = {
     "dsv4_sparse_prefill": (C.c_int, [C.POINTER(PrefillArgs), vp]),
     "dsv4_kv_store": (C.c_int, [C.POINTER(StoreArgs), vp]),
     "dsv4_kv_store_rows": (C.c_int, [C.POINTER(StoreRowsArgs), vp]),
+    "dsv4_dense_prefill": (C.c_int, [C.POINTER(DensePrefillArgs), vp]),
+    "dsv4_plan_dense_splits": (C.c_int, [C.c_int] * 6),
     "dsv4_build_slot_maps": (C.c_int, [C.POINTER(SlotMapArgs), vp]),
     "dsv4_page_indices": (C.c_int, [C.POINTER(PageIndicesArgs), vp]),
     "dsv4_gather_dequant": (C.c_int, [vp, i64, i32, i32, i32, vp, i32, vp, i32, vp]),

@@ -237,6 +237,71 @@ def sparse_prefill_fwd_fp8(q, kv, indices, sm_scale, d_v=512, attn_sink=None, to
                     kv.size(1), kv.size(0) * kv.size(1), kv.stride(0), flags)
 
 
+def dense_prefill_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, sm_scale, causal: bool = True,
+                      attn_sink=None, out=None, *, n_splits: Optional[int] = None):
+    """Dense attention of packed sequences over all their keys, with grouped heads: whole
+    prompts, chunks of prompts behind a cached context, single tokens.
+
+      q [t_q, h_q, d_qk], k [t_k, h_kv, d_qk], v [t_k, h_kv, d_v], bf16 or fp16, with
+      (d_qk, d_v) = (64, 64), (128, 128) or (192, 128) and h_q a multiple of h_kv;
+      cu_seqlens_q, cu_seqlens_k [b + 1] int32 (ascending, on the device)
+      -> (out [t_q, h_q, d_v], max_logits [t_q, h_q] fp32, lse [t_q, h_q] fp32)
+
+    causal: query i of a sequence sees the keys j <= i + len_k - len_q.  Returns and
+    attn_sink [h_q] as for `sparse_prefill_fwd` (lse excludes the sink; a row that sees
+    nothing: out 0, max_logits -inf, lse +inf).  Rows of no sequence are not written: they
+    stay as they were in `out` when it is given, and hold anything otherwise.  Token and
+    head strides are free (positive multiples of 8 elements).  `n_splits` is a test hook.
+    No counterpart in the reference, whose prefill is sparse only."""
+    _require(q.is_cuda and k.device == q.device and v.device == q.device, "q, k and v must be CUDA tensors of one device")
+    _require(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "q, k and v must be 3-D [tokens, heads, d]")
+    _require(q.dtype in (torch.bfloat16, torch.float16) and k.dtype == q.dtype and v.dtype == q.dtype,
+             "q, k and v must be bf16 or fp16, all of one type")
+    t_q, h_q, d_qk = q.shape
+    t_k, h_kv, d_v = v.shape
+    _require((d_qk, d_v) in ((64, 64), (128, 128), (192, 128)),
+             f"(d_qk, d_v) must be (64, 64), (128, 128) or (192, 128); got ({d_qk}, {d_v})")
+    _require(k.shape == (t_k, h_kv, d_qk), "k must be [t_k, h_kv, d_qk], with v's tokens and heads")
+    _require(h_kv >= 1 and h_q >= 1 and h_q % h_kv == 0, f"h_q ({h_q}) must be a multiple of h_kv ({h_kv})")
+    _require(q.stride(2) == 1 and k.stride(2) == 1 and v.stride(2) == 1, "q, k and v must be dense in the last dim")
+    dev = q.device
+    _int32_on("cu_seqlens_q", cu_seqlens_q, dev, 1)
+    _int32_on("cu_seqlens_k", cu_seqlens_k, dev, 1)
+    b = cu_seqlens_q.numel() - 1
+    _require(b >= 0 and cu_seqlens_k.numel() == b + 1 and cu_seqlens_q.is_contiguous()
+             and cu_seqlens_k.is_contiguous(), "cu_seqlens_q and cu_seqlens_k must be contiguous [b + 1]")
+    if attn_sink is not None:
+        _require(attn_sink.dtype == torch.float32 and attn_sink.numel() == h_q and attn_sink.is_contiguous()
+                 and attn_sink.device == dev, f"attn_sink must be contiguous float32 [{h_q}] on {dev}")
+    if out is not None:
+        _require(out.dtype == q.dtype and out.shape == (t_q, h_q, d_v) and out.device == dev and out.stride(2) == 1,
+                 "out must be [t_q, h_q, d_v] of q's type, dense in the last dim")
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty((t_q, h_q, d_v), dtype=q.dtype, device=dev)
+        max_logits = torch.empty((t_q, h_q), dtype=torch.float32, device=dev)
+        lse = torch.empty((t_q, h_q), dtype=torch.float32, device=dev)
+        if n_splits is None:
+            n_splits = N.lib.dsv4_plan_dense_splits(t_q, t_k, b, h_q, h_kv, num_sms(dev))
+        a = N.DensePrefillArgs()
+        a.b, a.t_q, a.t_k, a.h_q, a.h_kv, a.d_qk, a.d_v = b, t_q, t_k, h_q, h_kv, d_qk, d_v
+        a.dtype = N.DTYPE_BF16 if q.dtype == torch.bfloat16 else N.DTYPE_FP16
+        a.causal, a.n_splits, a.sm_scale = int(bool(causal)), n_splits, float(sm_scale)
+        a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+        a.cu_seqlens_q, a.cu_seqlens_k = cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr()
+        a.attn_sink, a.max_logits, a.lse = _ptr(attn_sink), max_logits.data_ptr(), lse.data_ptr()
+        if n_splits > 1:
+            o_accum = torch.empty((n_splits, t_q, h_q, d_v), dtype=torch.float32, device=dev)
+            stat_accum = torch.empty((n_splits, t_q, h_q, 2), dtype=torch.float32, device=dev)
+            a.o_accum, a.stat_accum = o_accum.data_ptr(), stat_accum.data_ptr()
+        (a.stride_q_t, a.stride_q_h, _), (a.stride_k_t, a.stride_k_h, _) = q.stride(), k.stride()
+        (a.stride_v_t, a.stride_v_h, _), (a.stride_o_t, a.stride_o_h, _) = v.stride(), out.stride()
+        a.stride_ml_t = a.stride_lse_t = h_q
+        N.check(N.lib.dsv4_dense_prefill(C.byref(a), torch.cuda.current_stream(dev).cuda_stream),
+                "dsv4_dense_prefill")
+    return out, max_logits, lse
+
+
 def kv_store(k_nope, k_rope, slots, kv) -> None:
     """Quantise and store tokens into the paged cache in place.
     k_nope [n, 448|512] bf16, k_rope [n, 64] bf16, slots [n] int64 (negative = skip),

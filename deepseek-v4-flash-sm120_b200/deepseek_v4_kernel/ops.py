@@ -58,6 +58,12 @@ def sparse_prefill_fwd_fp8(q, kv, indices, sm_scale, d_v=512, attn_sink=None, to
                                         topk_length)
 
 
+def dense_prefill_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, sm_scale, causal=True, attn_sink=None, out=None):
+    """Dense causal attention of packed sequences with grouped heads (prompts, chunks behind a
+    context, single tokens): the same returns as sparse_prefill_fwd."""
+    return _cuda.dense_prefill_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, float(sm_scale), causal, attn_sink, out)
+
+
 def kv_store(k_nope, k_rope, slots, kv) -> None:
     """Quantise BF16 latent + RoPE rows into the FP8 paged cache at `slots`."""
     _cuda.kv_store(k_nope, k_rope, slots, kv)

@@ -264,6 +264,55 @@ typedef struct Dsv4PrefillArgs {
 int dsv4_sparse_prefill(const Dsv4PrefillArgs* args, void* cuda_stream);
 
 /* ---------------------------------------------------------------------------
+ * Dense prefill: attention of packed sequences over all their keys, with grouped heads.
+ * No counterpart in the reference, whose prefill is sparse only: a prompt no longer than
+ * its top-k selects every key, and latent attention with the keys and values of every head
+ * written out (d_qk 192, d_v 128) costs a fraction of the products of the 576 / 512 form.
+ *
+ * Sequence s has the query rows [cu_seqlens_q[s], cu_seqlens_q[s + 1]) of q and the keys
+ * [cu_seqlens_k[s], cu_seqlens_k[s + 1]) of k and v; query head h reads key/value head
+ * h / (h_q / h_kv).  With causal != 0 query i of len_q sees the keys j <= i + len_k - len_q
+ * (the queries are the last ones of the keys: whole prompts, chunks behind a context, single
+ * tokens), otherwise all of them.  Outputs as dsv4_sparse_prefill's: out (the type of q),
+ * max_logits and lse fp32 [t_q, h_q] (natural log; lse excludes the sink; a row that sees no
+ * key gives out 0, max_logits -inf, lse +inf).  Rows of no sequence are not written.  Masked
+ * keys and values may hold anything, NaN included.  The bounds are read on the device and
+ * clamped to the tensors; they have to ascend.
+ *
+ * (d_qk, d_v) is (64, 64), (128, 128) or (192, 128); q, k, v, out of one type.  Strides are
+ * in elements, multiples of 8, positive (k and v of several tokens or heads cannot be
+ * broadcast views); pointers are 16-byte aligned; the last dimension is dense.  sm_scale is
+ * positive and finite.  n_splits > 1 cuts every sequence's keys into that many ranges and
+ * needs o_accum [n_splits, t_q, h_q, d_v] and stat_accum [n_splits, t_q, h_q, 2].           */
+enum Dsv4Dtype { DSV4_DTYPE_BF16 = 0, DSV4_DTYPE_FP16 = 1 };
+typedef struct Dsv4DensePrefillArgs {
+  int32_t b, t_q, t_k, h_q, h_kv, d_qk, d_v;
+  int32_t dtype;                /* Dsv4Dtype                                      */
+  int32_t causal, n_splits;     /* n_splits >= 1; see dsv4_plan_dense_splits      */
+  float sm_scale;
+  int32_t reserved;
+  const void* q;                /* [t_q, h_q, d_qk]                               */
+  const void* k;                /* [t_k, h_kv, d_qk]                              */
+  const void* v;                /* [t_k, h_kv, d_v]                               */
+  const int32_t* cu_seqlens_q;  /* [b + 1]                                        */
+  const int32_t* cu_seqlens_k;  /* [b + 1]                                        */
+  const float* attn_sink;       /* [h_q] or null                                  */
+  void* out;                    /* [t_q, h_q, d_v]                                */
+  float* max_logits;
+  float* lse;
+  float* o_accum;               /* scratch, n_splits > 1                          */
+  float* stat_accum;            /* scratch, n_splits > 1                          */
+  int64_t stride_q_t, stride_q_h, stride_k_t, stride_k_h, stride_v_t, stride_v_h;
+  int64_t stride_o_t, stride_o_h, stride_ml_t, stride_lse_t;
+} Dsv4DensePrefillArgs;
+
+int dsv4_dense_prefill(const Dsv4DensePrefillArgs* args, void* cuda_stream);
+
+/* Key ranges for a dense prefill: a pure function of sizes and the SM count (stable under
+ * graph capture); more than one only when the query rows alone leave SMs idle.             */
+int dsv4_plan_dense_splits(int t_q, int t_k, int b, int h_q, int h_kv, int num_sms);
+
+/* ---------------------------------------------------------------------------
  * KV store / quantise.  The reference has no such kernel: its cache is written
  * by the serving framework (tests/reference.py:48-49 names quant_k_cache_v4).
  * Per token i with slot s = slots[i] >= 0 (page s / P, row s % P): for each
