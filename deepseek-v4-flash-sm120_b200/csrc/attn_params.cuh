@@ -52,6 +52,7 @@ struct AttnParams {
   int64_t stride_lse_b, stride_lse_s, stride_lse_h;
   int64_t stride_ml_b;                          // max_logits row stride (prefill)
   long long* prof;                              // optional timeline buffer (debug), or null
+  int keep_partials;  // decode: leave partials (o_accum, lse_accum) for a later combine even with one split
 };
 
 // Effective list lengths of request `req`: `len` entries of the main list then

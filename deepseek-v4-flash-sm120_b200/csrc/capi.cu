@@ -320,6 +320,143 @@ int dsv4_sparse_prefill(const Dsv4PrefillArgs* a, void* stream) {
   return e ? cuda_fail(e) : DSV4_OK;
 }
 
+// Splits of the two parts of a shared-prefix decode, and its scratch.
+struct SharedPlan {
+  int prefix_splits, suffix_splits;        // 0: the part does not exist
+  int64_t prefix_list, suffix_list;        // entries of the index lists
+  int64_t bytes;
+};
+static SharedPlan plan_shared(const Dsv4SharedPrefixArgs* a, int num_sms) {
+  SharedPlan p{};
+  const int64_t rows = static_cast<int64_t>(a->b) * a->s_q * a->h_q;
+  const int64_t plen = static_cast<int64_t>(a->prefix_pages) * a->page_block_size;
+  const int64_t slen = static_cast<int64_t>(a->max_pages) * a->page_block_size;
+  if (plen > 0)
+    p.prefix_splits = a->prefix_splits > 0 ? a->prefix_splits
+                                           : dsv4_plan_splits(1, 1, static_cast<int>(rows), static_cast<int>(plen), 0, num_sms);
+  if (slen > 0)
+    p.suffix_splits = a->suffix_splits > 0 ? a->suffix_splits
+                                           : dsv4_plan_splits(a->b, a->s_q, a->h_q, static_cast<int>(slen), 0, num_sms);
+  p.prefix_list = plen;
+  p.suffix_list = slen * a->b * a->s_q;
+  p.bytes = (p.prefix_list + p.suffix_list) * 4;
+  return p;
+}
+
+static int check_shared(const Dsv4SharedPrefixArgs* a) {
+  if (!a) return DSV4_ERR_NULL;
+  if (a->b < 0 || a->s_q < 1 || a->h_q < 1 || a->num_blocks < 1 || a->page_block_size < 1 || a->d_v != dsv4::D_V ||
+      a->prefix_pages < 0 || a->max_pages < 0 || a->prefix_splits < 0 || a->suffix_splits < 0 ||
+      a->prefix_splits > 64 || a->suffix_splits > 64)
+    return DSV4_ERR_SHAPE;
+  const int64_t most = 0x7fffffff;
+  if (static_cast<int64_t>(a->num_blocks) * a->page_block_size > most ||
+      static_cast<int64_t>(a->prefix_pages) * a->page_block_size > most ||
+      static_cast<int64_t>(a->max_pages) * a->page_block_size > most ||
+      static_cast<int64_t>(a->b) * a->s_q > most / a->h_q ||
+      static_cast<int64_t>(a->b) * a->s_q * a->h_q > 64ll * 65535)
+    return DSV4_ERR_SHAPE;
+  return DSV4_OK;
+}
+
+int dsv4_shared_prefix_scratch(const Dsv4SharedPrefixArgs* a, int num_sms, int32_t* sets, int64_t* bytes) {
+  int rc = check_shared(a);
+  if (rc) return rc;
+  if (!sets || !bytes) return DSV4_ERR_NULL;
+  if (num_sms < 1) return DSV4_ERR_SHAPE;
+  const SharedPlan p = plan_shared(a, num_sms);
+  *sets = p.prefix_splits + p.suffix_splits;
+  *bytes = p.bytes;
+  return DSV4_OK;
+}
+
+int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* a, void* stream) {
+  int rc = check_shared(a);
+  if (rc) return rc;
+  if (!a->q || !a->kv || !a->out || !a->lse || (a->prefix_pages && (!a->prefix_table || !a->prefix_length)) ||
+      (a->max_pages && (!a->block_table || !a->suffix_length)))
+    return DSV4_ERR_NULL;
+  if ((rc = check_paged(a->kv_format, a->d_qk, a->page_block_size, a->stride_kv_block, a->kv))) return rc;
+  if (a->max_pages && a->stride_table < 0) return DSV4_ERR_SHAPE;
+  if (!aligned16(a->q) || !aligned16(a->out) || (a->stride_o_b & 7) || (a->stride_o_s & 7) || (a->stride_o_h & 7))
+    return DSV4_ERR_ALIGN;
+  if ((rc = current_device_is_sm100())) return rc;
+  if (a->b == 0) return DSV4_OK;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e) return cuda_fail(e);
+  DevInfo info;
+  if ((rc = device_info(dev, info))) return rc;
+  const SharedPlan plan = plan_shared(a, info.sms);
+  const int sets = plan.prefix_splits + plan.suffix_splits;
+  if (sets > 0) {
+    if (!a->o_accum || !a->lse_accum || !a->workspace) return DSV4_ERR_SCRATCH;
+    if (!aligned16(a->o_accum) || !aligned16(a->workspace)) return DSV4_ERR_ALIGN;
+  }
+  const int64_t rows = static_cast<int64_t>(a->b) * a->s_q * a->h_q;
+  int32_t* prefix_list = static_cast<int32_t*>(a->workspace);
+  int32_t* suffix_list = prefix_list + plan.prefix_list;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((e = dsv4::launch_shared_lists(*a, prefix_list, suffix_list, st))) return cuda_fail(e);
+
+  dsv4::AttnParams p{};
+  p.cluster = 1;
+  p.keep_partials = 1;
+  p.flags = DSV4_FLAG_MASK_INVALID | DSV4_FLAG_ZERO_LENGTH_EMPTY;
+  p.mode = dsv4::MODE_DECODE;
+  p.page_block = a->page_block_size;
+  p.n_tok = a->num_blocks * a->page_block_size;
+  p.extra_page_block = 1;
+  p.page_shift = log2_or_minus1(p.page_block);
+  p.sm_scale = a->sm_scale;
+  p.q = static_cast<const __nv_bfloat16*>(a->q);
+  p.kv = static_cast<const uint8_t*>(a->kv);
+  p.stride_kv = a->stride_kv_block;
+  p.stride_q_h = a->d_qk;
+  p.out = static_cast<__nv_bfloat16*>(a->out);
+  p.lse = a->lse;
+  auto attend = [&]() {
+    return want_simple(a->flags) ? dsv4::launch_simple_attn(p, a->kv_format, a->d_qk, st)
+                                 : dsv4::launch_sm100_attn(p, a->kv_format, a->d_qk, st);
+  };
+  if (plan.prefix_splits > 0) {
+    // the rows of all requests as the heads of one: each block of 64 rows walks the prefix once
+    p.n_req = p.s_q = 1;
+    p.h_q = static_cast<int>(rows);
+    p.topk = static_cast<int>(plan.prefix_list);
+    p.n_splits = plan.prefix_splits;
+    p.indices = prefix_list;
+    p.topk_length = a->prefix_length;
+    p.o_accum = a->o_accum;
+    p.lse_accum = a->lse_accum;
+    if ((e = attend())) return cuda_fail(e);
+  }
+  if (plan.suffix_splits > 0) {
+    p.n_req = a->b * a->s_q;
+    p.s_q = a->s_q;
+    p.h_q = a->h_q;
+    p.topk = a->max_pages * a->page_block_size;
+    p.n_splits = plan.suffix_splits;
+    p.indices = suffix_list;
+    p.topk_length = a->suffix_length;
+    p.stride_q_s = static_cast<int64_t>(a->h_q) * a->d_qk;
+    p.stride_q_b = p.stride_q_s * a->s_q;
+    p.stride_idx_s = p.topk;
+    p.stride_idx_b = static_cast<int64_t>(p.topk) * a->s_q;
+    p.o_accum = a->o_accum + plan.prefix_splits * rows * dsv4::D_V;
+    p.lse_accum = a->lse_accum + plan.prefix_splits * rows;
+    if ((e = attend())) return cuda_fail(e);
+  }
+  Dsv4CombineArgs c{};
+  c.n_rows = a->b * a->s_q; c.s_q = a->s_q; c.h_q = a->h_q; c.n_splits = sets;
+  c.o_accum = a->o_accum; c.lse_accum = a->lse_accum; c.attn_sink = a->attn_sink;
+  c.out = a->out; c.lse = a->lse;
+  c.stride_o_b = a->stride_o_b; c.stride_o_s = a->stride_o_s; c.stride_o_h = a->stride_o_h;
+  c.stride_lse_b = a->stride_lse_b; c.stride_lse_s = a->stride_lse_s; c.stride_lse_h = a->stride_lse_h;
+  e = dsv4::launch_combine(c, st);
+  return e ? cuda_fail(e) : DSV4_OK;
+}
+
 int dsv4_plan_dense_splits(int t_q, int t_k, int b, int h_q, int h_kv, int num_sms) {
   if (t_q < 1 || t_k < 1 || b < 1 || h_q < 1 || h_kv < 1 || h_q % h_kv || num_sms < 1) return 1;
   const int64_t ctas = dsv4::dense_ctas(t_q, b, h_q, h_kv);

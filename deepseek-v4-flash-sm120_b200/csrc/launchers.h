@@ -41,6 +41,10 @@ cudaError_t launch_gather_dequant(const void* kv, int64_t stride, int kv_format,
 constexpr int SLOT_MAP_MAX_REQUESTS = 16384;     // both sums of a request list in shared memory
 cudaError_t launch_slot_maps(const Dsv4SlotMapArgs& a, cudaStream_t st);
 cudaError_t launch_page_indices(const Dsv4PageIndicesArgs& a, cudaStream_t st);
+// Token indices of the first length[0] tokens of one table row (`prefix`), and of every
+// request's own tokens as each of its s_q query tokens sees them (`suffix`, one list of
+// max_pages * page tokens per query token).
+cudaError_t launch_shared_lists(const Dsv4SharedPrefixArgs& a, int32_t* prefix, int32_t* suffix, cudaStream_t st);
 
 // Dense attention over packed sequences (dense_attn_sm100.cu).
 constexpr int DENSE_MAX_SPLITS = 64;

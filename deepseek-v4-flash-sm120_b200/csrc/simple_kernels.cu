@@ -131,7 +131,7 @@ simple_attn_kernel(AttnParams p) {
     }
   }
 
-  if (p.n_splits > 1) {
+  if (p.n_splits > 1 || p.keep_partials) {
     const int64_t slot = (static_cast<int64_t>(split) * p.n_req + req) * p.h_q + h;
     const bool empty = (l_run == 0.f);
     if (tid == 0) p.lse_accum[slot] = empty ? -INFINITY : logf(l_run) + m_run;

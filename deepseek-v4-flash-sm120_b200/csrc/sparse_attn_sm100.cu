@@ -756,7 +756,7 @@ sm100_attn_kernel(const AttnParams p) {
   const int heads_here = min(NH, p.h_q - head0);
   const int bi = req / p.s_q, si = req % p.s_q;
   const bool mask_invalid = !decode || (p.flags & DSV4_FLAG_MASK_INVALID);
-  const bool split_out = p.n_splits > 1;
+  const bool split_out = p.n_splits > 1 || p.keep_partials;
   const bool want_ml = p.max_logits != nullptr;
 
   ListView lv;

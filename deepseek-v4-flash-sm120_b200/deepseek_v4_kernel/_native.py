@@ -97,6 +97,16 @@ class DensePrefillArgs(C.Structure):
                            "stride_v_h", "stride_o_t", "stride_o_h", "stride_ml_t", "stride_lse_t")]
 
 
+class SharedPrefixArgs(C.Structure):
+    _fields_ = [(n, i32) for n in ("b", "s_q", "h_q", "d_qk", "d_v", "kv_format", "num_blocks",
+                                   "page_block_size", "prefix_pages", "max_pages", "prefix_splits",
+                                   "suffix_splits", "flags")] + [("sm_scale", f32)] + [
+        (n, vp) for n in ("q", "kv", "prefix_table", "prefix_length", "block_table", "suffix_length",
+                          "attn_sink", "out", "lse", "o_accum", "lse_accum", "workspace")] + [
+        (n, i64) for n in ("stride_kv_block", "stride_table", "stride_o_b", "stride_o_s", "stride_o_h",
+                           "stride_lse_b", "stride_lse_s", "stride_lse_h")]
+
+
 # name -> (restype, argtypes); every symbol include/dsv4_b200.h declares.
 SYMBOLS = {
     "dsv4_abi_version": (C.c_int, []),
@@ -116,6 +126,9 @@ SYMBOLS = {
     "dsv4_kv_store_rows": (C.c_int, [C.POINTER(StoreRowsArgs), vp]),
     "dsv4_dense_prefill": (C.c_int, [C.POINTER(DensePrefillArgs), vp]),
     "dsv4_plan_dense_splits": (C.c_int, [C.c_int] * 6),
+    "dsv4_shared_prefix_decode": (C.c_int, [C.POINTER(SharedPrefixArgs), vp]),
+    "dsv4_shared_prefix_scratch": (C.c_int, [C.POINTER(SharedPrefixArgs), C.c_int, C.POINTER(i32),
+                                             C.POINTER(i64)]),
     "dsv4_build_slot_maps": (C.c_int, [C.POINTER(SlotMapArgs), vp]),
     "dsv4_page_indices": (C.c_int, [C.POINTER(PageIndicesArgs), vp]),
     "dsv4_gather_dequant": (C.c_int, [vp, i64, i32, i32, i32, vp, i32, vp, i32, vp]),

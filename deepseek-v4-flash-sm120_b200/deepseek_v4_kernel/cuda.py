@@ -237,6 +237,77 @@ def sparse_prefill_fwd_fp8(q, kv, indices, sm_scale, d_v=512, attn_sink=None, to
                     kv.size(1), kv.size(0) * kv.size(1), kv.stride(0), flags)
 
 
+def shared_prefix_decode_fwd(q, kv, prefix_table, prefix_length, block_table, suffix_length, attn_sink, d_v,
+                             sm_scale, *, prefix_splits: int = 0, suffix_splits: int = 0, flags: int = 0):
+    """Decode of a batch whose requests share a long prefix: the prefix is attended once for
+    the rows of all requests together, every request's own tokens separately, and the two
+    parts are joined by their log-sum-exps.
+
+      q [b, s_q, h_q, d_qk] bf16 (contiguous); kv [num_blocks, page_block, 1, bytes]
+      fp8/uint8/int8 as for `sparse_decode_fwd`; prefix_table [prefix_pages] int32 and
+      prefix_length [1] int32: the shared tokens; block_table [b, max_pages] int32 and
+      suffix_length [b] int32: each request's own tokens, its s_q query tokens the last of
+      them; attn_sink [h_q] fp32 or None
+      -> (out [b, s_q, h_q, 512] bf16, lse [b, h_q, s_q] fp32, sink-merged)
+
+    Query token s sees the whole prefix and suffix_length - (s_q - 1 - s) own tokens.  A row
+    that sees nothing gives out 0 and lse = its sink, or -inf.  Tokens on pages outside the
+    cache are masked.  The lengths stay on the device, so a captured call can be replayed
+    with others.  `prefix_splits` / `suffix_splits` / `flags` are test hooks.  No counterpart
+    in the reference."""
+    _require(q.is_cuda and kv.device == q.device, "q and kv must be CUDA tensors of one device")
+    _require(q.dim() == 4 and q.dtype == torch.bfloat16 and q.is_contiguous(),
+             "q must be contiguous bf16 [b, s_q, h_q, d_qk]")
+    _require(kv.dim() == 4 and kv.dtype in _KV_DTYPES and kv.size(2) == 1,
+             "kv must be [num_blocks, page_block, 1, bytes] fp8_e4m3 / uint8 / int8")
+    b, s_q, h_q, d_qk = q.shape
+    num_blocks, page_block, _, token_bytes = kv.shape
+    fmt = _kv_format(d_qk, token_bytes)
+    _require(int(d_v) == 512, "Only d_v=512 supported")
+    _require(kv.stride(1) == token_bytes and kv.stride(3) == 1,
+             "kv pages must be dense (only the page stride may be padded)")
+    dev = q.device
+    _int32_on("prefix_table", prefix_table, dev, 1)
+    _int32_on("prefix_length", prefix_length, dev, 1)
+    _int32_on("block_table", block_table, dev, 2)
+    _int32_on("suffix_length", suffix_length, dev, 1)
+    _require(prefix_length.numel() == 1 and prefix_table.is_contiguous(), "prefix_length [1], prefix_table contiguous expected")
+    _require(block_table.size(0) == b and suffix_length.numel() == b and suffix_length.is_contiguous(),
+             f"block_table [{b}, max_pages] and contiguous suffix_length [{b}] expected")
+    max_pages = block_table.size(1)
+    _require(max_pages <= 1 or block_table.stride(1) == 1, "block_table rows must be dense")
+    if attn_sink is not None:
+        _require(attn_sink.dtype == torch.float32 and attn_sink.numel() == h_q and attn_sink.is_contiguous()
+                 and attn_sink.device == dev, "attn_sink must be contiguous float32 [h_q]")
+    with torch.cuda.device(dev):
+        out = torch.empty((b, s_q, h_q, 512), dtype=torch.bfloat16, device=dev)
+        lse = torch.empty((b, h_q, s_q), dtype=torch.float32, device=dev)
+        a = N.SharedPrefixArgs()
+        a.b, a.s_q, a.h_q, a.d_qk, a.d_v, a.kv_format = b, s_q, h_q, d_qk, 512, fmt
+        a.num_blocks, a.page_block_size = num_blocks, page_block
+        a.prefix_pages, a.max_pages = prefix_table.numel(), max_pages
+        a.prefix_splits, a.suffix_splits, a.flags, a.sm_scale = prefix_splits, suffix_splits, flags, float(sm_scale)
+        sets, nbytes = C.c_int32(0), C.c_int64(0)
+        N.check(N.lib.dsv4_shared_prefix_scratch(C.byref(a), num_sms(dev), C.byref(sets), C.byref(nbytes)),
+                "dsv4_shared_prefix_scratch")
+        rows = b * s_q * h_q
+        o_accum = torch.empty((sets.value, rows, 512), dtype=torch.float32, device=dev)
+        lse_accum = torch.empty((sets.value, rows), dtype=torch.float32, device=dev)
+        workspace = torch.empty((nbytes.value,), dtype=torch.uint8, device=dev)
+        a.q, a.kv, a.attn_sink = q.data_ptr(), kv.data_ptr(), _ptr(attn_sink)
+        a.prefix_table, a.prefix_length = prefix_table.data_ptr(), prefix_length.data_ptr()
+        a.block_table, a.suffix_length = block_table.data_ptr(), suffix_length.data_ptr()
+        a.out, a.lse = out.data_ptr(), lse.data_ptr()
+        a.o_accum, a.lse_accum, a.workspace = o_accum.data_ptr(), lse_accum.data_ptr(), workspace.data_ptr()
+        a.stride_kv_block, a.stride_table = kv.stride(0), block_table.stride(0)
+        a.stride_o_b, a.stride_o_s, a.stride_o_h = out.stride(0), out.stride(1), out.stride(2)
+        a.stride_lse_b, a.stride_lse_h, a.stride_lse_s = lse.stride(0), lse.stride(1), lse.stride(2)
+        if b > 0:
+            N.check(N.lib.dsv4_shared_prefix_decode(C.byref(a), torch.cuda.current_stream(dev).cuda_stream),
+                    "dsv4_shared_prefix_decode")
+    return out, lse
+
+
 def dense_prefill_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, sm_scale, causal: bool = True,
                       attn_sink=None, out=None, *, n_splits: Optional[int] = None):
     """Dense attention of packed sequences over all their keys, with grouped heads: whole

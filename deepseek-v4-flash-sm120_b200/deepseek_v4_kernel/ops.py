@@ -58,6 +58,13 @@ def sparse_prefill_fwd_fp8(q, kv, indices, sm_scale, d_v=512, attn_sink=None, to
                                         topk_length)
 
 
+def shared_prefix_decode_fwd(q, kv, prefix_table, prefix_length, block_table, suffix_length, attn_sink, d_v, sm_scale):
+    """Dense decode of a batch that shares a long prefix over the FP8 paged cache, the prefix
+    attended once for all requests: returns (out, lse[b, h_q, s_q])."""
+    return _cuda.shared_prefix_decode_fwd(q, kv, prefix_table, prefix_length, block_table, suffix_length, attn_sink,
+                                          int(d_v), float(sm_scale))
+
+
 def dense_prefill_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, sm_scale, causal=True, attn_sink=None, out=None):
     """Dense causal attention of packed sequences with grouped heads (prompts, chunks behind a
     context, single tokens): the same returns as sparse_prefill_fwd."""

@@ -264,6 +264,55 @@ typedef struct Dsv4PrefillArgs {
 int dsv4_sparse_prefill(const Dsv4PrefillArgs* args, void* cuda_stream);
 
 /* ---------------------------------------------------------------------------
+ * Decode of a batch that shares a long prefix.  No counterpart in the reference (its
+ * decode takes one index list per request and would read the prefix once for each).
+ *
+ * All requests attend to the first prefix_length[0] tokens of the pages prefix_table
+ * [prefix_pages], and request r also to the first suffix_length[r] tokens of its own pages
+ * block_table[r, 0:max_pages): query token s of s_q sees suffix_length[r] - (s_q - 1 - s) of
+ * them (the last s_q tokens are the queries' own).  The products with the prefix are formed
+ * once for the rows of all requests together; the two parts are joined by their
+ * log-sum-exps.  Layouts, out, lse (sink-merged) and strides as dsv4_sparse_decode's; a row
+ * that sees nothing gives out 0 and lse = its sink, or -inf.  Tokens of a page id outside
+ * [0, num_blocks) are masked; lengths are clamped to the tables.  The lengths live on the
+ * device; launches depend on sizes only.
+ *
+ * q rows are dense: stride_q_h = d_qk, [b, s_q, h_q] contiguous.  Scratch, sized by
+ * dsv4_shared_prefix_scratch(args): o_accum fp32 [sets, b, s_q, h_q, 512], lse_accum fp32
+ * [sets, b, s_q, h_q], workspace bytes.  num_blocks * page_block_size < 2^31.                */
+typedef struct Dsv4SharedPrefixArgs {
+  int32_t b, s_q, h_q, d_qk, d_v;
+  int32_t kv_format;            /* DSV4_KV_MODEL1 or DSV4_KV_V32                 */
+  int32_t num_blocks, page_block_size;
+  int32_t prefix_pages, max_pages;
+  int32_t prefix_splits, suffix_splits;   /* 0: chosen by the library             */
+  int32_t flags;                /* DSV4_FLAG_IMPL_SIMPLE                          */
+  float sm_scale;
+  const void* q;                /* BF16 [b, s_q, h_q, d_qk]                       */
+  const void* kv;               /* bytes [num_blocks, stride_kv_block]            */
+  const int32_t* prefix_table;  /* [prefix_pages]                                 */
+  const int32_t* prefix_length; /* [1]                                            */
+  const int32_t* block_table;   /* [b, max_pages]                                 */
+  const int32_t* suffix_length; /* [b]                                            */
+  const float* attn_sink;       /* [h_q] or null                                  */
+  void* out;                    /* BF16 [b, s_q, h_q, 512]                        */
+  float* lse;                   /* fp32, addressed with the three lse strides     */
+  float* o_accum;
+  float* lse_accum;
+  void* workspace;
+  int64_t stride_kv_block, stride_table;
+  int64_t stride_o_b, stride_o_s, stride_o_h;
+  int64_t stride_lse_b, stride_lse_s, stride_lse_h;
+} Dsv4SharedPrefixArgs;
+
+int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* args, void* cuda_stream);
+
+/* Scratch of such a call (sizes and split counts of `args`; pointers are not looked at):
+ * partial sets, and bytes of workspace.                                                    */
+int dsv4_shared_prefix_scratch(const Dsv4SharedPrefixArgs* args, int num_sms, int32_t* sets,
+                               int64_t* workspace_bytes);
+
+/* ---------------------------------------------------------------------------
  * Dense prefill: attention of packed sequences over all their keys, with grouped heads.
  * No counterpart in the reference, whose prefill is sparse only: a prompt no longer than
  * its top-k selects every key, and latent attention with the keys and values of every head
