@@ -11,9 +11,11 @@
 //   S_s [128 rows, 128 keys] = Q_s K^T        A, B from shared memory, K-major
 //   O_s [128 rows, d_v]     += P_s V          A = P from TMEM, B = V, MN-major as it was loaded
 //
-// The two tiles (s = 0, 1) take turns: while the tensor core works for one, a warpgroup of
-// softmax threads works for the other.  A softmax thread owns one row (its TMEM lane), so the
-// maximum and the sum of a row need no exchange; P is written over S in TMEM.  O is rescaled
+// A softmax thread owns one row (its TMEM lane), so the maximum and the sum of a row need no
+// exchange.  It takes the 128 scores of a tile into registers at once and frees their TMEM
+// columns: the two tiles (s = 0, 1) share one score buffer (O_0, O_1, P_0 and P_1 fill the rest
+// of TMEM at d_v = 128), the scores of the next tile are formed while this one's exponentials
+// are, and the product with V waits for neither.  O is rescaled
 // only when a row's maximum has grown by more than 2^8 since its reference was set (the sums
 // are 32-bit and P has as many significant bits at any scale), by the same threads, so there
 // is no correction stage.  Q, K and V arrive by TMA; K's ring is recycled in blocks of 64
@@ -21,7 +23,7 @@
 //
 // Masked keys: scores are replaced, not added to, so nothing in a masked key's K row counts.
 // A product with weight zero would still let a NaN or an infinity of a masked V row through,
-// so in the tiles that some row sees only in part two idle warps look over V in shared memory
+// so in the tiles that some row sees only in part an idle warp looks over V in shared memory
 // before the tensor core may read it: rows no one sees are cleared, and elements that are not
 // finite are cleared and handed by the epilogue to the rows that do see them.
 //
@@ -31,6 +33,7 @@
 #include <cuda_fp16.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "attn_params.cuh"
 #include "launchers.h"
@@ -47,31 +50,43 @@ using namespace ptx;
 constexpr int TILE_M = 128, TILE_N = 128;
 constexpr int BLOCK_BYTES = 128 * 128;               // [128 rows][64 16-bit values], swizzled
 constexpr int SOFTMAX_THREADS = 256;                 // two warpgroups, one per row tile
-constexpr int THREADS = SOFTMAX_THREADS + 128;       // + MMA, TMA and two looking-over warps
+constexpr int THREADS = SOFTMAX_THREADS + 128;       // + two MMA warps, TMA, looking over V
 // 384 threads start with 168 registers; the third warpgroup hands most of its own over:
 // 128 * 72 + 256 * 216 = 384 * 168.
 constexpr int LAUNCH_REGS = 168, SOFTMAX_REGS = 216, HELPER_REGS = 72;
 static_assert(SOFTMAX_THREADS * SOFTMAX_REGS + 128 * HELPER_REGS <= THREADS * LAUNCH_REGS,
               "setmaxnreg.inc can only take what setmaxnreg.dec gave back");
 static_assert(THREADS * (LAUNCH_REGS + 8) > 65536, "LAUNCH_REGS is what the launch bound yields");
-constexpr int WARP_MMA = 8, WARP_TMA = 9, WARP_LOOK = 10;
+constexpr int WARP_QK = 8, WARP_PV = 9, WARP_TMA = 10, WARP_LOOK = 11;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float RESCALE_THRESHOLD = 8.0f;            // log2 units
-constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_O = 256;   // S_s at 128 s, O_s at 256 + 128 s
+#ifndef EMU
+#define EMU 0
+#endif
+constexpr int EMULATED = EMU;
+constexpr uint32_t TMEM_COLS = 512;
 
-enum DenseErr { ERR_Q = 11, ERR_K = 12, ERR_V = 13, ERR_P = 14, ERR_S = 15, ERR_O = 16, ERR_SLOT = 17, ERR_LOOK = 18 };
+enum DenseErr { ERR_Q = 11, ERR_K = 12, ERR_V = 13, ERR_P = 14, ERR_S = 15, ERR_O = 16, ERR_SLOT = 17, ERR_LOOK = 18,
+                ERR_FREE = 19 };
 
 template <int DQK, int DV> struct DCfg {
   static constexpr int QB = DQK / 64, VB = DV / 64;
   static constexpr int K_SLOTS = DQK == 192 ? 4 : DQK == 128 ? 6 : 4;   // blocks of 64 columns
+  static constexpr int K_STEP = DQK == 192 ? 1 : QB;      // blocks handed over together
+  static constexpr int K_RING = K_SLOTS / K_STEP;
   static constexpr int V_UNITS = DQK == 64 ? 4 : 2;                     // whole tiles
+  // TMEM columns: O_s (d_v each), P_s (64 each), and what is left for scores: one tile that the
+  // row tiles use in turn at d_v = 128, one each at d_v = 64.
+  static constexpr int S_BUFS = DV == 64 ? 2 : 1;
+  static constexpr uint32_t COL_S = 0, COL_P = 128 * S_BUFS, COL_O = COL_P + 128;
+  static_assert(COL_O + 2 * DV <= TMEM_COLS, "512 columns");
   static constexpr int Q_BYTES = 2 * QB * BLOCK_BYTES, K_BYTES = K_SLOTS * BLOCK_BYTES;
   static constexpr int V_UNIT_BYTES = VB * BLOCK_BYTES, V_BYTES = V_UNITS * V_UNIT_BYTES;
 };
 
 struct DenseCtrl {
-  uint64_t q_full[2], s_full[2], p_full[2], o_done[2];
-  uint64_t k_full[6], k_empty[6], v_full[4], v_empty[4];
+  uint64_t q_full[2], s_full[2], s_free[2], p_full[2], o_done[2];
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
   // tiles that are looked over (the last ones) land on v_look instead of v_full, so that the
   // looking warps count only their own phases; v_clean hands them on
   uint64_t v_look[4], v_clean[4];
@@ -106,6 +121,57 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// Pairs of 32-bit floats in one 64-bit register: one instruction for both.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// Largest of three; NaN if one of them is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^y for two values of at most RESCALE_THRESHOLD without the special-function unit, which is
+// what the softmax is bound by: 2^y = 2^n 2^f with n the nearest integer (left in the low bits
+// by adding 1.5 * 2^23) and |f| <= 1/2, 2^f by the polynomial of degree 5 of least relative
+// error there (fitted by Lawson's reweighting: 7.5e-8 off, 2.1e-7 as evaluated in 32 bits, about
+// the special-function unit's own error).
+// Below 2^-126 the result stays 2^-126.
+__device__ __forceinline__ void ex2_pair(uint64_t y, float& a, float& b) {
+  constexpr float BIG = 12582912.0f;
+  constexpr float C0 = 1.00000012f, C1 = 0.693146944f, C2 = 0.240221202f, C3 = 0.0555071309f, C4 = 0.00967554096f,
+                  C5 = 0.00132764725f;
+  unpair(y, a, b);
+  y = pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+  const uint64_t t = add_pair(y, pair(BIG, BIG));
+  const uint64_t f = fma_pair(add_pair(t, pair(-BIG, -BIG)), pair(-1.f, -1.f), y);
+  uint64_t r = pair(C5, C5);
+  r = fma_pair(r, f, pair(C4, C4));
+  r = fma_pair(r, f, pair(C3, C3));
+  r = fma_pair(r, f, pair(C2, C2));
+  r = fma_pair(r, f, pair(C1, C1));
+  r = fma_pair(r, f, pair(C0, C0));
+  float n0, n1;
+  unpair(t, n0, n1);
+  unpair(r, a, b);
+  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(n0) << 23));
+  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(n1) << 23));
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -182,7 +248,7 @@ template <int DV, bool BF16>
 __device__ __forceinline__ void store_stats(const DenseParams& p, int split, int64_t t, int h, float m_raw, float m_ref,
                                             float l, bool fail, float& factor) {
   // m_ref: reference in log2 units (-inf: nothing seen); l: sum relative to it
-  const bool none = l == 0.f;                  // (a sum of NaN scores is not zero: it shows)
+  const bool none = m_ref == -INFINITY && l == l;      // (NaN scores set no reference, but show)
   const float lse = none ? -INFINITY : logf(l) + m_ref * LN2;
   const float ml = none ? -INFINITY : m_raw * p.sm_scale;
   factor = none ? 0.f : 1.f / l;
@@ -238,23 +304,22 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   }
 
   auto bar = [&](uint64_t* x) { return smem_u32(x); };
-  if (warp == WARP_MMA) {
+  if (warp == WARP_QK) {
     if (lane == 0) {
       for (int s = 0; s < 2; ++s) {
         mbar_init(bar(&ctrl.q_full[s]), 1);
         mbar_init(bar(&ctrl.s_full[s]), 1);
+        mbar_init(bar(&ctrl.s_free[s]), 4);
         mbar_init(bar(&ctrl.p_full[s]), 4);
         mbar_init(bar(&ctrl.o_done[s]), 1);
       }
-      for (int i = 0; i < 6; ++i) {
+      for (int i = 0; i < 4; ++i) {
         mbar_init(bar(&ctrl.k_full[i]), 1);
         mbar_init(bar(&ctrl.k_empty[i]), 1);
-      }
-      for (int i = 0; i < 4; ++i) {
         mbar_init(bar(&ctrl.v_full[i]), 1);
         mbar_init(bar(&ctrl.v_empty[i]), 1);
         mbar_init(bar(&ctrl.v_look[i]), 1);
-        mbar_init(bar(&ctrl.v_clean[i]), 2);
+        mbar_init(bar(&ctrl.v_clean[i]), 1);
       }
       ctrl.fail = 0;
       ctrl.bad = 0;
@@ -275,7 +340,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     *reinterpret_cast<volatile int*>(&ctrl.fail) = 1;
   };
 
-  if (warp >= WARP_MMA) {
+  if (warp >= WARP_QK) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(HELPER_REGS));
     if (warp == WARP_TMA) {
       // ======================= loads ======================================================
@@ -292,11 +357,12 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
         int ks = 0, kphase = 0, vu = 0, vphase = 0;
         for (int i = 0; i < n_tiles && ok; ++i) {
           const int row = w.k0 + (w.first + i) * TILE_N;
-          for (int c = 0; c < C::QB && ok; ++c) {
+          for (int c = 0; c < C::QB; c += C::K_STEP) {
             if (!mbar_wait(bar(&ctrl.k_empty[ks]), kphase ^ 1)) { gave_up(ERR_SLOT); ok = false; break; }
-            mbar_expect_tx(bar(&ctrl.k_full[ks]), BLOCK_BYTES);
-            tma_load_3d(sK + ks * BLOCK_BYTES, &p.mk, 64 * c, kvh, row, bar(&ctrl.k_full[ks]));
-            if (++ks == C::K_SLOTS) { ks = 0; kphase ^= 1; }
+            mbar_expect_tx(bar(&ctrl.k_full[ks]), C::K_STEP * BLOCK_BYTES);
+            for (int d = 0; d < C::K_STEP; ++d)
+              tma_load_3d(sK + (ks * C::K_STEP + d) * BLOCK_BYTES, &p.mk, 64 * (c + d), kvh, row, bar(&ctrl.k_full[ks]));
+            if (++ks == C::K_RING) { ks = 0; kphase ^= 1; }
           }
           if (i == 0 && w.count[1] > 0) load_q(1);
           if (!ok || !mbar_wait(bar(&ctrl.v_empty[vu]), vphase ^ 1)) { gave_up(ERR_SLOT); break; }
@@ -308,74 +374,89 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
         }
       }
       __syncwarp();
-    } else if (warp == WARP_MMA) {
+    } else if (warp < WARP_TMA) {
       // ======================= products ===================================================
-      const uint32_t idesc_qk = make_idesc_16(BF16, TILE_M, TILE_N, 0, 0);
-      const uint32_t idesc_pv = make_idesc_16(BF16, TILE_M, DV, 0, 1);
-      const uint64_t dQ = make_smem_desc(sQ, 16, 1024, SWZ_128B);
-      const uint64_t dK = make_smem_desc(sK, 16, 1024, SWZ_128B);
-      const uint64_t dV = make_smem_desc(sV, BLOCK_BYTES, 1024, SWZ_128B);   // MN-major
+      // One warp issues the scores of both row tiles, another one the products with V: the two
+      // streams write different accumulators and interleave in the tensor core, and a wait of
+      // one does not hold up the other.  Every lane runs the code, one issues; the values it
+      // starts from are broadcast so that they are known to be uniform.
+      const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
+      const int count0 = __shfl_sync(0xffffffffu, w.count[0], 0), count1 = __shfl_sync(0xffffffffu, w.count[1], 0);
+      const int tiles = max(count0, count1);
       const uint32_t elected = elect_one();
       bool ok = true;
-      uint32_t clean_parity = 0;
       auto wait = [&](uint64_t* b, int parity, int code) {
-        if (ok && !mbar_wait_warp(bar(b), parity, lane)) {
+        if (ok && !mbar_wait(bar(b), parity)) {
           if (lane == 0) gave_up(code);
           ok = false;
         }
+        __syncwarp();
       };
-      // S_s of key tile i; `last`: nobody reads the tile's K after this product.
-      auto scores = [&](int s, int i, bool last) {
-        int idx = i * C::QB;
-        int ks = idx % C::K_SLOTS, kphase = (idx / C::K_SLOTS) & 1;
-        if (i == 0) wait(&ctrl.q_full[s], 0, ERR_Q);
-#pragma unroll
-        for (int c = 0; c < C::QB; ++c) {
-          wait(&ctrl.k_full[ks], kphase, ERR_K);
-          if (!ok) return;
-          tc_fence_after_sync();
-#pragma unroll
-          for (int k4 = 0; k4 < 4; ++k4)
-            umma_bf16_elect(tmem + COL_S + 128 * s, dQ + (((s * C::QB + c) * BLOCK_BYTES + k4 * 32) >> 4),
-                            dK + ((ks * BLOCK_BYTES + k4 * 32) >> 4), idesc_qk, (c | k4) != 0, elected);
-          if (last) umma_commit_elect(bar(&ctrl.k_empty[ks]), elected);
-          if (++ks == C::K_SLOTS) { ks = 0; kphase ^= 1; }
-        }
-        umma_commit_elect(bar(&ctrl.s_full[s]), elected);
-      };
-      for (int s = 0; s < 2; ++s)
-        if (w.count[s] > 0 && ok) scores(s, 0, s == 1 || w.count[1] <= 0);
+      if (warp == WARP_QK) {
+        constexpr uint32_t idesc = make_idesc_16(BF16, TILE_M, TILE_N, 0, 0);
+        const uint64_t dQ = make_smem_desc(sQ, 16, 1024, SWZ_128B);
+        const uint64_t dK = make_smem_desc(sK, 16, 1024, SWZ_128B);
+        int turn = 0;                                    // score tiles so far
 #pragma unroll 1
-      for (int i = 0; i < n_tiles && ok; ++i) {
-        const int vu = i % C::V_UNITS, vphase = (i / C::V_UNITS) & 1;
-        bool have_v = false;
-#pragma unroll 1
-        for (int s = 0; s < 2 && ok; ++s) {
-          if (i >= w.count[s]) continue;
-          wait(&ctrl.p_full[s], i & 1, ERR_P);
-          if (!have_v) {
-            have_v = true;
-            if (w.first + i >= w.look) {
-              wait(&ctrl.v_clean[vu], (clean_parity >> vu) & 1, ERR_LOOK);
-              clean_parity ^= 1u << vu;
-            } else {
-              wait(&ctrl.v_full[vu], vphase, ERR_V);
+        for (int i = 0; i < tiles && ok; ++i) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if (i >= (s == 0 ? count0 : count1) || !ok) continue;
+            const bool last = s == 1 || i >= count1;     // nobody reads the tile's K after this
+            if (i == 0) wait(&ctrl.q_full[s], 0, ERR_Q);
+            // the scores that were here have been read
+            if (C::S_BUFS == 1) wait(&ctrl.s_free[0], (turn & 1) ^ 1, ERR_FREE);
+            else wait(&ctrl.s_free[s], (i & 1) ^ 1, ERR_FREE);
+            ++turn;
+            const uint32_t tS = t0 + C::COL_S + (C::S_BUFS == 1 ? 0 : 128 * s);
+            int ks = (i * (C::QB / C::K_STEP)) % C::K_RING, kphase = (i * (C::QB / C::K_STEP) / C::K_RING) & 1;
+#pragma unroll
+            for (int c = 0; c < C::QB; c += C::K_STEP) {
+              wait(&ctrl.k_full[ks], kphase, ERR_K);
+              if (!ok) break;
+              tc_fence_after_sync();
+              const uint64_t d = dK + ((ks * C::K_STEP * BLOCK_BYTES) >> 4);
+#pragma unroll
+              for (int k = 0; k < 4 * C::K_STEP; ++k)
+                umma_bf16_elect(tS, dQ + (((s * C::QB + c + (k >> 2)) * BLOCK_BYTES + (k & 3) * 32) >> 4),
+                                d + (((k >> 2) * BLOCK_BYTES + (k & 3) * 32) >> 4), idesc, (c | k) != 0, elected);
+              if (last) umma_commit_elect(bar(&ctrl.k_empty[ks]), elected);
+              if (++ks == C::K_RING) { ks = 0; kphase ^= 1; }
             }
+            if (ok) umma_commit_elect(bar(&ctrl.s_full[s]), elected);
           }
-          if (!ok) break;
-          tc_fence_after_sync();
+        }
+      } else {
+        constexpr uint32_t idesc = make_idesc_16(BF16, TILE_M, DV, 0, 1);
+        const uint64_t dV = make_smem_desc(sV, BLOCK_BYTES, 1024, SWZ_128B);   // MN-major
+        uint32_t clean_parity = 0;
+#pragma unroll 1
+        for (int i = 0; i < tiles && ok; ++i) {
+          const int vu = i % C::V_UNITS, vphase = (i / C::V_UNITS) & 1;
+          const uint64_t d = dV + ((vu * C::V_UNIT_BYTES) >> 4);
+          if (w.first + i >= w.look) {
+            wait(&ctrl.v_clean[vu], (clean_parity >> vu) & 1, ERR_LOOK);
+            clean_parity ^= 1u << vu;
+          } else {
+            wait(&ctrl.v_full[vu], vphase, ERR_V);
+          }
 #pragma unroll
-          for (int k = 0; k < TILE_N / 16; ++k)
-            umma_ts_elect(tmem + COL_O + 128 * s, tmem + COL_S + 128 * s + 8 * k,
-                          dV + ((vu * C::V_UNIT_BYTES + k * 2048) >> 4), idesc_pv, (i | k) != 0, elected);
-          umma_commit_elect(bar(&ctrl.o_done[s]), elected);
-          if (s == 1 || i >= w.count[1]) umma_commit_elect(bar(&ctrl.v_empty[vu]), elected);
-          if (i + 1 < w.count[s]) scores(s, i + 1, s == 1 || i + 1 >= w.count[1]);
+          for (int s = 0; s < 2; ++s) {
+            if (i >= (s == 0 ? count0 : count1)) continue;
+            wait(&ctrl.p_full[s], i & 1, ERR_P);
+            if (!ok) break;
+            tc_fence_after_sync();
+#pragma unroll
+            for (int k = 0; k < TILE_N / 16; ++k)
+              umma_ts_elect(t0 + C::COL_O + DV * s, t0 + C::COL_P + 64 * s + 8 * k, d + ((k * 2048) >> 4), idesc,
+                            (i | k) != 0, elected);
+            umma_commit_elect(bar(&ctrl.o_done[s]), elected);
+            if (s == 1 || i >= count1) umma_commit_elect(bar(&ctrl.v_empty[vu]), elected);
+          }
         }
       }
     } else {
       // ======================= looking over V =============================================
-      const int t2 = (warp - WARP_LOOK) * 32 + lane;
       // keys the whole CTA sees (its last row sees the most)
       const int seen = reach_of(p, w, min(w.t0 + 2 * p.tok_tile, w.len_q) - 1);
       uint32_t parity = 0;
@@ -388,7 +469,8 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
         parity ^= 1u << vu;
         const int live = min(seen - (w.first + i) * TILE_N, TILE_N);   // rows of the tile that count
         uint32_t found = 0;
-        for (int c = t2; c < C::V_UNIT_BYTES / 16; c += 64) {
+#pragma unroll 4
+        for (int c = lane; c < C::V_UNIT_BYTES / 16; c += 32) {
           const uint32_t addr = sV + vu * C::V_UNIT_BYTES + c * 16;
           const int row = (c >> 3) & 127;
           uint32_t x[4];
@@ -423,7 +505,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    if (warp == WARP_MMA) tmem_dealloc(tmem, TMEM_COLS);
+    if (warp == WARP_QK) tmem_dealloc(tmem, TMEM_COLS);
     return;
   }
 
@@ -437,7 +519,8 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   const int reach = live ? reach_of(p, w, tok) : 0;
   const int n_mine = w.count[s];
   const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-  const uint32_t tS = tmem + lanes + COL_S + 128 * s, tO = tmem + lanes + COL_O + 128 * s;
+  const uint32_t tS = tmem + lanes + C::COL_S + (C::S_BUFS == 1 ? 0 : 128 * s), tP = tmem + lanes + C::COL_P + 64 * s;
+  const uint32_t tO = tmem + lanes + C::COL_O + DV * s;
   const float c = p.sm_scale * LOG2E;
   // tiles below this one are seen whole by every row of this tile that exists
   const int whole = reach_of(p, w, w.t0 + s * p.tok_tile) / TILE_N;
@@ -452,6 +535,10 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) tmem_ld32(tS + 32 * k, x + 32 * k);
     tmem_ld_wait();
+    // The scores are in registers: their columns are free for the other row tile's.
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(&ctrl.s_free[C::S_BUFS == 1 ? 0 : s]));
     if (w.first + i >= whole) {
       const int see = reach - (w.first + i) * TILE_N;
 #pragma unroll
@@ -459,9 +546,10 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     }
     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int k = 0; k < TILE_N; ++k) mx[k & 3] = fmaxf(mx[k & 3], __uint_as_float(x[k]));
-    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-    m_raw = fmaxf(m_raw, top);
+    for (int k = 0; k < TILE_N; k += 2)
+      mx[(k >> 1) & 3] = max3(mx[(k >> 1) & 3], __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+    const float top = max3(mx[0], mx[1], max3(mx[2], mx[3], -INFINITY));
+    m_raw = max3(m_raw, top, -INFINITY);
     const float top2 = top * c;
     const bool raise = top2 > m_ref + RESCALE_THRESHOLD;       // also the first finite one
     float alpha = 1.f;
@@ -470,9 +558,12 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
       m_ref = top2;
       l *= alpha;
     }
-    if (i > 0 && __any_sync(0xffffffffu, raise)) {
+    // the product of the tile before has read P, and O is its result
+    if (i > 0) {
       if (!mbar_wait(bar(&ctrl.o_done[s]), (i - 1) & 1)) { gave_up(ERR_O); ok = false; break; }
       tc_fence_after_sync();
+    }
+    if (i > 0 && __any_sync(0xffffffffu, raise)) {
 #pragma unroll 1
       for (int k = 0; k < DV / 16; ++k) {
         uint32_t o[16];
@@ -484,21 +575,38 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
       }
     }
     const float ref = m_ref == -INFINITY ? 0.f : m_ref;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!(top2 < INFINITY)) l = NAN;                 // a NaN or infinite score: the row shows it
+    const uint64_t c2 = pair(c, c), minus_ref = pair(-ref, -ref);
+    uint64_t sum[2] = {0, 0};
+    // A share of the exponentials goes to the FMA pipe: of four pairs EMULATED are computed there.
+    // (Not in a tile with masked keys: their weights have to be zero.)
+    auto weights = [&](auto masked) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      uint32_t pk[32];
+      for (int q = 0; q < 2; ++q) {
+        uint32_t pk[32];
 #pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const float a = ex2(fmaf(__uint_as_float(x[64 * q + 2 * k]), c, -ref));
-        const float b = ex2(fmaf(__uint_as_float(x[64 * q + 2 * k + 1]), c, -ref));
-        sum[(2 * k) & 3] += a;
-        sum[(2 * k + 1) & 3] += b;
-        pk[k] = pack2<BF16>(a, b);
+        for (int k = 0; k < 32; ++k) {
+          const uint64_t y = fma_pair(pair(__uint_as_float(x[64 * q + 2 * k]), __uint_as_float(x[64 * q + 2 * k + 1])), c2, minus_ref);
+          float a, b;
+          if (!decltype(masked)::value && (k & 3) < EMULATED) {
+            ex2_pair(y, a, b);
+          } else {
+            unpair(y, a, b);
+            a = ex2(a);
+            b = ex2(b);
+          }
+          sum[k & 1] = add_pair(sum[k & 1], pair(a, b));
+          pk[k] = pack2<BF16>(a, b);
+        }
+        tmem_st32(tP + 32 * q, pk);
       }
-      tmem_st32(tS + 32 * q, pk);
-    }
-    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    };
+    if (w.first + i >= whole) weights(std::true_type{});
+    else weights(std::false_type{});
+    float s0, s1, s2, s3;
+    unpair(sum[0], s0, s1);
+    unpair(sum[1], s2, s3);
+    l += (s0 + s1) + (s2 + s3);
     tmem_st_wait();
     tc_fence_before_sync();
     __syncwarp();
@@ -513,6 +621,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   const int64_t t = static_cast<int64_t>(w.q0) + tok;
   float factor = 0.f;
   if (live) store_stats<DV, BF16>(p, split, t, h, m_raw, m_ref, l, fail, factor);
+  const bool nothing = m_ref == -INFINITY && l == l;
   const bool bad = *reinterpret_cast<volatile int*>(&ctrl.bad) != 0;
   const int64_t acc = ((static_cast<int64_t>(split) * p.t_q + t) * p.h_q + h) * DV;
 #pragma unroll 1
@@ -524,7 +633,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     }
     float f[32];
 #pragma unroll
-    for (int q = 0; q < 32; ++q) f[q] = factor == 0.f && l == 0.f ? 0.f : __uint_as_float(o[q]) * factor;
+    for (int q = 0; q < 32; ++q) f[q] = nothing ? 0.f : __uint_as_float(o[q]) * factor;
     if (bad && live) {
       // the values that were cleared, for the rows that see them: their weight is positive,
       // so an infinity stays one (and two of both signs, or a NaN, make a NaN)
