@@ -190,6 +190,15 @@ __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
               : ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
 }
 
+// Larger magnitude in each half of a word (the sign is of no meaning); NaN if either is.
+template <bool BF16>
+__device__ __forceinline__ uint32_t abs_max2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (BF16) asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
 // The part of a sequence that a CTA works on.
 struct Work {
   int q0, len_q, k0, len_k;      // rows of the packed tensors
@@ -468,28 +477,40 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
         }
         parity ^= 1u << vu;
         const int live = min(seen - (w.first + i) * TILE_N, TILE_N);   // rows of the tile that count
-        uint32_t found = 0;
-#pragma unroll 4
-        for (int c = lane; c < C::V_UNIT_BYTES / 16; c += 32) {
-          const uint32_t addr = sV + vu * C::V_UNIT_BYTES + c * 16;
-          const int row = (c >> 3) & 127;
-          uint32_t x[4];
-          if (row >= live) {
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory");
-            continue;
+        // 32 chunks of 16 bytes (four rows of a block) at a time
+        constexpr int BATCH = 8;
+        const uint32_t mine = sV + vu * C::V_UNIT_BYTES + lane * 16;
+        uint32_t most = 0;                           // largest magnitude, pairwise; NaN stays
+        for (int c0 = 0; c0 < C::V_UNIT_BYTES / 512; c0 += BATCH) {
+          uint32_t x[BATCH][4];
+#pragma unroll
+          for (int k = 0; k < BATCH; ++k) {
+            const int row = ((c0 + k) * 4 + (lane >> 3)) & 127;
+            const uint32_t addr = mine + (c0 + k) * 512;
+            x[k][0] = x[k][1] = x[k][2] = x[k][3] = 0;
+            if (row < live)
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(x[k][0]), "=r"(x[k][1]), "=r"(x[k][2]), "=r"(x[k][3]) : "r"(addr) : "memory");
+            else
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory");
           }
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(addr) : "memory");
-          uint32_t f = 0;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) f |= not_finite2<BF16>(x[k]);
-          if (f) {
-            found = 1;
+          for (int k = 0; k < BATCH; ++k)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t h = not_finite2<BF16>(x[k]);
-              if (h & 0x8000u) x[k] &= 0xffff0000u;
-              if (h & 0x80000000u) x[k] &= 0x0000ffffu;
+            for (int q = 0; q < 4; ++q) most = abs_max2<BF16>(most, x[k][q]);
+        }
+        const bool found = not_finite2<BF16>(most) != 0;
+        if (found) {                                 // rare: clear them
+          for (int c = 0; c < C::V_UNIT_BYTES / 512; ++c) {
+            const uint32_t addr = mine + c * 512;
+            uint32_t x[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(addr) : "memory");
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t h = not_finite2<BF16>(x[q]);
+              if (h & 0x8000u) x[q] &= 0xffff0000u;
+              if (h & 0x80000000u) x[q] &= 0x0000ffffu;
             }
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
                          ::"r"(addr), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
