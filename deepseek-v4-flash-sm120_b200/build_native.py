@@ -17,7 +17,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.environ.get("DSV4_BUILD_OUT") or os.path.join(HERE, "deepseek_v4_kernel", "libdsv4_b200.so")
 SOURCES = ["capi.cu", "simple_kernels.cu", "umma_selftest.cu", "sparse_attn_sm100.cu",
-           "noalloc_entry.cu", "head_gather.cu", "paging.cu", "dense_attn_sm100.cu"]
+           "noalloc_entry.cu", "head_gather.cu", "paging.cu", "dense_attn_sm100.cu",
+           "shared_prefix_sm100.cu", "tensor_map.cu"]
 
 
 def _stale() -> bool:

@@ -322,31 +322,38 @@ int dsv4_sparse_prefill(const Dsv4PrefillArgs* a, void* stream) {
 
 // Splits of the two parts of a shared-prefix decode, and its scratch.
 struct SharedPlan {
-  int prefix_splits, suffix_splits;        // 0: the part does not exist
-  int64_t prefix_list, suffix_list;        // entries of the index lists
-  int64_t bytes;
+  int prefix_sets, suffix_splits;          // partial sets of the two parts; 0: the part does not exist
+  bool dense;                              // the prefix by launch_prefix_attn, else by an index list
+  int64_t prefix_bytes, suffix_bytes;      // of the workspace: the prefix's part, then the lists
 };
+// The dense form converts the whole prefix first and works in blocks of 128 rows; below this
+// many rows the list form, which reads the FP8 rows as they are, is faster.
+constexpr int64_t DENSE_PREFIX_ROWS = 65;
 static SharedPlan plan_shared(const Dsv4SharedPrefixArgs* a, int num_sms) {
   SharedPlan p{};
   const int64_t rows = static_cast<int64_t>(a->b) * a->s_q * a->h_q;
   const int64_t plen = static_cast<int64_t>(a->prefix_pages) * a->page_block_size;
   const int64_t slen = static_cast<int64_t>(a->max_pages) * a->page_block_size;
-  if (plen > 0)
-    p.prefix_splits = a->prefix_splits > 0 ? a->prefix_splits
-                                           : dsv4_plan_splits(1, 1, static_cast<int>(rows), static_cast<int>(plen), 0, num_sms);
+  p.dense = plen > 0 && a->prefix_splits == 0 && rows >= DENSE_PREFIX_ROWS && !want_simple(a->flags);
+  if (p.dense) {
+    p.prefix_sets = dsv4::prefix_attn_sets(rows, num_sms);
+    p.prefix_bytes = dsv4::prefix_attn_workspace(plen, a->d_qk);
+  } else if (plen > 0) {
+    p.prefix_sets = a->prefix_splits > 0 ? a->prefix_splits
+                                         : dsv4_plan_splits(1, 1, static_cast<int>(rows), static_cast<int>(plen), 0, num_sms);
+    p.prefix_bytes = (plen + 63) / 64 * 64 * 4;
+  }
   if (slen > 0)
     p.suffix_splits = a->suffix_splits > 0 ? a->suffix_splits
                                            : dsv4_plan_splits(a->b, a->s_q, a->h_q, static_cast<int>(slen), 0, num_sms);
-  p.prefix_list = plen;
-  p.suffix_list = slen * a->b * a->s_q;
-  p.bytes = (p.prefix_list + p.suffix_list) * 4;
+  p.suffix_bytes = slen * a->b * a->s_q * 4;
   return p;
 }
 
 static int check_shared(const Dsv4SharedPrefixArgs* a) {
   if (!a) return DSV4_ERR_NULL;
   if (a->b < 0 || a->s_q < 1 || a->h_q < 1 || a->num_blocks < 1 || a->page_block_size < 1 || a->d_v != dsv4::D_V ||
-      a->prefix_pages < 0 || a->max_pages < 0 || a->prefix_splits < 0 || a->suffix_splits < 0 ||
+      !(a->sm_scale > 0.0f) || !(a->sm_scale <= 3.0e38f) || a->prefix_pages < 0 || a->max_pages < 0 || a->prefix_splits < 0 || a->suffix_splits < 0 ||
       a->prefix_splits > 64 || a->suffix_splits > 64)
     return DSV4_ERR_SHAPE;
   const int64_t most = 0x7fffffff;
@@ -363,10 +370,10 @@ int dsv4_shared_prefix_scratch(const Dsv4SharedPrefixArgs* a, int num_sms, int32
   int rc = check_shared(a);
   if (rc) return rc;
   if (!sets || !bytes) return DSV4_ERR_NULL;
-  if (num_sms < 1) return DSV4_ERR_SHAPE;
+  if (num_sms < 2) return DSV4_ERR_SHAPE;
   const SharedPlan p = plan_shared(a, num_sms);
-  *sets = p.prefix_splits + p.suffix_splits;
-  *bytes = p.bytes;
+  *sets = p.prefix_sets + p.suffix_splits;
+  *bytes = p.prefix_bytes + p.suffix_bytes;
   return DSV4_OK;
 }
 
@@ -388,16 +395,17 @@ int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* a, void* stream) {
   DevInfo info;
   if ((rc = device_info(dev, info))) return rc;
   const SharedPlan plan = plan_shared(a, info.sms);
-  const int sets = plan.prefix_splits + plan.suffix_splits;
+  const int sets = plan.prefix_sets + plan.suffix_splits;
   if (sets > 0) {
     if (!a->o_accum || !a->lse_accum || !a->workspace) return DSV4_ERR_SCRATCH;
     if (!aligned16(a->o_accum) || !aligned16(a->workspace)) return DSV4_ERR_ALIGN;
   }
   const int64_t rows = static_cast<int64_t>(a->b) * a->s_q * a->h_q;
-  int32_t* prefix_list = static_cast<int32_t*>(a->workspace);
-  int32_t* suffix_list = prefix_list + plan.prefix_list;
+  int32_t* prefix_list = plan.dense ? nullptr : static_cast<int32_t*>(a->workspace);
+  int32_t* suffix_list = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(a->workspace) + plan.prefix_bytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if ((e = dsv4::launch_shared_lists(*a, prefix_list, suffix_list, st))) return cuda_fail(e);
+  if (plan.dense && (e = dsv4::launch_prefix_attn(*a, a->workspace, info.sms, st))) return cuda_fail(e);
 
   dsv4::AttnParams p{};
   p.cluster = 1;
@@ -419,12 +427,12 @@ int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* a, void* stream) {
     return want_simple(a->flags) ? dsv4::launch_simple_attn(p, a->kv_format, a->d_qk, st)
                                  : dsv4::launch_sm100_attn(p, a->kv_format, a->d_qk, st);
   };
-  if (plan.prefix_splits > 0) {
+  if (plan.prefix_sets > 0 && !plan.dense) {
     // the rows of all requests as the heads of one: each block of 64 rows walks the prefix once
     p.n_req = p.s_q = 1;
     p.h_q = static_cast<int>(rows);
-    p.topk = static_cast<int>(plan.prefix_list);
-    p.n_splits = plan.prefix_splits;
+    p.topk = a->prefix_pages * a->page_block_size;
+    p.n_splits = plan.prefix_sets;
     p.indices = prefix_list;
     p.topk_length = a->prefix_length;
     p.o_accum = a->o_accum;
@@ -443,8 +451,8 @@ int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* a, void* stream) {
     p.stride_q_b = p.stride_q_s * a->s_q;
     p.stride_idx_s = p.topk;
     p.stride_idx_b = static_cast<int64_t>(p.topk) * a->s_q;
-    p.o_accum = a->o_accum + plan.prefix_splits * rows * dsv4::D_V;
-    p.lse_accum = a->lse_accum + plan.prefix_splits * rows;
+    p.o_accum = a->o_accum + plan.prefix_sets * rows * dsv4::D_V;
+    p.lse_accum = a->lse_accum + plan.prefix_sets * rows;
     if ((e = attend())) return cuda_fail(e);
   }
   Dsv4CombineArgs c{};
@@ -598,6 +606,8 @@ int dsv4_device_status(int32_t* status_out, int reset) {
   if (e) return cuda_fail(e);
   int d = 0;
   if ((e = dsv4::read_dense_error(&d, reset != 0))) return cuda_fail(e);
+  if (v == 0) v = d;
+  if ((e = dsv4::read_prefix_error(&d, reset != 0))) return cuda_fail(e);
   if (v == 0) v = d;
   *status_out = v;
   return DSV4_OK;

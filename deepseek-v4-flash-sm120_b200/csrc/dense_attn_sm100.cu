@@ -29,7 +29,6 @@
 //
 // Few rows (single tokens over long contexts): the keys are cut into n_splits ranges, each
 // CTA leaves a normalised 32-bit partial, and dense_combine_kernel joins them.
-#include <cuda.h>
 #include <cuda_fp16.h>
 
 #include <mutex>
@@ -38,6 +37,7 @@
 #include "attn_params.cuh"
 #include "launchers.h"
 #include "sm100_ptx.cuh"
+#include "tensor_map.h"
 
 namespace dsv4 {
 
@@ -736,45 +736,6 @@ dense_combine_kernel(const __grid_constant__ DenseParams p) {
 constexpr int MAX_DEVICES = 64;
 std::mutex g_dense_mu;
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// The driver's tensor-map encoder, looked up once (the library links no driver library).
-cudaError_t encoder(EncodeTiled* out) {
-  std::lock_guard<std::mutex> lk(g_dense_mu);
-  static EncodeTiled fn = nullptr;
-  if (fn == nullptr) {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult st;
-    cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &st);
-    if (e) return e;
-    if (st != cudaDriverEntryPointSuccess || f == nullptr) return cudaErrorNotSupported;
-    fn = reinterpret_cast<EncodeTiled>(f);
-  }
-  *out = fn;
-  return cudaSuccess;
-}
-
-// Map of a [tokens, heads, d] tensor of 16-bit values with boxes of `box_t` tokens, `box_h`
-// heads and 64 values.
-cudaError_t make_map(CUtensorMap* m, bool bf16, const void* ptr, int tokens, int heads, int d, int64_t stride_t,
-                     int64_t stride_h, int box_t, int box_h) {
-  EncodeTiled enc;
-  cudaError_t e = encoder(&enc);
-  if (e) return e;
-  // the stride of a dimension of one element is never used, but has to be a legal one
-  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(heads > 1 ? stride_h : d) * 2,
-                                 static_cast<cuuint64_t>(tokens > 1 ? stride_t : d) * 2};
-  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_h), static_cast<cuuint32_t>(box_t)};
-  const cuuint32_t ones[3] = {1, 1, 1};
-  const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-                         const_cast<void*>(ptr), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
-}
-
 template <int DQK, int DV, bool BF16>
 cudaError_t launch_one(const DenseParams& p, cudaStream_t st) {
   constexpr size_t smem = dense_smem_bytes<DQK, DV>();
@@ -839,12 +800,12 @@ cudaError_t launch_dense_prefill(const Dsv4DensePrefillArgs& a, cudaStream_t st)
   p.stride_ml_t = a.stride_ml_t; p.stride_lse_t = a.stride_lse_t;
   p.o_accum = a.o_accum; p.stat_accum = a.stat_accum;
   cudaError_t e;
-  if ((e = make_map(&p.mq, bf16, a.q, a.t_q, a.h_q, a.d_qk, a.stride_q_t, a.stride_q_h, p.tok_tile, p.pack))) return e;
+  if ((e = make_map_16bit(&p.mq, bf16, a.q, a.t_q, a.h_q, a.d_qk, a.stride_q_t, a.stride_q_h, p.tok_tile, p.pack))) return e;
   // a batch without any key still needs legal maps: nothing is loaded through them
   const bool keys = a.t_k > 0;
-  if ((e = make_map(&p.mk, bf16, keys ? a.k : a.q, keys ? a.t_k : 1, keys ? a.h_kv : 1, a.d_qk,
+  if ((e = make_map_16bit(&p.mk, bf16, keys ? a.k : a.q, keys ? a.t_k : 1, keys ? a.h_kv : 1, a.d_qk,
                     a.stride_k_t, a.stride_k_h, TILE_N, 1))) return e;
-  if ((e = make_map(&p.mv, bf16, keys ? a.v : a.q, keys ? a.t_k : 1, keys ? a.h_kv : 1, a.d_v,
+  if ((e = make_map_16bit(&p.mv, bf16, keys ? a.v : a.q, keys ? a.t_k : 1, keys ? a.h_kv : 1, a.d_v,
                     a.stride_v_t, a.stride_v_h, TILE_N, 1))) return e;
   if (a.d_qk == 192) return bf16 ? launch_one<192, 128, true>(p, st) : launch_one<192, 128, false>(p, st);
   if (a.d_qk == 128) return bf16 ? launch_one<128, 128, true>(p, st) : launch_one<128, 128, false>(p, st);

@@ -43,8 +43,15 @@ cudaError_t launch_slot_maps(const Dsv4SlotMapArgs& a, cudaStream_t st);
 cudaError_t launch_page_indices(const Dsv4PageIndicesArgs& a, cudaStream_t st);
 // Token indices of the first length[0] tokens of one table row (`prefix`), and of every
 // request's own tokens as each of its s_q query tokens sees them (`suffix`, one list of
-// max_pages * page tokens per query token).
+// max_pages * page tokens per query token).  A null `prefix` leaves that part out.
 cudaError_t launch_shared_lists(const Dsv4SharedPrefixArgs& a, int32_t* prefix, int32_t* suffix, cudaStream_t st);
+
+// Attention of many rows over a shared prefix, into the first prefix_attn_sets partial sets
+// (shared_prefix_sm100.cu).
+int prefix_attn_sets(int64_t rows, int num_sms);
+int64_t prefix_attn_workspace(int64_t tokens, int d_qk);       // bytes
+cudaError_t launch_prefix_attn(const Dsv4SharedPrefixArgs& a, void* workspace, int num_sms, cudaStream_t st);
+cudaError_t read_prefix_error(int* value, bool reset);
 
 // Dense attention over packed sequences (dense_attn_sm100.cu).
 constexpr int DENSE_MAX_SPLITS = 64;

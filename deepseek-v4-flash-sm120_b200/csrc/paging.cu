@@ -256,7 +256,7 @@ std::mutex g_paging_mu;
 
 cudaError_t launch_shared_lists(const Dsv4SharedPrefixArgs& a, int32_t* prefix, int32_t* suffix, cudaStream_t st) {
   const int64_t n = static_cast<int64_t>(a.prefix_pages) * a.page_block_size;
-  const int prefix_ctas = static_cast<int>(n < 64 * 1024 ? (n + 1023) / 1024 : 64);
+  const int prefix_ctas = prefix == nullptr ? 0 : static_cast<int>(n < 64 * 1024 ? (n + 1023) / 1024 : 64);
   const int rows = a.max_pages > 0 ? a.b * a.s_q : 0;
   if (prefix_ctas + rows == 0) return cudaSuccess;
   cudaLaunchConfig_t cfg = {};

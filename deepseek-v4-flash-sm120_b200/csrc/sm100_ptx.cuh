@@ -71,6 +71,26 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
   }
   return true;
 }
+// The same for a barrier on which other CTAs of the cluster arrive.
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t n = 0;
+  uint64_t t0 = 0;
+#pragma unroll 1
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
+    if ((++n & 255u) == 0) {
+      const uint64_t now = global_timer_ns();
+      if (t0 == 0) t0 = now;
+      else if (now - t0 > 50000000ull) return false;
+    }
+  }
+}
 // The same for a whole warp: lane 0 waits, the result is broadcast.  Keeps the number
 // of waiters on shared memory at one per warp.
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, int lane) {

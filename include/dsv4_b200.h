@@ -279,7 +279,8 @@ int dsv4_sparse_prefill(const Dsv4PrefillArgs* args, void* cuda_stream);
  *
  * q rows are dense: stride_q_h = d_qk, [b, s_q, h_q] contiguous.  Scratch, sized by
  * dsv4_shared_prefix_scratch(args): o_accum fp32 [sets, b, s_q, h_q, 512], lse_accum fp32
- * [sets, b, s_q, h_q], workspace bytes.  num_blocks * page_block_size < 2^31.                */
+ * [sets, b, s_q, h_q], workspace bytes.  num_blocks * page_block_size < 2^31; sm_scale is
+ * positive and finite.                                                                      */
 typedef struct Dsv4SharedPrefixArgs {
   int32_t b, s_q, h_q, d_qk, d_v;
   int32_t kv_format;            /* DSV4_KV_MODEL1 or DSV4_KV_V32                 */
