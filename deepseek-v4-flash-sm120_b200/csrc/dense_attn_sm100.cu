@@ -367,14 +367,14 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
         for (int i = 0; i < n_tiles && ok; ++i) {
           const int row = w.k0 + (w.first + i) * TILE_N;
           for (int c = 0; c < C::QB; c += C::K_STEP) {
-            if (!mbar_wait(bar(&ctrl.k_empty[ks]), kphase ^ 1)) { gave_up(ERR_SLOT); ok = false; break; }
+            if (!mbar_wait_fast(bar(&ctrl.k_empty[ks]), kphase ^ 1)) { gave_up(ERR_SLOT); ok = false; break; }
             mbar_expect_tx(bar(&ctrl.k_full[ks]), C::K_STEP * BLOCK_BYTES);
             for (int d = 0; d < C::K_STEP; ++d)
               tma_load_3d(sK + (ks * C::K_STEP + d) * BLOCK_BYTES, &p.mk, 64 * (c + d), kvh, row, bar(&ctrl.k_full[ks]));
             if (++ks == C::K_RING) { ks = 0; kphase ^= 1; }
           }
           if (i == 0 && w.count[1] > 0) load_q(1);
-          if (!ok || !mbar_wait(bar(&ctrl.v_empty[vu]), vphase ^ 1)) { gave_up(ERR_SLOT); break; }
+          if (!ok || !mbar_wait_fast(bar(&ctrl.v_empty[vu]), vphase ^ 1)) { gave_up(ERR_SLOT); break; }
           const uint32_t landed = bar(w.first + i >= w.look ? &ctrl.v_look[vu] : &ctrl.v_full[vu]);
           mbar_expect_tx(landed, C::V_UNIT_BYTES);
           for (int c = 0; c < C::VB; ++c)
@@ -395,7 +395,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
       const uint32_t elected = elect_one();
       bool ok = true;
       auto wait = [&](uint64_t* b, int parity, int code) {
-        if (ok && !mbar_wait(bar(b), parity)) {
+        if (ok && !mbar_wait_fast(bar(b), parity)) {
           if (lane == 0) gave_up(code);
           ok = false;
         }
@@ -471,7 +471,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
       uint32_t parity = 0;
       for (int i = max(w.look - w.first, 0); i < n_tiles; ++i) {
         const int vu = i % C::V_UNITS;
-        if (!mbar_wait_warp(bar(&ctrl.v_look[vu]), (parity >> vu) & 1, lane)) {
+        if (!mbar_wait_fast(bar(&ctrl.v_look[vu]), (parity >> vu) & 1)) {
           if (lane == 0) gave_up(ERR_V);
           break;
         }
@@ -550,7 +550,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   bool ok = true;
 #pragma unroll 1
   for (int i = 0; i < n_mine; ++i) {
-    if (!mbar_wait(bar(&ctrl.s_full[s]), i & 1)) { gave_up(ERR_S); ok = false; break; }
+    if (!mbar_wait_fast(bar(&ctrl.s_full[s]), i & 1)) { gave_up(ERR_S); ok = false; break; }
     tc_fence_after_sync();
     uint32_t x[TILE_N];
 #pragma unroll
@@ -581,7 +581,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     }
     // the product of the tile before has read P, and O is its result
     if (i > 0) {
-      if (!mbar_wait(bar(&ctrl.o_done[s]), (i - 1) & 1)) { gave_up(ERR_O); ok = false; break; }
+      if (!mbar_wait_fast(bar(&ctrl.o_done[s]), (i - 1) & 1)) { gave_up(ERR_O); ok = false; break; }
       tc_fence_after_sync();
     }
     if (i > 0 && __any_sync(0xffffffffu, raise)) {
@@ -636,7 +636,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   grid_launch_dependents();
 
   // ---- epilogue --------------------------------------------------------------------------
-  if (n_mine > 0 && ok && !mbar_wait(bar(&ctrl.o_done[s]), (n_mine - 1) & 1)) { gave_up(ERR_O); ok = false; }
+  if (n_mine > 0 && ok && !mbar_wait_fast(bar(&ctrl.o_done[s]), (n_mine - 1) & 1)) { gave_up(ERR_O); ok = false; }
   tc_fence_after_sync();
   const bool fail = !ok || *reinterpret_cast<volatile int*>(&ctrl.fail) != 0;
   const int64_t t = static_cast<int64_t>(w.q0) + tok;

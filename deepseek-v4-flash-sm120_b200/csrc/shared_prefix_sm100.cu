@@ -44,9 +44,10 @@ using namespace ptx;
 
 constexpr int ROWS = 64;                        // query rows of a CTA
 constexpr int TILE = 128;                       // tokens
-constexpr int THREADS = 256;                    // 4 softmax warps and 4 that issue and load
-constexpr int SOFTMAX_THREADS = 128;
-constexpr int WARP_QK = 4, WARP_PV = 5, WARP_LOAD_K = 6, WARP_LOAD_V = 7;
+constexpr int GROUP = 128, SOFTMAX_THREADS = 2 * GROUP;         // two softmax warpgroups
+constexpr int THREADS = SOFTMAX_THREADS + 128;                  // and four warps that issue and load
+constexpr int WARP_QK = 8, WARP_PV = 9, WARP_LOAD_K = 10, WARP_LOAD_V = 11;
+constexpr int BAR_BOTH = 1, BAR_DECIDED = 2, BAR_GROUP = 4;     // named barriers (2 and 3, 4 and 5)
 constexpr int QK_BLOCK = ROWS * 128;            // [64 rows or tokens][64 values]: 8 KB
 constexpr int V_BLOCK = TILE * 128;             // [128 tokens][64 columns]: 16 KB
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -65,12 +66,13 @@ template <int DQK> struct PCfg {
 
 struct PrefixCtrl {
   // of this CTA: TMA, or a commit of the leader's products, arrives
-  uint64_t q_land, k_land[4], v_land[2], k_empty[4], v_empty[2], s_full[2], o_done;
+  uint64_t q_land, k_land[4], v_land[2], k_empty[4], v_empty[2], s_full[2], o_done[2];
   // of the leader: what the other CTA, or the softmax warps of both, report
   uint64_t q_peer, k_peer[4], v_peer[2], s_free[2], p_full, o_free;
   uint32_t tmem;
   int fail;
-  alignas(16) float top[2][ROWS], sum[2][ROWS];
+  alignas(16) float ref[ROWS];
+  float part[4][ROWS];           // by group and half: a tile's maxima; at a segment's end the sums
 };
 
 template <int DQK> constexpr size_t prefix_smem_bytes() {
@@ -97,11 +99,15 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Arrive on the leader's barrier at the same offset as `bar` here.
+// Arrive on the leader's barrier at the same offset as `bar` here.  What it reports is read by
+// the tensor core alone, out of the reporting CTA's own shared memory and TMEM: rows that TMA
+// brought (the reporter has waited for them), P (written here, then fence.proxy.async) or TMEM
+// (tcgen05 fences).  No thread reads another CTA's memory, so the arrival releases at CTA scope;
+// releasing and acquiring at cluster scope took 270 to 1300 clk each.
 __device__ __forceinline__ void arrive_leader(uint32_t bar) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(bar));
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
 }
 __device__ __forceinline__ void umma2(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t elected) {
   asm volatile(
@@ -186,10 +192,10 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
         mbar_init(bar(&ctrl.v_empty[h]), 1);
         mbar_init(bar(&ctrl.s_full[h]), 1);
         mbar_init(bar(&ctrl.s_free[h]), 8);      // four softmax warps of each CTA
+        mbar_init(bar(&ctrl.o_done[h]), 1);
       }
-      mbar_init(bar(&ctrl.o_done), 1);
       mbar_init(bar(&ctrl.p_full), 8);
-      mbar_init(bar(&ctrl.o_free), 8);
+      mbar_init(bar(&ctrl.o_free), 16);
       ctrl.fail = 0;
       mbar_init_fence();
     }
@@ -216,7 +222,7 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
 
   if (warp >= WARP_QK) {
     auto wait = [&](uint64_t* b, int parity, int code) {
-      if (ok && !mbar_wait_cluster(bar(b), parity)) {
+      if (ok && !mbar_wait_fast(bar(b), parity)) {
         if (lane == 0) gave_up(code);
         ok = false;
       }
@@ -351,35 +357,48 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
                     dV + ((2 * h * V_BLOCK + k * 2048) >> 4), idesc, (i | k) != 0, elected);
             commit2(bar(&ctrl.v_empty[h]), elected);
           }
-          if (ok) commit2(bar(&ctrl.o_done), elected);
+          if (ok) commit2(bar(&ctrl.o_done[n & 1]), elected);
         }
       }
     }
   } else {
     // ======================= softmax =======================================================
-    // Lane l of the CTA's 128: row l & 63, tokens [64 * (l >> 6), +64) of the tile.
-    const int r = tid & 63, half = tid >> 6;
-    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+    // The two warpgroups take the tiles in turn (tile n: group n & 1), so that one's waits and
+    // stores hide behind the other's arithmetic.  Thread l of a group: row l & 63, tokens
+    // [64 * (l >> 6), +64) of the tile.  The rows' reference maxima are common (they scale O):
+    // a group decides about raising them once the other one has decided for the tile before.
+    const int group = tid >> 7, r = tid & 63, half = (tid >> 6) & 1;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const float c = p.sm_scale * LOG2E;
     const uint32_t prow = sP + half * QK_BLOCK + r * 128;
     auto wait = [&](uint64_t* b, int parity, int code) {
-      if (ok && !mbar_wait_cluster(bar(b), parity)) gave_up(code);
+      if (ok && !mbar_wait_fast(bar(b), parity)) gave_up(code);
     };
+    const int64_t total_tiles = w.end - w.at;
     int n = 0;
     while (w.next()) {
-      float m_ref = -INFINITY, l = 0.f;
+      if (tid < ROWS) ctrl.ref[tid] = -INFINITY;
+      bar_sync(BAR_BOTH, SOFTMAX_THREADS);
+      float m_ref = -INFINITY, l = 0.f;            // l is relative to m_ref
+      const uint2* bits = reinterpret_cast<const uint2*>(p.valid) + w.first * 2 + half;
+      const int mine = (n & 1) == group ? 0 : 1;   // this group's first tile of the segment
+      uint2 ahead = make_uint2(0u, 0u);
+      if (mine < w.count) ahead = __ldg(bits + 2 * mine);
+      const int n0 = n;                            // tiles of the segments before
 #pragma unroll 1
-      for (int i = 0; i < w.count; ++i, ++n) {
-        const uint2 seen = __ldg(reinterpret_cast<const uint2*>(p.valid + (w.first + i) * 4 + half * 2));
-        wait(&ctrl.s_full[n & 1], (n >> 1) & 1, ERR_S);
+      for (int i = mine; i < w.count; i += 2) {
+        n = n0 + i;
+        const uint2 seen = ahead;
+        if (i + 2 < w.count) ahead = __ldg(bits + 2 * (i + 2));
+        wait(&ctrl.s_full[group], (n >> 1) & 1, ERR_S);
         tc_fence_after_sync();
         uint32_t x[64];
-        tmem_ld32(tmem + lanes + COL_S + 64 * (n & 1), x);
-        tmem_ld32(tmem + lanes + COL_S + 64 * (n & 1) + 32, x + 32);
+        tmem_ld32(tmem + lanes + COL_S + 64 * group, x);
+        tmem_ld32(tmem + lanes + COL_S + 64 * group + 32, x + 32);
         tmem_ld_wait();
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) arrive_leader(bar(&ctrl.s_free[n & 1]));
+        if (lane == 0) arrive_leader(bar(&ctrl.s_free[group]));
         if ((seen.x & seen.y) != 0xffffffffu) {
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
@@ -391,20 +410,23 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
 #pragma unroll
         for (int k = 0; k < 64; ++k) mx[k & 3] = fmaxf(mx[k & 3], __uint_as_float(x[k]));
         const float top2 = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
-        if (bar_red_or(1, SOFTMAX_THREADS, top2 > m_ref + RESCALE_THRESHOLD)) {
+
+        if (n > 0) bar_sync(BAR_DECIDED + (group ^ 1), SOFTMAX_THREADS);
+        float ref = ctrl.ref[r];
+        if (bar_red_or(BAR_GROUP + group, GROUP, top2 > ref + RESCALE_THRESHOLD)) {
           // some row's reference is raised (always in a segment's first tile)
-          ctrl.top[half][r] = top2;
-          bar_sync(1, SOFTMAX_THREADS);
-          const float both = fmaxf(top2, ctrl.top[half ^ 1][r]);
-          bar_sync(1, SOFTMAX_THREADS);          // read before the next tile writes
+          ctrl.part[2 * group + half][r] = top2;
+          bar_sync(BAR_GROUP + group, GROUP);
+          const float both = fmaxf(top2, ctrl.part[2 * group + (half ^ 1)][r]);
           float alpha = 1.f;
-          if (both > m_ref + RESCALE_THRESHOLD) {
-            alpha = ex2(m_ref - both);           // 0 for the first
-            m_ref = both;
-            l *= alpha;
+          if (both > ref + RESCALE_THRESHOLD) {
+            alpha = ex2(ref - both);               // 0 for the first
+            ref = both;
           }
+          bar_sync(BAR_GROUP + group, GROUP);      // both threads of a row have read the old one
+          if (half == 0) ctrl.ref[r] = ref;
           if (i > 0) {
-            wait(&ctrl.o_done, (n - 1) & 1, ERR_O);
+            wait(&ctrl.o_done[group ^ 1], ((n - 1) >> 1) & 1, ERR_O);
             tc_fence_after_sync();
             if (__any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
@@ -420,19 +442,25 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
             }
           }
         }
-        const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+        if (n + 1 < total_tiles) bar_arrive(BAR_DECIDED + group, SOFTMAX_THREADS);
+        if (ref != m_ref) {                        // raised here or by the other group
+          l *= ex2(m_ref - ref);
+          m_ref = ref;
+        }
+        const float sub = ref == -INFINITY ? 0.f : ref;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
         uint32_t pk[32];
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
-          const float a = ex2(fmaf(__uint_as_float(x[2 * k]), c, -ref));
-          const float b = ex2(fmaf(__uint_as_float(x[2 * k + 1]), c, -ref));
+          const float a = ex2(fmaf(__uint_as_float(x[2 * k]), c, -sub));
+          const float b = ex2(fmaf(__uint_as_float(x[2 * k + 1]), c, -sub));
           sum[(2 * k) & 3] += a;
           sum[(2 * k + 1) & 3] += b;
           pk[k] = pack_bf16x2(a, b);
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (n > 0) wait(&ctrl.o_done, (n - 1) & 1, ERR_O);       // P V of the tile before has read P
+        // P V of the tile before has read P
+        if (n > 0) wait(&ctrl.o_done[group ^ 1], ((n - 1) >> 1) & 1, ERR_O);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(prow + ((k ^ (r & 7)) << 4)), "r"(pk[4 * k]),
@@ -442,35 +470,39 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
         __syncwarp();
         if (lane == 0) arrive_leader(bar(&ctrl.p_full));
       }
+      n = n0 + w.count;
       // ---- the segment's partial ------------------------------------------------------------
-      ctrl.sum[half][r] = l;
-      bar_sync(1, SOFTMAX_THREADS);
-      const float total = l + ctrl.sum[half ^ 1][r];
-      bar_sync(1, SOFTMAX_THREADS);
-      wait(&ctrl.o_done, (n - 1) & 1, ERR_O);
+      bar_sync(BAR_BOTH, SOFTMAX_THREADS);         // every decision has been made
+      const float ref = ctrl.ref[r];
+      if (ref != m_ref) l *= ex2(m_ref - ref);
+      ctrl.part[2 * group + half][r] = l;
+      bar_sync(BAR_BOTH, SOFTMAX_THREADS);
+      const float total = (ctrl.part[0][r] + ctrl.part[1][r]) + (ctrl.part[2][r] + ctrl.part[3][r]);
+      wait(&ctrl.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1, ERR_O);
       tc_fence_after_sync();
       const bool fail = *reinterpret_cast<volatile int*>(&ctrl.fail) != 0;
       const int row = w.block * 2 * ROWS + rank * ROWS + r;
       const bool none = total == 0.f;
       const float f = none ? 0.f : 1.f / total;
-      if (half == 0 && row < p.rows) {
-        p.lse_accum[static_cast<int64_t>(w.set) * p.rows + row] = fail ? NAN : none ? -INFINITY : logf(total) + m_ref * LN2;
+      if (group == 0 && half == 0 && row < p.rows) {
+        p.lse_accum[static_cast<int64_t>(w.set) * p.rows + row] = fail ? NAN : none ? -INFINITY : logf(total) + ref * LN2;
         if (w.last)
           for (int s = w.set + 1; s < p.sets; ++s) p.lse_accum[static_cast<int64_t>(s) * p.rows + row] = -INFINITY;
       }
-      float* dst = p.o_accum + (static_cast<int64_t>(w.set) * p.rows + row) * D_V + half * 128;
+      // each group writes the 256 columns of one product
+      float* dst = p.o_accum + (static_cast<int64_t>(w.set) * p.rows + row) * D_V + group * 256 + half * 128;
 #pragma unroll 1
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 4; ++k) {
         uint32_t o[32];
-        tmem_ld32(tmem + lanes + COL_O + 32 * k, o);             // warp-collective
+        tmem_ld32(tmem + lanes + COL_O + 128 * group + 32 * k, o);             // warp-collective
         tmem_ld_wait();
-        if (k == 7) {
+        if (k == 3) {
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) arrive_leader(bar(&ctrl.o_free));
         }
         if (row < p.rows && !fail) {
-          float4* d = reinterpret_cast<float4*>(dst + (k >> 2) * 256 + (k & 3) * 32);
+          float4* d = reinterpret_cast<float4*>(dst + 32 * k);
 #pragma unroll
           for (int q = 0; q < 8; ++q)
             d[q] = make_float4(__uint_as_float(o[4 * q]) * f, __uint_as_float(o[4 * q + 1]) * f,
