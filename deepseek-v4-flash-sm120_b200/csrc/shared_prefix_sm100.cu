@@ -65,10 +65,10 @@ template <int DQK> struct PCfg {
 };
 
 struct PrefixCtrl {
-  // of this CTA: TMA, or a commit of the leader's products, arrives
-  uint64_t q_land, k_land[4], v_land[2], k_empty[4], v_empty[2], s_full[2], o_done[2];
-  // of the leader: what the other CTA, or the softmax warps of both, report
-  uint64_t q_peer, k_peer[4], v_peer[2], s_free[2], p_full, o_free;
+  // of each CTA: a commit of the leader's products arrives
+  uint64_t k_empty[4], v_empty[2], s_full[2], o_done[2];
+  // of the leader: the TMA loads of both CTAs, or the softmax warps of both, report
+  uint64_t q_land, k_land[4], v_land[2], s_free[2], p_full, o_free;
   uint32_t tmem;
   int fail;
   alignas(16) float ref[ROWS];
@@ -99,15 +99,26 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Arrive on the leader's barrier at the same offset as `bar` here.  What it reports is read by
-// the tensor core alone, out of the reporting CTA's own shared memory and TMEM: rows that TMA
-// brought (the reporter has waited for them), P (written here, then fence.proxy.async) or TMEM
-// (tcgen05 fences).  No thread reads another CTA's memory, so the arrival releases at CTA scope;
-// releasing and acquiring at cluster scope took 270 to 1300 clk each.
-__device__ __forceinline__ void arrive_leader(uint32_t bar) {
+// The leader's barrier at the same offset as `bar` here.
+__device__ __forceinline__ uint32_t of_leader(uint32_t bar) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(bar));
+  return a;
+}
+// Arrive on the leader's barrier.  What the softmax warps report is read by the tensor core
+// alone, out of the reporting CTA's own shared memory and TMEM: P (written, then
+// fence.proxy.async) or TMEM (tcgen05 fences).  No thread reads another CTA's memory, so the
+// arrival releases at CTA scope; releasing and acquiring at cluster scope took 270 to 1300 clk.
+__device__ __forceinline__ void arrive_leader(uint32_t bar) {
+  const uint32_t a = of_leader(bar);
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
+}
+// A box into this CTA's shared memory, reported to a barrier of either CTA of the pair.
+__device__ __forceinline__ void load_pair(uint32_t dst, const void* map, int x, int y, int z, uint32_t cluster_bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(cluster_bar) : "memory");
 }
 __device__ __forceinline__ void umma2(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t elected) {
   asm volatile(
@@ -180,15 +191,12 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
   if (warp == WARP_QK) {
     if (lane == 0) {
       mbar_init(bar(&ctrl.q_land), 1);
-      mbar_init(bar(&ctrl.q_peer), 1);
       for (int g = 0; g < 4; ++g) {
         mbar_init(bar(&ctrl.k_land[g]), 1);
-        mbar_init(bar(&ctrl.k_peer[g]), 1);
         mbar_init(bar(&ctrl.k_empty[g]), 1);
       }
       for (int h = 0; h < 2; ++h) {
         mbar_init(bar(&ctrl.v_land[h]), 1);
-        mbar_init(bar(&ctrl.v_peer[h]), 1);
         mbar_init(bar(&ctrl.v_empty[h]), 1);
         mbar_init(bar(&ctrl.s_full[h]), 1);
         mbar_init(bar(&ctrl.s_free[h]), 8);      // four softmax warps of each CTA
@@ -231,7 +239,7 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
     if (warp == WARP_LOAD_K) {
       // ======================= Q and K ======================================================
       const uint32_t elected = elect_one();
-      int n = 0, seg = 0;
+      int n = 0;
       while (ok && w.next()) {
         for (int i = 0; i < w.count && ok; ++i, ++n) {
           if (i == 0) {
@@ -239,20 +247,19 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
             for (int g = 0; g < C::GROUPS; ++g) wait(&ctrl.k_empty[g], (n & 1) ^ 1, ERR_SLOT);
             if (!ok) break;
             if (elected) {
-              mbar_expect_tx(bar(&ctrl.q_land), C::Q_BYTES);
+              if (rank == 0) mbar_expect_tx(bar(&ctrl.q_land), 2 * C::Q_BYTES);
               for (int c = 0; c < C::NB; ++c)
-                tma_load_3d(sQ + c * QK_BLOCK, &p.mq, 64 * c, 0, w.block * 2 * ROWS + rank * ROWS, bar(&ctrl.q_land));
+                load_pair(sQ + c * QK_BLOCK, &p.mq, 64 * c, 0, w.block * 2 * ROWS + rank * ROWS, of_leader(bar(&ctrl.q_land)));
             }
-            ++seg;
           }
           const int tok = (w.first + i) * TILE + rank * ROWS;
           for (int g = 0; g < C::GROUPS; ++g) {
             wait(&ctrl.k_empty[g], (n & 1) ^ 1, ERR_SLOT);
             if (!ok) break;
             if (elected) {
-              mbar_expect_tx(bar(&ctrl.k_land[g]), C::PER * QK_BLOCK);
+              if (rank == 0) mbar_expect_tx(bar(&ctrl.k_land[g]), 2 * C::PER * QK_BLOCK);
               for (int c = g * C::PER; c < (g + 1) * C::PER; ++c)
-                tma_load_3d(sK + c * QK_BLOCK, &p.mk, 64 * c, 0, tok, bar(&ctrl.k_land[g]));
+                load_pair(sK + c * QK_BLOCK, &p.mk, 64 * c, 0, tok, of_leader(bar(&ctrl.k_land[g])));
             }
           }
         }
@@ -268,36 +275,15 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
             wait(&ctrl.v_empty[h], (n & 1) ^ 1, ERR_SLOT);
             if (!ok) break;
             if (elected) {
-              mbar_expect_tx(bar(&ctrl.v_land[h]), 2 * V_BLOCK);
+              if (rank == 0) mbar_expect_tx(bar(&ctrl.v_land[h]), 4 * V_BLOCK);
               for (int c = 0; c < 2; ++c)
-                tma_load_3d(sV + (2 * h + c) * V_BLOCK, &p.mv, 256 * h + 128 * rank + 64 * c, 0, tok, bar(&ctrl.v_land[h]));
+                load_pair(sV + (2 * h + c) * V_BLOCK, &p.mv, 256 * h + 128 * rank + 64 * c, 0, tok, of_leader(bar(&ctrl.v_land[h])));
             }
           }
         }
       }
     } else if (rank != 0) {
-      // ======================= tell the leader what has landed here ========================
-      int n = 0, seg = 0;
-      while (ok && w.next()) {
-        if (warp == WARP_QK) {
-          wait(&ctrl.q_land, seg & 1, ERR_Q);
-          if (lane == 0 && ok) arrive_leader(bar(&ctrl.q_peer));
-          ++seg;
-        }
-        for (int i = 0; i < w.count && ok; ++i, ++n) {
-          if (warp == WARP_QK) {
-            for (int g = 0; g < C::GROUPS; ++g) {
-              wait(&ctrl.k_land[g], n & 1, ERR_K);
-              if (lane == 0 && ok) arrive_leader(bar(&ctrl.k_peer[g]));
-            }
-          } else {
-            for (int h = 0; h < 2; ++h) {
-              wait(&ctrl.v_land[h], n & 1, ERR_V);
-              if (lane == 0 && ok) arrive_leader(bar(&ctrl.v_peer[h]));
-            }
-          }
-        }
-      }
+      // the leader issues the products of both CTAs
     } else if (warp == WARP_QK) {
       // ======================= scores (leader) ==============================================
       constexpr uint32_t idesc = make_idesc_bf16(128, TILE, 0, 0);
@@ -307,7 +293,6 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
       int n = 0, seg = 0;
       while (ok && w.next()) {
         wait(&ctrl.q_land, seg & 1, ERR_Q);
-        wait(&ctrl.q_peer, seg & 1, ERR_Q);
         ++seg;
         const int count = __shfl_sync(0xffffffffu, w.count, 0);
 #pragma unroll 1
@@ -317,7 +302,6 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
 #pragma unroll
           for (int g = 0; g < C::GROUPS; ++g) {
             wait(&ctrl.k_land[g], n & 1, ERR_K);
-            wait(&ctrl.k_peer[g], n & 1, ERR_K);
             if (!ok) break;
             tc_fence_after_sync();
 #pragma unroll
@@ -348,7 +332,6 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             wait(&ctrl.v_land[h], n & 1, ERR_V);
-            wait(&ctrl.v_peer[h], n & 1, ERR_V);
             if (!ok) break;
             tc_fence_after_sync();
 #pragma unroll
