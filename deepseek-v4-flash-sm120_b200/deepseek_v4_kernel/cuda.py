@@ -11,6 +11,7 @@ fallback path: without the native library this module cannot be imported.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 from typing import Optional, Tuple
@@ -19,6 +20,7 @@ import torch
 
 from . import _native as N
 
+_DENSE_DTYPES = {torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_FP16}
 _KV_DTYPES = (torch.float8_e4m3fn, torch.uint8, torch.int8)
 _SCHED_META_INT32S = 8        # 32-byte record kept for FlashMLA binary parity
 _sm_count = {}
@@ -31,6 +33,30 @@ def _require(cond: bool, msg: str) -> None:
 
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
+
+
+# The serving operators below are called for a few microseconds of GPU work each, so their host
+# cost counts: checks that build no message unless they fail, no context for the current device,
+# and the stream as the plain handle.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(index: int) -> int:
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _current(index: int):
+    """Context that makes device `index` current; nothing when it is already."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def _int32(name, t, index, dim, dense_rows=False) -> None:
+    """Refuse anything but an int32 tensor of `dim` dimensions on CUDA device `index`: contiguous,
+    or (dense_rows) dense in the last dimension."""
+    if t.dtype != torch.int32 or t.dim() != dim or t.get_device() != index:
+        raise RuntimeError(f"{name} must be {dim}-D int32 on cuda:{index}")
+    if not (t.is_contiguous() or (dense_rows and (t.size(-1) <= 1 or t.stride(-1) == 1))):
+        raise RuntimeError(f"{name} must be {'dense in the last dim' if dense_rows else 'contiguous'}")
 
 
 def num_sms(device: torch.device) -> int:
@@ -255,56 +281,57 @@ def shared_prefix_decode_fwd(q, kv, prefix_table, prefix_length, block_table, su
     cache are masked.  The lengths stay on the device, so a captured call can be replayed
     with others.  `prefix_splits` / `suffix_splits` / `flags` are test hooks.  No counterpart
     in the reference."""
-    _require(q.is_cuda and kv.device == q.device, "q and kv must be CUDA tensors of one device")
-    _require(q.dim() == 4 and q.dtype == torch.bfloat16 and q.is_contiguous(),
-             "q must be contiguous bf16 [b, s_q, h_q, d_qk]")
-    _require(kv.dim() == 4 and kv.dtype in _KV_DTYPES and kv.size(2) == 1,
-             "kv must be [num_blocks, page_block, 1, bytes] fp8_e4m3 / uint8 / int8")
+    if not (q.is_cuda and kv.get_device() == q.get_device()):
+        raise RuntimeError("q and kv must be CUDA tensors of one device")
+    if q.dim() != 4 or q.dtype != torch.bfloat16 or not q.is_contiguous():
+        raise RuntimeError("q must be contiguous bf16 [b, s_q, h_q, d_qk]")
+    if kv.dim() != 4 or kv.dtype not in _KV_DTYPES or kv.size(2) != 1:
+        raise RuntimeError("kv must be [num_blocks, page_block, 1, bytes] fp8_e4m3 / uint8 / int8")
     b, s_q, h_q, d_qk = q.shape
     num_blocks, page_block, _, token_bytes = kv.shape
     fmt = _kv_format(d_qk, token_bytes)
-    _require(int(d_v) == 512, "Only d_v=512 supported")
-    _require(kv.stride(1) == token_bytes and kv.stride(3) == 1,
-             "kv pages must be dense (only the page stride may be padded)")
-    dev = q.device
-    _int32_on("prefix_table", prefix_table, dev, 1)
-    _int32_on("prefix_length", prefix_length, dev, 1)
-    _int32_on("block_table", block_table, dev, 2)
-    _int32_on("suffix_length", suffix_length, dev, 1)
-    _require(prefix_length.numel() == 1 and prefix_table.is_contiguous(), "prefix_length [1], prefix_table contiguous expected")
-    _require(block_table.size(0) == b and suffix_length.numel() == b and suffix_length.is_contiguous(),
-             f"block_table [{b}, max_pages] and contiguous suffix_length [{b}] expected")
-    max_pages = block_table.size(1)
-    _require(max_pages <= 1 or block_table.stride(1) == 1, "block_table rows must be dense")
-    if attn_sink is not None:
-        _require(attn_sink.dtype == torch.float32 and attn_sink.numel() == h_q and attn_sink.is_contiguous()
-                 and attn_sink.device == dev, "attn_sink must be contiguous float32 [h_q]")
-    with torch.cuda.device(dev):
-        out = torch.empty((b, s_q, h_q, 512), dtype=torch.bfloat16, device=dev)
-        lse = torch.empty((b, h_q, s_q), dtype=torch.float32, device=dev)
+    if int(d_v) != 512:
+        raise RuntimeError("Only d_v=512 supported")
+    kv_strides = kv.stride()
+    if (page_block > 1 and kv_strides[1] != token_bytes) or kv_strides[3] != 1:
+        raise RuntimeError("kv pages must be dense (only the page stride may be padded)")
+    idx = q.get_device()
+    _int32("prefix_table", prefix_table, idx, 1)
+    _int32("prefix_length", prefix_length, idx, 1)
+    _int32("block_table", block_table, idx, 2, dense_rows=True)
+    _int32("suffix_length", suffix_length, idx, 1)
+    if prefix_length.numel() != 1 or block_table.size(0) != b or suffix_length.numel() != b:
+        raise RuntimeError(f"prefix_length [1], block_table [{b}, max_pages] and suffix_length [{b}] expected")
+    if attn_sink is not None and not (attn_sink.dtype == torch.float32 and attn_sink.numel() == h_q
+                                      and attn_sink.is_contiguous() and attn_sink.get_device() == idx):
+        raise RuntimeError("attn_sink must be contiguous float32 [h_q]")
+    with _current(idx):
+        out = q.new_empty((b, s_q, h_q, 512))
+        lse = q.new_empty((b, h_q, s_q), dtype=torch.float32)
+        if b == 0:
+            return out, lse
         a = N.SharedPrefixArgs()
         a.b, a.s_q, a.h_q, a.d_qk, a.d_v, a.kv_format = b, s_q, h_q, d_qk, 512, fmt
         a.num_blocks, a.page_block_size = num_blocks, page_block
-        a.prefix_pages, a.max_pages = prefix_table.numel(), max_pages
+        a.prefix_pages, a.max_pages = prefix_table.numel(), block_table.size(1)
         a.prefix_splits, a.suffix_splits, a.flags, a.sm_scale = prefix_splits, suffix_splits, flags, float(sm_scale)
         sets, nbytes = C.c_int32(0), C.c_int64(0)
-        N.check(N.lib.dsv4_shared_prefix_scratch(C.byref(a), num_sms(dev), C.byref(sets), C.byref(nbytes)),
+        N.check(N.lib.dsv4_shared_prefix_scratch(C.byref(a), num_sms(q.device), C.byref(sets), C.byref(nbytes)),
                 "dsv4_shared_prefix_scratch")
-        rows = b * s_q * h_q
-        o_accum = torch.empty((sets.value, rows, 512), dtype=torch.float32, device=dev)
-        lse_accum = torch.empty((sets.value, rows), dtype=torch.float32, device=dev)
-        workspace = torch.empty((nbytes.value,), dtype=torch.uint8, device=dev)
+        # one allocation: partial outputs, their log-sum-exps, workspace
+        rows = sets.value * b * s_q * h_q
+        lse_at, work_at = rows * 2048, rows * 2048 + (rows * 4 + 255) // 256 * 256
+        scratch = q.new_empty((work_at + nbytes.value,), dtype=torch.uint8)
+        at = scratch.data_ptr()
+        a.o_accum, a.lse_accum, a.workspace = at, at + lse_at, at + work_at
         a.q, a.kv, a.attn_sink = q.data_ptr(), kv.data_ptr(), _ptr(attn_sink)
         a.prefix_table, a.prefix_length = prefix_table.data_ptr(), prefix_length.data_ptr()
         a.block_table, a.suffix_length = block_table.data_ptr(), suffix_length.data_ptr()
         a.out, a.lse = out.data_ptr(), lse.data_ptr()
-        a.o_accum, a.lse_accum, a.workspace = o_accum.data_ptr(), lse_accum.data_ptr(), workspace.data_ptr()
-        a.stride_kv_block, a.stride_table = kv.stride(0), block_table.stride(0)
-        a.stride_o_b, a.stride_o_s, a.stride_o_h = out.stride(0), out.stride(1), out.stride(2)
-        a.stride_lse_b, a.stride_lse_h, a.stride_lse_s = lse.stride(0), lse.stride(1), lse.stride(2)
-        if b > 0:
-            N.check(N.lib.dsv4_shared_prefix_decode(C.byref(a), torch.cuda.current_stream(dev).cuda_stream),
-                    "dsv4_shared_prefix_decode")
+        a.stride_kv_block, a.stride_table = kv_strides[0], block_table.stride(0)
+        a.stride_o_b, a.stride_o_s, a.stride_o_h = s_q * h_q * 512, h_q * 512, 512
+        a.stride_lse_b, a.stride_lse_h, a.stride_lse_s = h_q * s_q, s_q, 1
+        N.check(N.lib.dsv4_shared_prefix_decode(C.byref(a), _stream(idx)), "dsv4_shared_prefix_decode")
     return out, lse
 
 
@@ -324,52 +351,59 @@ def dense_prefill_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, sm_scale, causal: boo
     stay as they were in `out` when it is given, and hold anything otherwise.  Token and
     head strides are free (positive multiples of 8 elements).  `n_splits` is a test hook.
     No counterpart in the reference, whose prefill is sparse only."""
-    _require(q.is_cuda and k.device == q.device and v.device == q.device, "q, k and v must be CUDA tensors of one device")
-    _require(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "q, k and v must be 3-D [tokens, heads, d]")
-    _require(q.dtype in (torch.bfloat16, torch.float16) and k.dtype == q.dtype and v.dtype == q.dtype,
-             "q, k and v must be bf16 or fp16, all of one type")
+    idx = q.get_device()
+    if not (q.is_cuda and k.get_device() == idx and v.get_device() == idx):
+        raise RuntimeError("q, k and v must be CUDA tensors of one device")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise RuntimeError("q, k and v must be 3-D [tokens, heads, d]")
+    dtype = q.dtype
+    if dtype not in _DENSE_DTYPES or k.dtype != dtype or v.dtype != dtype:
+        raise RuntimeError("q, k and v must be bf16 or fp16, all of one type")
     t_q, h_q, d_qk = q.shape
     t_k, h_kv, d_v = v.shape
-    _require((d_qk, d_v) in ((64, 64), (128, 128), (192, 128)),
-             f"(d_qk, d_v) must be (64, 64), (128, 128) or (192, 128); got ({d_qk}, {d_v})")
-    _require(k.shape == (t_k, h_kv, d_qk), "k must be [t_k, h_kv, d_qk], with v's tokens and heads")
-    _require(h_kv >= 1 and h_q >= 1 and h_q % h_kv == 0, f"h_q ({h_q}) must be a multiple of h_kv ({h_kv})")
-    _require(q.stride(2) == 1 and k.stride(2) == 1 and v.stride(2) == 1, "q, k and v must be dense in the last dim")
-    dev = q.device
-    _int32_on("cu_seqlens_q", cu_seqlens_q, dev, 1)
-    _int32_on("cu_seqlens_k", cu_seqlens_k, dev, 1)
+    if (d_qk, d_v) not in ((64, 64), (128, 128), (192, 128)):
+        raise RuntimeError(f"(d_qk, d_v) must be (64, 64), (128, 128) or (192, 128); got ({d_qk}, {d_v})")
+    if k.shape != (t_k, h_kv, d_qk):
+        raise RuntimeError("k must be [t_k, h_kv, d_qk], with v's tokens and heads")
+    if h_kv < 1 or h_q < 1 or h_q % h_kv:
+        raise RuntimeError(f"h_q ({h_q}) must be a multiple of h_kv ({h_kv})")
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    if sq[2] != 1 or sk[2] != 1 or sv[2] != 1:
+        raise RuntimeError("q, k and v must be dense in the last dim")
+    _int32("cu_seqlens_q", cu_seqlens_q, idx, 1)
+    _int32("cu_seqlens_k", cu_seqlens_k, idx, 1)
     b = cu_seqlens_q.numel() - 1
-    _require(b >= 0 and cu_seqlens_k.numel() == b + 1 and cu_seqlens_q.is_contiguous()
-             and cu_seqlens_k.is_contiguous(), "cu_seqlens_q and cu_seqlens_k must be contiguous [b + 1]")
-    if attn_sink is not None:
-        _require(attn_sink.dtype == torch.float32 and attn_sink.numel() == h_q and attn_sink.is_contiguous()
-                 and attn_sink.device == dev, f"attn_sink must be contiguous float32 [{h_q}] on {dev}")
-    if out is not None:
-        _require(out.dtype == q.dtype and out.shape == (t_q, h_q, d_v) and out.device == dev and out.stride(2) == 1,
-                 "out must be [t_q, h_q, d_v] of q's type, dense in the last dim")
-    with torch.cuda.device(dev):
+    if b < 0 or cu_seqlens_k.numel() != b + 1:
+        raise RuntimeError("cu_seqlens_q and cu_seqlens_k must both have b + 1 entries")
+    if attn_sink is not None and not (attn_sink.dtype == torch.float32 and attn_sink.numel() == h_q
+                                      and attn_sink.is_contiguous() and attn_sink.get_device() == idx):
+        raise RuntimeError(f"attn_sink must be contiguous float32 [{h_q}]")
+    if out is not None and not (out.dtype == dtype and out.shape == (t_q, h_q, d_v) and out.get_device() == idx
+                                and out.stride(2) == 1):
+        raise RuntimeError("out must be [t_q, h_q, d_v] of q's type, dense in the last dim")
+    with _current(idx):
         if out is None:
-            out = torch.empty((t_q, h_q, d_v), dtype=q.dtype, device=dev)
-        max_logits = torch.empty((t_q, h_q), dtype=torch.float32, device=dev)
-        lse = torch.empty((t_q, h_q), dtype=torch.float32, device=dev)
-        if n_splits is None:
-            n_splits = N.lib.dsv4_plan_dense_splits(t_q, t_k, b, h_q, h_kv, num_sms(dev))
+            out = q.new_empty((t_q, h_q, d_v))
+        stats = q.new_empty((2, t_q, h_q), dtype=torch.float32)
         a = N.DensePrefillArgs()
+        if n_splits is None:
+            n_splits = N.lib.dsv4_plan_dense_splits(t_q, t_k, b, h_q, h_kv, num_sms(q.device))
         a.b, a.t_q, a.t_k, a.h_q, a.h_kv, a.d_qk, a.d_v = b, t_q, t_k, h_q, h_kv, d_qk, d_v
-        a.dtype = N.DTYPE_BF16 if q.dtype == torch.bfloat16 else N.DTYPE_FP16
-        a.causal, a.n_splits, a.sm_scale = int(bool(causal)), n_splits, float(sm_scale)
+        a.dtype, a.causal, a.n_splits, a.sm_scale = _DENSE_DTYPES[dtype], int(bool(causal)), n_splits, float(sm_scale)
         a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
         a.cu_seqlens_q, a.cu_seqlens_k = cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr()
-        a.attn_sink, a.max_logits, a.lse = _ptr(attn_sink), max_logits.data_ptr(), lse.data_ptr()
+        at = stats.data_ptr()
+        a.attn_sink, a.max_logits, a.lse = _ptr(attn_sink), at, at + 4 * t_q * h_q
         if n_splits > 1:
-            o_accum = torch.empty((n_splits, t_q, h_q, d_v), dtype=torch.float32, device=dev)
-            stat_accum = torch.empty((n_splits, t_q, h_q, 2), dtype=torch.float32, device=dev)
-            a.o_accum, a.stat_accum = o_accum.data_ptr(), stat_accum.data_ptr()
-        (a.stride_q_t, a.stride_q_h, _), (a.stride_k_t, a.stride_k_h, _) = q.stride(), k.stride()
-        (a.stride_v_t, a.stride_v_h, _), (a.stride_o_t, a.stride_o_h, _) = v.stride(), out.stride()
+            rows = n_splits * t_q * h_q
+            scratch = q.new_empty((rows * (d_v + 2),), dtype=torch.float32)
+            a.o_accum, a.stat_accum = scratch.data_ptr(), scratch.data_ptr() + rows * d_v * 4
+        a.stride_q_t, a.stride_q_h, a.stride_k_t, a.stride_k_h = sq[0], sq[1], sk[0], sk[1]
+        a.stride_v_t, a.stride_v_h = sv[0], sv[1]
+        a.stride_o_t, a.stride_o_h, _ = out.stride()
         a.stride_ml_t = a.stride_lse_t = h_q
-        N.check(N.lib.dsv4_dense_prefill(C.byref(a), torch.cuda.current_stream(dev).cuda_stream),
-                "dsv4_dense_prefill")
+        N.check(N.lib.dsv4_dense_prefill(C.byref(a), _stream(idx)), "dsv4_dense_prefill")
+    max_logits, lse = stats.unbind(0)
     return out, max_logits, lse
 
 
@@ -422,11 +456,6 @@ def kv_store_rows(k, loc, kv) -> None:
                 "dsv4_kv_store_rows")
 
 
-def _int32_on(name, t, device, dim) -> None:
-    _require(t.dtype == torch.int32 and t.dim() == dim and t.device == device,
-             f"{name} must be {dim}-D int32 on {device}")
-
-
 def build_slot_maps(block_table, cached_lens, new_lens, free_pages, page_block: int, n_slots: int):
     """Block tables and slot maps of one serving step, from request lengths on the device.
 
@@ -442,33 +471,34 @@ def build_slot_maps(block_table, cached_lens, new_lens, free_pages, page_block: 
     arrays `dense_prefill_fwd` takes).  n_taken > n_free says that the free list was too
     short.  No host synchronisation; see dsv4_build_slot_maps in the C header.  No
     counterpart in the reference, whose serving framework builds these on the host."""
-    _require(block_table.is_cuda, "block_table must be a CUDA tensor")
-    dev = block_table.device
-    _int32_on("block_table", block_table, dev, 2)
+    if not block_table.is_cuda:
+        raise RuntimeError("block_table must be a CUDA tensor")
+    idx = block_table.get_device()
+    _int32("block_table", block_table, idx, 2, dense_rows=True)
     b, max_pages = block_table.shape
-    for name, t in (("cached_lens", cached_lens), ("new_lens", new_lens)):
-        _int32_on(name, t, dev, 1)
-        _require(t.numel() == b and t.is_contiguous(), f"{name} must be contiguous [{b}]")
-    _int32_on("free_pages", free_pages, dev, 1)
-    _require(free_pages.is_contiguous(), "free_pages must be contiguous")
-    _require(max_pages <= 1 or block_table.stride(1) == 1, "block_table rows must be dense")
+    _int32("cached_lens", cached_lens, idx, 1)
+    _int32("new_lens", new_lens, idx, 1)
+    _int32("free_pages", free_pages, idx, 1)
+    if cached_lens.numel() != b or new_lens.numel() != b:
+        raise RuntimeError(f"cached_lens and new_lens must have {b} entries")
     page_block, n_slots = int(page_block), int(n_slots)
-    _require(1 <= page_block < 2 ** 31 and 0 <= n_slots < 2 ** 31, "page_block >= 1 and n_slots >= 0 expected")
-    _require(b <= 16384, "at most 16384 requests")
-    with torch.cuda.device(dev):
-        slots = torch.empty((n_slots,), dtype=torch.int64, device=dev)
-        ints = torch.empty((n_slots + 2 * (b + 1) + 1,), dtype=torch.int32, device=dev)
-        positions, cu_new, cu_total, n_taken = ints.split([n_slots, b + 1, b + 1, 1])
+    if not (1 <= page_block < 2 ** 31 and 0 <= n_slots < 2 ** 31):
+        raise RuntimeError("page_block >= 1 and n_slots >= 0 expected")
+    if b > 16384:
+        raise RuntimeError("at most 16384 requests")
+    with _current(idx):
+        slots = cached_lens.new_empty((n_slots,), dtype=torch.int64)
+        ints = cached_lens.new_empty((n_slots + 2 * b + 3,))
         a = N.SlotMapArgs()
         a.b, a.max_pages, a.page_block_size, a.n_slots = b, max_pages, page_block, n_slots
         a.n_free = free_pages.numel()
         a.block_table, a.stride_table = block_table.data_ptr(), block_table.stride(0) if b > 1 else max_pages
         a.cached_lens, a.new_lens, a.free_pages = cached_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr()
-        a.slots, a.positions = slots.data_ptr(), positions.data_ptr()
-        a.cu_new, a.cu_total, a.n_taken = cu_new.data_ptr(), cu_total.data_ptr(), n_taken.data_ptr()
-        N.check(N.lib.dsv4_build_slot_maps(C.byref(a), torch.cuda.current_stream(dev).cuda_stream),
-                "dsv4_build_slot_maps")
-    return slots, positions, cu_new, cu_total, n_taken
+        a.slots, at = slots.data_ptr(), ints.data_ptr()
+        a.positions, a.cu_new, a.cu_total = at, at + 4 * n_slots, at + 4 * (n_slots + b + 1)
+        a.n_taken = at + 4 * (n_slots + 2 * b + 2)
+        N.check(N.lib.dsv4_build_slot_maps(C.byref(a), _stream(idx)), "dsv4_build_slot_maps")
+    return (slots,) + torch.split_with_sizes(ints, (n_slots, b + 1, b + 1, 1))
 
 
 def page_indices(block_table, positions, page_block: int, cu_seqlens=None) -> torch.Tensor:
@@ -481,34 +511,40 @@ def page_indices(block_table, positions, page_block: int, cu_seqlens=None) -> to
 
     A negative position, one past the table, one on a page with a negative id, and a row of
     no request give -1."""
-    _require(block_table.is_cuda, "block_table must be a CUDA tensor")
-    dev = block_table.device
-    _int32_on("block_table", block_table, dev, 2)
+    if not block_table.is_cuda:
+        raise RuntimeError("block_table must be a CUDA tensor")
+    idx = block_table.get_device()
+    _int32("block_table", block_table, idx, 2, dense_rows=True)
     b, max_pages = block_table.shape
-    _int32_on("positions", positions, dev, 3 if cu_seqlens is None else 2)
+    _int32("positions", positions, idx, 3 if cu_seqlens is None else 2, dense_rows=True)
+    page_block = int(page_block)
+    if not 1 <= page_block < 2 ** 31:
+        raise RuntimeError("page_block >= 1 expected")
     topk = positions.size(-1)
-    _require(topk <= 1 or positions.stride(-1) == 1, "positions must be dense in the last dim")
-    _require(max_pages <= 1 or block_table.stride(1) == 1, "block_table rows must be dense")
-    _require(1 <= int(page_block) < 2 ** 31, "page_block >= 1 expected")
+    flat, s_q, n_rows = positions, 1, positions.size(0)
     if cu_seqlens is None:
-        _require(positions.size(0) == b, f"positions must be [{b}, s_q, topk]")
-        s_q, n_rows = positions.size(1), b * positions.size(1)
-        flat = positions.reshape(n_rows, topk)           # a view for every dense arrangement
+        if n_rows != b:
+            raise RuntimeError(f"positions must be [{b}, s_q, topk]")
+        s_q = positions.size(1)
+        n_rows = b * s_q
+        if not positions.is_contiguous():
+            flat = positions.reshape(n_rows, topk)       # a view when the rows have one stride
     else:
-        _int32_on("cu_seqlens", cu_seqlens, dev, 1)
-        _require(cu_seqlens.numel() == b + 1 and cu_seqlens.is_contiguous(), f"cu_seqlens must be contiguous [{b + 1}]")
-        s_q, n_rows, flat = 1, positions.size(0), positions
-    with torch.cuda.device(dev):
-        out = torch.empty(positions.shape, dtype=torch.int32, device=dev)
+        _int32("cu_seqlens", cu_seqlens, idx, 1)
+        if cu_seqlens.numel() != b + 1:
+            raise RuntimeError(f"cu_seqlens must have {b + 1} entries")
+    with _current(idx):
+        out = positions.new_empty(positions.shape)
         a = N.PageIndicesArgs()
         a.n_rows, a.topk, a.b, a.s_q = n_rows, topk, b, max(s_q, 1)
-        a.max_pages, a.page_block_size = max_pages, int(page_block)
+        a.max_pages, a.page_block_size = max_pages, page_block
         a.block_table, a.positions, a.indices = block_table.data_ptr(), flat.data_ptr(), out.data_ptr()
         a.cu_seqlens = _ptr(cu_seqlens)
         a.stride_table = block_table.stride(0)
-        a.stride_positions = flat.stride(0) if n_rows > 1 else topk
-        N.check(N.lib.dsv4_page_indices(C.byref(a), torch.cuda.current_stream(dev).cuda_stream),
-                "dsv4_page_indices")
+        a.stride_positions = topk if n_rows <= 1 else flat.stride(-2)
+        if s_q > 1 and flat is not positions:
+            a.stride_positions = flat.stride(0)
+        N.check(N.lib.dsv4_page_indices(C.byref(a), _stream(idx)), "dsv4_page_indices")
     return out
 
 
