@@ -28,7 +28,10 @@
 // finite are cleared and handed by the epilogue to the rows that do see them.
 //
 // Few rows (single tokens over long contexts): the keys are cut into n_splits ranges, each
-// CTA leaves a normalised 32-bit partial, and dense_combine_kernel joins them.
+// CTA leaves normalised 32-bit partials, and dense_combine_kernel joins them.  A CTA whose
+// second row tile would be empty then gives the first one's odd key tiles to the second
+// pipeline ("twin"), which halves its chain of products and softmaxes; a range therefore has
+// two partial sets.
 #include <cuda_fp16.h>
 
 #include <mutex>
@@ -114,7 +117,7 @@ struct DenseParams {
   int64_t stride_v_t, stride_v_h, stride_o_t, stride_o_h, stride_ml_t, stride_lse_t;
   void* out;
   float *max_logits, *lse;
-  float *o_accum, *stat_accum;   // [split][t][h][d_v], [split][t][h][2] (max logit, log-sum-exp)
+  float *o_accum, *stat_accum;   // [2 splits][t][h][d_v], [2 splits][t][h][2] (max logit, log-sum-exp)
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -203,7 +206,9 @@ __device__ __forceinline__ uint32_t abs_max2(uint32_t a, uint32_t b) {
 struct Work {
   int q0, len_q, k0, len_k;      // rows of the packed tensors
   int t0;                        // first query token of row tile 0, in the sequence
-  int first, count[2];           // key tiles: [first, first + count[s])
+  int first, tiles;              // key tiles [first, first + tiles)
+  int count[2];                  // of them row tile s takes the first count[s] ...
+  bool twin;                     // ... or, both row tiles being the same, every second one from s on
   int look;                      // key tiles from this one on are seen only in part by some row
   bool any;
 };
@@ -217,19 +222,28 @@ __device__ __forceinline__ int reach_of(const DenseParams& p, const Work& w, int
 
 __device__ __forceinline__ int clamp_to(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
+template <bool RANGES>
 __device__ __forceinline__ Work find_work(const DenseParams& p, int slot, int split) {
   Work w;
   // Sequence s owns the slots from cu_q[s] / span + s on: at least ceil(len / span) of them.
-  const int span = 2 * p.tok_tile;
-  int lo = 0, hi = p.b;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (clamp_to(__ldg(p.cu_q + mid), 0, p.t_q) / span + mid <= slot) lo = mid; else hi = mid;
+  // Every warp looks for it 32 candidates at a time: the loads of a step do not wait for one
+  // another (bisection took one memory latency a halving, up to 2 us of a short CTA's 8).
+  const int span = 2 * p.tok_tile, lane = threadIdx.x & 31;
+  int lo = 0, n = p.b;                     // the sequence is one of [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const int at = lo + lane * step;
+    const bool below = lane * step < n && clamp_to(__ldg(p.cu_q + at), 0, p.t_q) / span + at <= slot;
+    const uint32_t hits = __ballot_sync(0xffffffffu, below) | 1u;
+    const int last = 31 - __clz(hits);     // (bounds that do not ascend land somewhere, in range)
+    n = min(step, n - last * step);
+    lo += last * step;
   }
-  w.q0 = clamp_to(__ldg(p.cu_q + lo), 0, p.t_q);
-  w.len_q = clamp_to(__ldg(p.cu_q + lo + 1), w.q0, p.t_q) - w.q0;
-  w.k0 = clamp_to(__ldg(p.cu_k + lo), 0, p.t_k);
-  w.len_k = clamp_to(__ldg(p.cu_k + lo + 1), w.k0, p.t_k) - w.k0;
+  const int q0 = __ldg(p.cu_q + lo), q1 = __ldg(p.cu_q + lo + 1), k0 = __ldg(p.cu_k + lo), k1 = __ldg(p.cu_k + lo + 1);
+  w.q0 = clamp_to(q0, 0, p.t_q);
+  w.len_q = clamp_to(q1, w.q0, p.t_q) - w.q0;
+  w.k0 = clamp_to(k0, 0, p.t_k);
+  w.len_k = clamp_to(k1, w.k0, p.t_k) - w.k0;
   const int64_t t0 = static_cast<int64_t>(slot - (w.q0 / span + lo)) * span;
   w.any = t0 >= 0 && t0 < w.len_q;
   w.t0 = static_cast<int>(w.any ? t0 : 0);
@@ -243,18 +257,27 @@ __device__ __forceinline__ Work find_work(const DenseParams& p, int slot, int sp
     }
   }
   const int total = max(tiles[0], tiles[1]);
-  const int per = (total + p.n_splits - 1) / p.n_splits;
-  w.first = min(split * per, total);
-  const int end = min(w.first + per, total);
+  int end = total;
+  w.first = 0;
+  if (RANGES) {
+    const int per = (total + p.n_splits - 1) / p.n_splits;
+    w.first = min(split * per, total);
+    end = min(w.first + per, total);
+  }
+  w.tiles = end - w.first;
 #pragma unroll
   for (int s = 0; s < 2; ++s) w.count[s] = max(min(tiles[s], end) - w.first, 0);
+  w.twin = RANGES && w.t0 + p.tok_tile >= w.len_q;
+  if (w.twin) {
+    w.count[0] = (w.tiles + 1) / 2;
+    w.count[1] = w.tiles / 2;
+  }
   w.look = reach_of(p, w, w.t0) / TILE_N;
   return w;
 }
 
 // Where a row's results go, and its final factor.
-template <int DV, bool BF16>
-__device__ __forceinline__ void store_stats(const DenseParams& p, int split, int64_t t, int h, float m_raw, float m_ref,
+__device__ __forceinline__ void store_stats(const DenseParams& p, int set, int64_t t, int h, float m_raw, float m_ref,
                                             float l, bool fail, float& factor) {
   // m_ref: reference in log2 units (-inf: nothing seen); l: sum relative to it
   const bool none = m_ref == -INFINITY && l == l;      // (NaN scores set no reference, but show)
@@ -262,7 +285,7 @@ __device__ __forceinline__ void store_stats(const DenseParams& p, int split, int
   const float ml = none ? -INFINITY : m_raw * p.sm_scale;
   factor = none ? 0.f : 1.f / l;
   if (p.n_splits > 1) {
-    float2* dst = reinterpret_cast<float2*>(p.stat_accum + ((static_cast<int64_t>(split) * p.t_q + t) * p.h_q + h) * 2);
+    float2* dst = reinterpret_cast<float2*>(p.stat_accum + ((static_cast<int64_t>(set) * p.t_q + t) * p.h_q + h) * 2);
     *dst = make_float2(ml, fail ? NAN : lse);
     return;
   }
@@ -271,7 +294,9 @@ __device__ __forceinline__ void store_stats(const DenseParams& p, int split, int
   p.lse[t * p.stride_lse_t + h] = fail ? NAN : none ? INFINITY : lse;
 }
 
-template <int DQK, int DV, bool BF16>
+// RANGES: the keys are cut into n_splits ranges, with twins (an instantiation of its own: the
+// choice inside the loops costs 4 to 6 % of a long prompt).
+template <int DQK, int DV, bool BF16, bool RANGES>
 __global__ void __launch_bounds__(THREADS, 1)
 dense_attn_kernel(const __grid_constant__ DenseParams p) {
   using C = DCfg<DQK, DV>;
@@ -282,16 +307,18 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   DenseCtrl& ctrl = *reinterpret_cast<DenseCtrl*>(smem_raw + (base - raw) + C::Q_BYTES + C::K_BYTES + C::V_BYTES);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == WARP_TMA && lane < 3) tma_prefetch_map(lane == 0 ? &p.mq : lane == 1 ? &p.mk : &p.mv);
   grid_dependency_wait();
   // Slots last to first: in a causal sequence the late rows are the long ones.
   const int chunk = blockIdx.x % p.chunks;
   const int slot = p.slots - 1 - static_cast<int>(blockIdx.x / p.chunks);
   const int split = blockIdx.z;
-  const Work w = find_work(p, slot, split);
+  const Work w = find_work<RANGES>(p, slot, split);
+  const bool twin = RANGES && w.twin;
   if (!w.any) return;
   const int head0 = chunk * p.pack;
   const int kvh = head0 / (p.h_q / p.h_kv);
-  const int n_tiles = max(w.count[0], w.count[1]);
+  const int n_tiles = w.tiles;
 
   if (n_tiles == 0) {                     // nothing in this CTA's range: results of empty rows
     const int rows = 2 * p.tok_tile * p.pack;
@@ -300,11 +327,11 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
       if (tok >= w.len_q) continue;
       const int64_t t = w.q0 + tok;
       float f;
-      store_stats<DV, BF16>(p, split, t, h, -INFINITY, -INFINITY, 0.f, false, f);
-      if (p.n_splits > 1) {
-        float4* d = reinterpret_cast<float4*>(p.o_accum + ((static_cast<int64_t>(split) * p.t_q + t) * p.h_q + h) * DV);
-        for (int c = 0; c < DV / 4; ++c) d[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (RANGES) {                       // (a set without weight: its values are not read)
+        store_stats(p, 2 * split, t, h, -INFINITY, -INFINITY, 0.f, false, f);
+        store_stats(p, 2 * split + 1, t, h, -INFINITY, -INFINITY, 0.f, false, f);
       } else {
+        store_stats(p, 0, t, h, -INFINITY, -INFINITY, 0.f, false, f);
         uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + t * p.stride_o_t + h * p.stride_o_h);
         for (int c = 0; c < DV / 8; ++c) d[c] = make_uint4(0, 0, 0, 0);
       }
@@ -359,7 +386,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
           mbar_expect_tx(bar(&ctrl.q_full[s]), q_bytes * C::QB);
           for (int c = 0; c < C::QB; ++c)
             tma_load_3d(sQ + (s * C::QB + c) * BLOCK_BYTES, &p.mq, 64 * c, head0,
-                        w.q0 + w.t0 + s * p.tok_tile, bar(&ctrl.q_full[s]));
+                        w.q0 + w.t0 + (twin ? 0 : s * p.tok_tile), bar(&ctrl.q_full[s]));
         };
         if (w.count[0] > 0) load_q(0);
         bool ok = true;
@@ -391,7 +418,11 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
       // starts from are broadcast so that they are known to be uniform.
       const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
       const int count0 = __shfl_sync(0xffffffffu, w.count[0], 0), count1 = __shfl_sync(0xffffffffu, w.count[1], 0);
-      const int tiles = max(count0, count1);
+      const int tiles = __shfl_sync(0xffffffffu, w.tiles, 0);
+      const bool twin = RANGES && __shfl_sync(0xffffffffu, w.twin ? 1 : 0, 0) != 0;
+      // does row tile s read key tile i, and as its how manieth?
+      auto takes = [&](int s, int i) { return twin ? (i & 1) == s : i < (s == 0 ? count0 : count1); };
+      auto nth = [&](int i) { return twin ? i >> 1 : i; };
       const uint32_t elected = elect_one();
       bool ok = true;
       auto wait = [&](uint64_t* b, int parity, int code) {
@@ -410,12 +441,13 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
         for (int i = 0; i < tiles && ok; ++i) {
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            if (i >= (s == 0 ? count0 : count1) || !ok) continue;
-            const bool last = s == 1 || i >= count1;     // nobody reads the tile's K after this
-            if (i == 0) wait(&ctrl.q_full[s], 0, ERR_Q);
+            if (!takes(s, i) || !ok) continue;
+            const bool last = twin || s == 1 || i >= count1;     // nobody reads the tile's K after this
+            const int j = nth(i);
+            if (j == 0) wait(&ctrl.q_full[s], 0, ERR_Q);
             // the scores that were here have been read
             if (C::S_BUFS == 1) wait(&ctrl.s_free[0], (turn & 1) ^ 1, ERR_FREE);
-            else wait(&ctrl.s_free[s], (i & 1) ^ 1, ERR_FREE);
+            else wait(&ctrl.s_free[s], (j & 1) ^ 1, ERR_FREE);
             ++turn;
             const uint32_t tS = t0 + C::COL_S + (C::S_BUFS == 1 ? 0 : 128 * s);
             int ks = (i * (C::QB / C::K_STEP)) % C::K_RING, kphase = (i * (C::QB / C::K_STEP) / C::K_RING) & 1;
@@ -451,16 +483,17 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
           }
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            if (i >= (s == 0 ? count0 : count1)) continue;
-            wait(&ctrl.p_full[s], i & 1, ERR_P);
+            if (!takes(s, i)) continue;
+            const int j = nth(i);
+            wait(&ctrl.p_full[s], j & 1, ERR_P);
             if (!ok) break;
             tc_fence_after_sync();
 #pragma unroll
             for (int k = 0; k < TILE_N / 16; ++k)
               umma_ts_elect(t0 + C::COL_O + DV * s, t0 + C::COL_P + 64 * s + 8 * k, d + ((k * 2048) >> 4), idesc,
-                            (i | k) != 0, elected);
+                            (j | k) != 0, elected);
             umma_commit_elect(bar(&ctrl.o_done[s]), elected);
-            if (s == 1 || i >= count1) umma_commit_elect(bar(&ctrl.v_empty[vu]), elected);
+            if (twin || s == 1 || i >= count1) umma_commit_elect(bar(&ctrl.v_empty[vu]), elected);
           }
         }
       }
@@ -534,7 +567,8 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
   const int s = warp >> 2;
   const int row = (warp & 3) * 32 + lane;
-  const int tok = w.t0 + s * p.tok_tile + row / p.pack;
+  const int row_t0 = w.t0 + (twin ? 0 : s * p.tok_tile);
+  const int tok = row_t0 + row / p.pack;
   const int h = head0 + row % p.pack;
   const bool live = row < p.pack * p.tok_tile && tok < w.len_q;
   const int reach = live ? reach_of(p, w, tok) : 0;
@@ -543,8 +577,9 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   const uint32_t tS = tmem + lanes + C::COL_S + (C::S_BUFS == 1 ? 0 : 128 * s), tP = tmem + lanes + C::COL_P + 64 * s;
   const uint32_t tO = tmem + lanes + C::COL_O + DV * s;
   const float c = p.sm_scale * LOG2E;
+  const bool idle = RANGES && !__any_sync(0xffffffffu, live);   // no row of this warp exists: its scores are not looked at
   // tiles below this one are seen whole by every row of this tile that exists
-  const int whole = reach_of(p, w, w.t0 + s * p.tok_tile) / TILE_N;
+  const int whole = reach_of(p, w, row_t0) / TILE_N;
 
   float m_ref = -INFINITY, m_raw = -INFINITY, l = 0.f;
   bool ok = true;
@@ -552,6 +587,15 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   for (int i = 0; i < n_mine; ++i) {
     if (!mbar_wait_fast(bar(&ctrl.s_full[s]), i & 1)) { gave_up(ERR_S); ok = false; break; }
     tc_fence_after_sync();
+    if (idle) {
+      if (lane == 0) mbar_arrive(bar(&ctrl.s_free[C::S_BUFS == 1 ? 0 : s]));
+      // the same order as below: P of this tile is reported once P of the one before has been read,
+      // or two reports of one warp could fall into one phase
+      if (i > 0 && !mbar_wait_fast(bar(&ctrl.o_done[s]), (i - 1) & 1)) { gave_up(ERR_O); ok = false; break; }
+      if (lane == 0) mbar_arrive(bar(&ctrl.p_full[s]));
+      __syncwarp();
+      continue;
+    }
     uint32_t x[TILE_N];
 #pragma unroll
     for (int k = 0; k < 4; ++k) tmem_ld32(tS + 32 * k, x + 32 * k);
@@ -560,8 +604,9 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     tc_fence_before_sync();
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(&ctrl.s_free[C::S_BUFS == 1 ? 0 : s]));
-    if (w.first + i >= whole) {
-      const int see = reach - (w.first + i) * TILE_N;
+    const int tile = w.first + (twin ? 2 * i + s : i);
+    if (tile >= whole) {
+      const int see = reach - tile * TILE_N;
 #pragma unroll
       for (int k = 0; k < TILE_N; ++k) x[k] = k < see ? x[k] : 0xff800000u;
     }
@@ -622,7 +667,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
         tmem_st32(tP + 32 * q, pk);
       }
     };
-    if (w.first + i >= whole) weights(std::true_type{});
+    if (tile >= whole) weights(std::true_type{});
     else weights(std::false_type{});
     float s0, s1, s2, s3;
     unpair(sum[0], s0, s1);
@@ -641,10 +686,15 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   const bool fail = !ok || *reinterpret_cast<volatile int*>(&ctrl.fail) != 0;
   const int64_t t = static_cast<int64_t>(w.q0) + tok;
   float factor = 0.f;
-  if (live) store_stats<DV, BF16>(p, split, t, h, m_raw, m_ref, l, fail, factor);
+  const int set = RANGES ? 2 * split + (twin ? s : 0) : 0;
+  if (live) {
+    store_stats(p, set, t, h, m_raw, m_ref, l, fail, factor);
+    float none;
+    if (RANGES && !twin) store_stats(p, set + 1, t, h, -INFINITY, -INFINITY, 0.f, false, none);
+  }
   const bool nothing = m_ref == -INFINITY && l == l;
   const bool bad = *reinterpret_cast<volatile int*>(&ctrl.bad) != 0;
-  const int64_t acc = ((static_cast<int64_t>(split) * p.t_q + t) * p.h_q + h) * DV;
+  const int64_t acc = ((static_cast<int64_t>(set) * p.t_q + t) * p.h_q + h) * DV;
 #pragma unroll 1
   for (int k = 0; k < DV / 32; ++k) {
     uint32_t o[32];
@@ -658,8 +708,9 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     if (bad && live) {
       // the values that were cleared, for the rows that see them: their weight is positive,
       // so an infinity stays one (and two of both signs, or a NaN, make a NaN)
-      const int from = max(w.look, w.first) * TILE_N, to = min(reach, (w.first + n_mine) * TILE_N);
+      const int from = max(w.look, w.first) * TILE_N, to = min(reach, (w.first + (twin ? w.tiles : n_mine)) * TILE_N);
       for (int j = from; j < to; ++j) {
+        if (twin && (((j / TILE_N - w.first) & 1) != s)) continue;
         const uint16_t* vr = static_cast<const uint16_t*>(p.v) + (w.k0 + j) * p.stride_v_t + kvh * p.stride_v_h + 32 * k;
 #pragma unroll
         for (int q = 0; q < 32; ++q) {
@@ -672,7 +723,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
       }
     }
     if (!live || fail) continue;
-    if (p.n_splits > 1) {
+    if (RANGES) {
       float4* d = reinterpret_cast<float4*>(p.o_accum + acc + 32 * k);
 #pragma unroll
       for (int q = 0; q < 8; ++q) d[q] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
@@ -701,7 +752,7 @@ dense_combine_kernel(const __grid_constant__ DenseParams p) {
   const int h = static_cast<int>(item - t * p.h_q);
   if (t < __ldg(p.cu_q) || t >= __ldg(p.cu_q + p.b)) return;   // a row of no sequence stays as it is
   float ml = -INFINITY, top = -INFINITY;
-  for (int s = 0; s < p.n_splits; ++s) {
+  for (int s = 0; s < 2 * p.n_splits; ++s) {
     const float2 v = *reinterpret_cast<const float2*>(p.stat_accum + ((static_cast<int64_t>(s) * p.t_q + t) * p.h_q + h) * 2);
     ml = fmaxf(ml, v.x);
     top = (v.y != v.y || top != top) ? NAN : fmaxf(top, v.y);  // a failed part shows
@@ -710,7 +761,7 @@ dense_combine_kernel(const __grid_constant__ DenseParams p) {
 #pragma unroll
   for (int k = 0; k < PER; ++k) acc[k] = 0.f;
   if (top != -INFINITY) {
-    for (int s = 0; s < p.n_splits; ++s) {
+    for (int s = 0; s < 2 * p.n_splits; ++s) {
       const int64_t at = (static_cast<int64_t>(s) * p.t_q + t) * p.h_q + h;
       const float e = p.stat_accum[at * 2 + 1];
       if (e == -INFINITY) continue;
@@ -736,7 +787,7 @@ dense_combine_kernel(const __grid_constant__ DenseParams p) {
 constexpr int MAX_DEVICES = 64;
 std::mutex g_dense_mu;
 
-template <int DQK, int DV, bool BF16>
+template <int DQK, int DV, bool BF16, bool RANGES>
 cudaError_t launch_one(const DenseParams& p, cudaStream_t st) {
   constexpr size_t smem = dense_smem_bytes<DQK, DV>();
   static bool configured[MAX_DEVICES] = {};
@@ -747,7 +798,7 @@ cudaError_t launch_one(const DenseParams& p, cudaStream_t st) {
   {
     std::lock_guard<std::mutex> lk(g_dense_mu);
     if (!configured[dev]) {
-      e = cudaFuncSetAttribute(dense_attn_kernel<DQK, DV, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      e = cudaFuncSetAttribute(dense_attn_kernel<DQK, DV, BF16, RANGES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                static_cast<int>(smem));
       if (e) return e;
       configured[dev] = true;
@@ -761,12 +812,18 @@ cudaError_t launch_one(const DenseParams& p, cudaStream_t st) {
   cudaLaunchAttribute attr[1];
   cfg.attrs = attr;
   cfg.numAttrs = add_overlap_attribute(attr);
-  if ((e = cudaLaunchKernelEx(&cfg, dense_attn_kernel<DQK, DV, BF16>, p))) return e;
-  if (p.n_splits == 1) return cudaSuccess;
+  if ((e = cudaLaunchKernelEx(&cfg, dense_attn_kernel<DQK, DV, BF16, RANGES>, p))) return e;
+  if (!RANGES) return cudaSuccess;
   cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.t_q) * p.h_q + 7) / 8));
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, dense_combine_kernel<DV, BF16>, p);
+}
+
+template <int DQK, int DV>
+cudaError_t launch_dims(const DenseParams& p, bool bf16, cudaStream_t st) {
+  if (p.n_splits > 1) return bf16 ? launch_one<DQK, DV, true, true>(p, st) : launch_one<DQK, DV, false, true>(p, st);
+  return bf16 ? launch_one<DQK, DV, true, false>(p, st) : launch_one<DQK, DV, false, false>(p, st);
 }
 
 // Heads packed into a row tile: the most heads of a group that divide it and fit.
@@ -807,9 +864,9 @@ cudaError_t launch_dense_prefill(const Dsv4DensePrefillArgs& a, cudaStream_t st)
                     a.stride_k_t, a.stride_k_h, TILE_N, 1))) return e;
   if ((e = make_map_16bit(&p.mv, bf16, keys ? a.v : a.q, keys ? a.t_k : 1, keys ? a.h_kv : 1, a.d_v,
                     a.stride_v_t, a.stride_v_h, TILE_N, 1))) return e;
-  if (a.d_qk == 192) return bf16 ? launch_one<192, 128, true>(p, st) : launch_one<192, 128, false>(p, st);
-  if (a.d_qk == 128) return bf16 ? launch_one<128, 128, true>(p, st) : launch_one<128, 128, false>(p, st);
-  return bf16 ? launch_one<64, 64, true>(p, st) : launch_one<64, 64, false>(p, st);
+  if (a.d_qk == 192) return launch_dims<192, 128>(p, bf16, st);
+  if (a.d_qk == 128) return launch_dims<128, 128>(p, bf16, st);
+  return launch_dims<64, 64>(p, bf16, st);
 }
 
 cudaError_t read_dense_error(int* value, bool reset) {

@@ -120,6 +120,9 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, int x
       "[%0], [%1, {%2, %3, %4}], [%5];"
       ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
+__device__ __forceinline__ void tma_prefetch_map(const void* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 
 // ---- fences ---------------------------------------------------------------
 // Generic-proxy shared-memory writes -> visible to the async proxy (tcgen05.mma).

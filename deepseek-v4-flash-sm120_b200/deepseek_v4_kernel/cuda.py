@@ -395,7 +395,7 @@ def dense_prefill_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, sm_scale, causal: boo
         at = stats.data_ptr()
         a.attn_sink, a.max_logits, a.lse = _ptr(attn_sink), at, at + 4 * t_q * h_q
         if n_splits > 1:
-            rows = n_splits * t_q * h_q
+            rows = 2 * n_splits * t_q * h_q          # two partial sets a range
             scratch = q.new_empty((rows * (d_v + 2),), dtype=torch.float32)
             a.o_accum, a.stat_accum = scratch.data_ptr(), scratch.data_ptr() + rows * d_v * 4
         a.stride_q_t, a.stride_q_h, a.stride_k_t, a.stride_k_h = sq[0], sq[1], sk[0], sk[1]

@@ -333,7 +333,7 @@ int dsv4_shared_prefix_scratch(const Dsv4SharedPrefixArgs* args, int num_sms, in
  * in elements, multiples of 8, positive (k and v of several tokens or heads cannot be
  * broadcast views); pointers are 16-byte aligned; the last dimension is dense.  sm_scale is
  * positive and finite.  n_splits > 1 cuts every sequence's keys into that many ranges and
- * needs o_accum [n_splits, t_q, h_q, d_v] and stat_accum [n_splits, t_q, h_q, 2].           */
+ * needs o_accum [2 n_splits, t_q, h_q, d_v] and stat_accum [2 n_splits, t_q, h_q, 2].       */
 enum Dsv4Dtype { DSV4_DTYPE_BF16 = 0, DSV4_DTYPE_FP16 = 1 };
 typedef struct Dsv4DensePrefillArgs {
   int32_t b, t_q, t_k, h_q, h_kv, d_qk, d_v;
