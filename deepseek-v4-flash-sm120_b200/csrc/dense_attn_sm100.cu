@@ -35,7 +35,6 @@
 #include <cuda_fp16.h>
 
 #include <mutex>
-#include <type_traits>
 
 #include "attn_params.cuh"
 #include "launchers.h"
@@ -63,10 +62,6 @@ static_assert(THREADS * (LAUNCH_REGS + 8) > 65536, "LAUNCH_REGS is what the laun
 constexpr int WARP_QK = 8, WARP_PV = 9, WARP_TMA = 10, WARP_LOOK = 11;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float RESCALE_THRESHOLD = 8.0f;            // log2 units
-#ifndef EMU
-#define EMU 0
-#endif
-constexpr int EMULATED = EMU;
 constexpr uint32_t TMEM_COLS = 512;
 
 enum DenseErr { ERR_Q = 11, ERR_K = 12, ERR_V = 13, ERR_P = 14, ERR_S = 15, ERR_O = 16, ERR_SLOT = 17, ERR_LOOK = 18,
@@ -150,32 +145,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^y for two values of at most RESCALE_THRESHOLD without the special-function unit, which is
-// what the softmax is bound by: 2^y = 2^n 2^f with n the nearest integer (left in the low bits
-// by adding 1.5 * 2^23) and |f| <= 1/2, 2^f by the polynomial of degree 5 of least relative
-// error there (fitted by Lawson's reweighting: 7.5e-8 off, 2.1e-7 as evaluated in 32 bits, about
-// the special-function unit's own error).
-// Below 2^-126 the result stays 2^-126.
-__device__ __forceinline__ void ex2_pair(uint64_t y, float& a, float& b) {
-  constexpr float BIG = 12582912.0f;
-  constexpr float C0 = 1.00000012f, C1 = 0.693146944f, C2 = 0.240221202f, C3 = 0.0555071309f, C4 = 0.00967554096f,
-                  C5 = 0.00132764725f;
-  unpair(y, a, b);
-  y = pair(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
-  const uint64_t t = add_pair(y, pair(BIG, BIG));
-  const uint64_t f = fma_pair(add_pair(t, pair(-BIG, -BIG)), pair(-1.f, -1.f), y);
-  uint64_t r = pair(C5, C5);
-  r = fma_pair(r, f, pair(C4, C4));
-  r = fma_pair(r, f, pair(C3, C3));
-  r = fma_pair(r, f, pair(C2, C2));
-  r = fma_pair(r, f, pair(C1, C1));
-  r = fma_pair(r, f, pair(C0, C0));
-  float n0, n1;
-  unpair(t, n0, n1);
-  unpair(r, a, b);
-  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(n0) << 23));
-  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(n1) << 23));
-}
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (BF16) {
@@ -230,6 +199,17 @@ __device__ __forceinline__ Work find_work(const DenseParams& p, int slot, int sp
   // another (bisection took one memory latency a halving, up to 2 us of a short CTA's 8).
   const int span = 2 * p.tok_tile, lane = threadIdx.x & 31;
   int lo = 0, n = p.b;                     // the sequence is one of [lo, lo + n)
+  int q0, q1, k0, k1;
+  if (n < 32) {                            // all bounds at once
+    const int cq = __ldg(p.cu_q + min(lane, n)), ck = __ldg(p.cu_k + min(lane, n));
+    const bool below = lane < n && clamp_to(cq, 0, p.t_q) / span + lane <= slot;
+    lo = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
+    q0 = __shfl_sync(0xffffffffu, cq, lo);
+    q1 = __shfl_sync(0xffffffffu, cq, lo + 1);
+    k0 = __shfl_sync(0xffffffffu, ck, lo);
+    k1 = __shfl_sync(0xffffffffu, ck, lo + 1);
+    n = 0;
+  }
   while (n > 1) {
     const int step = (n + 31) / 32;
     const int at = lo + lane * step;
@@ -239,7 +219,9 @@ __device__ __forceinline__ Work find_work(const DenseParams& p, int slot, int sp
     n = min(step, n - last * step);
     lo += last * step;
   }
-  const int q0 = __ldg(p.cu_q + lo), q1 = __ldg(p.cu_q + lo + 1), k0 = __ldg(p.cu_k + lo), k1 = __ldg(p.cu_k + lo + 1);
+  if (n > 0) {
+    q0 = __ldg(p.cu_q + lo), q1 = __ldg(p.cu_q + lo + 1), k0 = __ldg(p.cu_k + lo), k1 = __ldg(p.cu_k + lo + 1);
+  }
   w.q0 = clamp_to(q0, 0, p.t_q);
   w.len_q = clamp_to(q1, w.q0, p.t_q) - w.q0;
   w.k0 = clamp_to(k0, 0, p.t_k);
@@ -307,40 +289,8 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   DenseCtrl& ctrl = *reinterpret_cast<DenseCtrl*>(smem_raw + (base - raw) + C::Q_BYTES + C::K_BYTES + C::V_BYTES);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (warp == WARP_TMA && lane < 3) tma_prefetch_map(lane == 0 ? &p.mq : lane == 1 ? &p.mk : &p.mv);
-  grid_dependency_wait();
-  // Slots last to first: in a causal sequence the late rows are the long ones.
-  const int chunk = blockIdx.x % p.chunks;
-  const int slot = p.slots - 1 - static_cast<int>(blockIdx.x / p.chunks);
-  const int split = blockIdx.z;
-  const Work w = find_work<RANGES>(p, slot, split);
-  const bool twin = RANGES && w.twin;
-  if (!w.any) return;
-  const int head0 = chunk * p.pack;
-  const int kvh = head0 / (p.h_q / p.h_kv);
-  const int n_tiles = w.tiles;
-
-  if (n_tiles == 0) {                     // nothing in this CTA's range: results of empty rows
-    const int rows = 2 * p.tok_tile * p.pack;
-    for (int i = tid; i < rows; i += THREADS) {
-      const int tok = w.t0 + i / p.pack, h = head0 + i % p.pack;
-      if (tok >= w.len_q) continue;
-      const int64_t t = w.q0 + tok;
-      float f;
-      if (RANGES) {                       // (a set without weight: its values are not read)
-        store_stats(p, 2 * split, t, h, -INFINITY, -INFINITY, 0.f, false, f);
-        store_stats(p, 2 * split + 1, t, h, -INFINITY, -INFINITY, 0.f, false, f);
-      } else {
-        store_stats(p, 0, t, h, -INFINITY, -INFINITY, 0.f, false, f);
-        uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + t * p.stride_o_t + h * p.stride_o_h);
-        for (int c = 0; c < DV / 8; ++c) d[c] = make_uint4(0, 0, 0, 0);
-      }
-    }
-    return;
-  }
-
   auto bar = [&](uint64_t* x) { return smem_u32(x); };
-  if (warp == WARP_QK) {
+  if (warp == WARP_LOOK) {      // (the warp that has nothing to do at the start)
     if (lane == 0) {
       for (int s = 0; s < 2; ++s) {
         mbar_init(bar(&ctrl.q_full[s]), 1);
@@ -364,7 +314,44 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     __syncwarp();
     tmem_alloc(smem_u32(&ctrl.tmem), TMEM_COLS);
     tmem_relinquish();
+  } else if (warp == WARP_TMA && lane < 3) {
+    tma_prefetch_map(lane == 0 ? &p.mq : lane == 1 ? &p.mk : &p.mv);
   }
+  grid_dependency_wait();
+  // Slots last to first: in a causal sequence the late rows are the long ones.
+  const int chunk = blockIdx.x % p.chunks;
+  const int slot = p.slots - 1 - static_cast<int>(blockIdx.x / p.chunks);
+  const int split = blockIdx.z;
+  const Work w = find_work<RANGES>(p, slot, split);
+  const bool twin = RANGES && w.twin;
+  if (!w.any) {
+    if (warp == WARP_LOOK) tmem_dealloc(ctrl.tmem, TMEM_COLS);
+    return;
+  }
+  const int head0 = chunk * p.pack;
+  const int kvh = head0 / (p.h_q / p.h_kv);
+  const int n_tiles = w.tiles;
+
+  if (n_tiles == 0) {                     // nothing in this CTA's range: results of empty rows
+    const int rows = 2 * p.tok_tile * p.pack;
+    for (int i = tid; i < rows; i += THREADS) {
+      const int tok = w.t0 + i / p.pack, h = head0 + i % p.pack;
+      if (tok >= w.len_q) continue;
+      const int64_t t = w.q0 + tok;
+      float f;
+      if (RANGES) {                       // (a set without weight: its values are not read)
+        store_stats(p, 2 * split, t, h, -INFINITY, -INFINITY, 0.f, false, f);
+        store_stats(p, 2 * split + 1, t, h, -INFINITY, -INFINITY, 0.f, false, f);
+      } else {
+        store_stats(p, 0, t, h, -INFINITY, -INFINITY, 0.f, false, f);
+        uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + t * p.stride_o_t + h * p.stride_o_h);
+        for (int c = 0; c < DV / 8; ++c) d[c] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    if (warp == WARP_LOOK) tmem_dealloc(ctrl.tmem, TMEM_COLS);
+    return;
+  }
+
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -559,7 +546,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    if (warp == WARP_QK) tmem_dealloc(tmem, TMEM_COLS);
+    if (warp == WARP_LOOK) tmem_dealloc(tmem, TMEM_COLS);
     return;
   }
 
@@ -572,7 +559,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   const int h = head0 + row % p.pack;
   const bool live = row < p.pack * p.tok_tile && tok < w.len_q;
   const int reach = live ? reach_of(p, w, tok) : 0;
-  const int n_mine = w.count[s];
+  const int n_mine = s == 0 ? w.count[0] : w.count[1];
   const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
   const uint32_t tS = tmem + lanes + C::COL_S + (C::S_BUFS == 1 ? 0 : 128 * s), tP = tmem + lanes + C::COL_P + 64 * s;
   const uint32_t tO = tmem + lanes + C::COL_O + DV * s;
@@ -644,31 +631,20 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     if (!(top2 < INFINITY)) l = NAN;                 // a NaN or infinite score: the row shows it
     const uint64_t c2 = pair(c, c), minus_ref = pair(-ref, -ref);
     uint64_t sum[2] = {0, 0};
-    // A share of the exponentials goes to the FMA pipe: of four pairs EMULATED are computed there.
-    // (Not in a tile with masked keys: their weights have to be zero.)
-    auto weights = [&](auto masked) {
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t pk[32];
+    for (int q = 0; q < 4; ++q) {
+      uint32_t pk[16];
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          const uint64_t y = fma_pair(pair(__uint_as_float(x[64 * q + 2 * k]), __uint_as_float(x[64 * q + 2 * k + 1])), c2, minus_ref);
-          float a, b;
-          if (!decltype(masked)::value && (k & 3) < EMULATED) {
-            ex2_pair(y, a, b);
-          } else {
-            unpair(y, a, b);
-            a = ex2(a);
-            b = ex2(b);
-          }
-          sum[k & 1] = add_pair(sum[k & 1], pair(a, b));
-          pk[k] = pack2<BF16>(a, b);
-        }
-        tmem_st32(tP + 32 * q, pk);
+      for (int j = 0; j < 16; ++j) {
+        float a, b;
+        unpair(fma_pair(pair(__uint_as_float(x[32 * q + 2 * j]), __uint_as_float(x[32 * q + 2 * j + 1])), c2, minus_ref), a, b);
+        a = ex2(a);
+        b = ex2(b);
+        sum[j & 1] = add_pair(sum[j & 1], pair(a, b));
+        pk[j] = pack2<BF16>(a, b);
       }
-    };
-    if (tile >= whole) weights(std::true_type{});
-    else weights(std::false_type{});
+      tmem_st16(tP + 16 * q, pk);
+    }
     float s0, s1, s2, s3;
     unpair(sum[0], s0, s1);
     unpair(sum[1], s2, s3);
