@@ -468,15 +468,25 @@ int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* a, void* stream) {
 int dsv4_plan_dense_splits(int t_q, int t_k, int b, int h_q, int h_kv, int num_sms) {
   if (t_q < 1 || t_k < 1 || b < 1 || h_q < 1 || h_kv < 1 || h_q % h_kv || num_sms < 1) return 1;
   const int64_t ctas = dsv4::dense_ctas(t_q, b, h_q, h_kv);
-  const int64_t tiles = (static_cast<int64_t>(t_k) / b + 127) / 128;   // of a sequence, on average
-  if (ctas >= num_sms || tiles <= 2) return 1;
-  // In tile times: waves of CTAs, each with its own start and end; joining costs once.
-  const double fixed = 3.0, join = 4.0;
+  const double tiles = static_cast<double>(t_k) / b / 128.0;           // of a sequence, on average
+  if (ctas >= num_sms || tiles <= 2.0) return 1;
+  // In microseconds, fitted to calls of 1 to 60 sequences on a B200: a CTA starts and ends in 5,
+  // streams a tile of 128 keys in 1 (64 to 80 KB, what its buffers keep in flight), and the
+  // GPU's memory gives a tile in 0.0105; joining costs 3 and 0.15 a range.  The lengths are on
+  // the device: the longest sequence is taken to be three times the average one, and a plan of
+  // more CTAs than SMs to end 15 % unevenly.  (One sequence of 8000 keys, 64 heads on one: 78 us
+  // uncut, 23 in 8 ranges; 8 of 1000 to 16383 keys, 32 heads on 8: 105 and 61; 32 of 4096 fill
+  // the GPU: 95 uncut, 113 in 2.)
+  const double total = static_cast<double>(t_k) / 128.0;
+  const double longest = tiles * 3.0 < total ? tiles * 3.0 : total;
   int best = 1;
   double best_cost = 1e30;
   for (int s = 1; s <= dsv4::DENSE_MAX_SPLITS && s <= tiles; ++s) {
-    const int64_t waves = (ctas * s + num_sms - 1) / num_sms;
-    const double cost = waves * ((tiles + s - 1) / s + fixed) + (s > 1 ? join : 0.0);
+    const double at_once = ctas * s < num_sms ? static_cast<double>(ctas) * s : num_sms;
+    const double chain = 5.0 + longest / s;
+    const double streamed = ctas * tiles / at_once > ctas * tiles * 0.0105 ? ctas * tiles / at_once : ctas * tiles * 0.0105;
+    const double all = (ctas * s * 5.0 / num_sms + streamed) * (ctas * s > num_sms ? 1.15 : 1.0);
+    const double cost = (chain > all ? chain : all) + (s > 1 ? 3.0 + 0.15 * s : 0.0);
     if (cost < best_cost - 1e-9) { best_cost = cost; best = s; }
   }
   return best;

@@ -715,11 +715,14 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   __syncthreads();
 }
 
-// Joins the partials of the key ranges: one warp per (token, head), in range order.
+// Joins the partials of the key ranges: one warp per (token, head), in range order.  A lane looks
+// at up to four sets' log-sum-exps, so that no load waits for another one; the values of eight
+// sets are in flight at a time.
 template <int DV, bool BF16>
 __global__ void __launch_bounds__(256)
 dense_combine_kernel(const __grid_constant__ DenseParams p) {
   constexpr int PER = DV / 32;
+  static_assert(2 * DENSE_MAX_SPLITS <= 128, "four sets a lane");
   grid_dependency_wait();
   const int lane = threadIdx.x & 31;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -727,24 +730,62 @@ dense_combine_kernel(const __grid_constant__ DenseParams p) {
   const int64_t t = item / p.h_q;
   const int h = static_cast<int>(item - t * p.h_q);
   if (t < __ldg(p.cu_q) || t >= __ldg(p.cu_q + p.b)) return;   // a row of no sequence stays as it is
-  float ml = -INFINITY, top = -INFINITY;
-  for (int s = 0; s < 2 * p.n_splits; ++s) {
-    const float2 v = *reinterpret_cast<const float2*>(p.stat_accum + ((static_cast<int64_t>(s) * p.t_q + t) * p.h_q + h) * 2);
-    ml = fmaxf(ml, v.x);
-    top = (v.y != v.y || top != top) ? NAN : fmaxf(top, v.y);  // a failed part shows
+  const int sets = 2 * p.n_splits;
+  const int64_t rows = static_cast<int64_t>(p.t_q) * p.h_q;
+  float e[4], ml = -INFINITY, top = -INFINITY;
+  bool failed = false;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int s = 32 * k + lane;
+    float2 v = make_float2(-INFINITY, -INFINITY);
+    if (s < sets) v = *reinterpret_cast<const float2*>(p.stat_accum + (s * rows + item) * 2);
+    e[k] = v.y;
+    failed |= v.y != v.y;
+    ml = max3(ml, v.x, -INFINITY);
+    top = fmaxf(top, v.y);
   }
-  float acc[PER], sum = 0.f;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    ml = max3(ml, __shfl_xor_sync(0xffffffffu, ml, d), -INFINITY);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  }
+  if (__any_sync(0xffffffffu, failed)) top = NAN;              // a failed part, or NaN scores, show
+  float w[4], sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    w[k] = e[k] == -INFINITY ? 0.f : expf(e[k] - top);
+    sum += w[k];
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  float acc[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) acc[k] = 0.f;
-  if (top != -INFINITY) {
-    for (int s = 0; s < 2 * p.n_splits; ++s) {
-      const int64_t at = (static_cast<int64_t>(s) * p.t_q + t) * p.h_q + h;
-      const float e = p.stat_accum[at * 2 + 1];
-      if (e == -INFINITY) continue;
-      const float wgt = expf(e - top);
-      sum += wgt;
+  const float* src = p.o_accum + item * DV + lane * PER;
 #pragma unroll
-      for (int k = 0; k < PER; ++k) acc[k] = fmaf(wgt, p.o_accum[at * DV + lane * PER + k], acc[k]);
+  for (int k = 0; k < 4; ++k) {
+    for (int s0 = 32 * k; s0 < min(sets, 32 * k + 32); s0 += 8) {
+      float v[8][PER], ws[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        ws[j] = __shfl_sync(0xffffffffu, w[k], (s0 + j) & 31);
+#pragma unroll
+        for (int q = 0; q < PER; ++q) v[j][q] = 0.f;
+        if (ws[j] != 0.f) {                                    // (the values of a set without weight are not written)
+          const float* a = src + (s0 + j) * rows * DV;
+          if constexpr (PER == 4) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(a));
+            v[j][0] = f.x, v[j][1] = f.y, v[j][2] = f.z, v[j][3] = f.w;
+          } else {
+            const float2 f = __ldg(reinterpret_cast<const float2*>(a));
+            v[j][0] = f.x, v[j][1] = f.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int q = 0; q < PER; ++q) acc[q] = fmaf(ws[j], v[j][q], acc[q]);
     }
   }
   const bool none = top == -INFINITY;
