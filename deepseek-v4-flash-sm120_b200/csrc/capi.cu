@@ -320,22 +320,48 @@ int dsv4_sparse_prefill(const Dsv4PrefillArgs* a, void* stream) {
   return e ? cuda_fail(e) : DSV4_OK;
 }
 
-// Splits of the two parts of a shared-prefix decode, and its scratch.
+// How a shared-prefix decode is done, and its scratch.
+//   JOINED  one list per query token, of the prefix and its own tokens, for the sparse kernel:
+//           reads the prefix once per request, but is two or three short launches;
+//   DENSE   the prefix by launch_prefix_attn, the own tokens by the sparse kernel, joined;
+//   LISTS   the same with the prefix by the sparse kernel too, as one list for all rows.
+enum SharedForm { FORM_JOINED, FORM_DENSE, FORM_LISTS };
 struct SharedPlan {
-  int prefix_sets, suffix_splits;          // partial sets of the two parts; 0: the part does not exist
-  bool dense;                              // the prefix by launch_prefix_attn, else by an index list
+  SharedForm form;
+  int prefix_sets, suffix_splits;          // partial sets of the two parts (JOINED: splits in the second)
   int64_t prefix_bytes, suffix_bytes;      // of the workspace: the prefix's part, then the lists
 };
-// The dense form converts the whole prefix first and works in blocks of 128 rows; below this
-// many rows the list form, which reads the FP8 rows as they are, is faster.
-constexpr int64_t DENSE_PREFIX_ROWS = 65;
+static SharedForm choose_form(const Dsv4SharedPrefixArgs* a, int64_t rows, int64_t plen, int64_t slen, int num_sms) {
+  const bool by_list = a->prefix_splits > 0 || a->suffix_splits > 0 || want_simple(a->flags);
+  if (by_list || plen + slen == 0 || (a->flags & DSV4_FLAG_SHARED_LISTS)) return FORM_LISTS;
+  if (plen == 0 || (a->flags & DSV4_FLAG_SHARED_JOINED)) return FORM_JOINED;
+  if (a->flags & DSV4_FLAG_SHARED_DENSE) return FORM_DENSE;
+  // JOINED up to four tiles of 128 tokens an SM (for blocks of up to 64 rows) and lists of 16384
+  // tokens (microseconds, JOINED / DENSE / LISTS, tokens a request x requests x heads: 2100 x 4 x
+  // 16: 18 / 35 / 33; 2100 x 16 x 64: 27 / 40 / 41; 4100 x 16 x 64, 528 tiles: 37 / 43 / 49;
+  // 20100 x 8 x 8, 1264 tiles: 60 / 43 / 39; 30100 x 1 x 64: 53 / 53 / 43).
+  const int64_t tiles = static_cast<int64_t>(a->b) * a->s_q * ((a->h_q + 63) / 64) * ((plen + slen + 127) / 128);
+  if (tiles <= 4 * num_sms && plen + slen <= 16384) return FORM_JOINED;
+  // LISTS up to 128 rows: converting the whole prefix costs more than reading its FP8 rows twice
+  // (30100 x 4 x 16, 64 rows: 49 DENSE, 41 LISTS; 10100 x 4 x 32: 41 and 39; 4100 x 8 x 64, 512
+  // rows: 39 and 41; 33000 x 64 x 64: 269 and 667).
+  return rows > 128 ? FORM_DENSE : FORM_LISTS;
+}
+
 static SharedPlan plan_shared(const Dsv4SharedPrefixArgs* a, int num_sms) {
   SharedPlan p{};
   const int64_t rows = static_cast<int64_t>(a->b) * a->s_q * a->h_q;
   const int64_t plen = static_cast<int64_t>(a->prefix_pages) * a->page_block_size;
   const int64_t slen = static_cast<int64_t>(a->max_pages) * a->page_block_size;
-  p.dense = plen > 0 && a->prefix_splits == 0 && rows >= DENSE_PREFIX_ROWS && !want_simple(a->flags);
-  if (p.dense) {
+  const int64_t tokens = static_cast<int64_t>(a->b) * a->s_q;
+  const int64_t most = 0x7fffffff;
+  p.form = choose_form(a, rows, plen, slen, num_sms);
+  if (p.form == FORM_JOINED) {
+    p.suffix_splits = dsv4_plan_splits(a->b, a->s_q, a->h_q, static_cast<int>(plen + slen < most ? plen + slen : most), 0, num_sms);
+    p.suffix_bytes = (tokens * (plen + slen) + a->b) * 4;
+    return p;
+  }
+  if (p.form == FORM_DENSE) {
     p.prefix_sets = dsv4::prefix_attn_sets(rows, num_sms);
     p.prefix_bytes = dsv4::prefix_attn_workspace(plen, a->d_qk);
   } else if (plen > 0) {
@@ -346,7 +372,7 @@ static SharedPlan plan_shared(const Dsv4SharedPrefixArgs* a, int num_sms) {
   if (slen > 0)
     p.suffix_splits = a->suffix_splits > 0 ? a->suffix_splits
                                            : dsv4_plan_splits(a->b, a->s_q, a->h_q, static_cast<int>(slen), 0, num_sms);
-  p.suffix_bytes = slen * a->b * a->s_q * 4;
+  p.suffix_bytes = slen * tokens * 4;
   return p;
 }
 
@@ -360,6 +386,7 @@ static int check_shared(const Dsv4SharedPrefixArgs* a) {
   if (static_cast<int64_t>(a->num_blocks) * a->page_block_size > most ||
       static_cast<int64_t>(a->prefix_pages) * a->page_block_size > most ||
       static_cast<int64_t>(a->max_pages) * a->page_block_size > most ||
+      (static_cast<int64_t>(a->prefix_pages) + a->max_pages) * a->page_block_size > most ||
       static_cast<int64_t>(a->b) * a->s_q > most / a->h_q ||
       static_cast<int64_t>(a->b) * a->s_q * a->h_q > 64ll * 65535)
     return DSV4_ERR_SHAPE;
@@ -373,6 +400,7 @@ int dsv4_shared_prefix_scratch(const Dsv4SharedPrefixArgs* a, int num_sms, int32
   if (num_sms < 2) return DSV4_ERR_SHAPE;
   const SharedPlan p = plan_shared(a, num_sms);
   *sets = p.prefix_sets + p.suffix_splits;
+  if (p.form == FORM_JOINED && p.suffix_splits == 1) *sets = 0;      // final at once
   *bytes = p.prefix_bytes + p.suffix_bytes;
   return DSV4_OK;
 }
@@ -396,16 +424,51 @@ int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* a, void* stream) {
   if ((rc = device_info(dev, info))) return rc;
   const SharedPlan plan = plan_shared(a, info.sms);
   const int sets = plan.prefix_sets + plan.suffix_splits;
-  if (sets > 0) {
-    if (!a->o_accum || !a->lse_accum || !a->workspace) return DSV4_ERR_SCRATCH;
-    if (!aligned16(a->o_accum) || !aligned16(a->workspace)) return DSV4_ERR_ALIGN;
+  if (sets > 0 && (plan.form != FORM_JOINED || sets > 1)) {
+    if (!a->o_accum || !a->lse_accum) return DSV4_ERR_SCRATCH;
+    if (!aligned16(a->o_accum)) return DSV4_ERR_ALIGN;
+  }
+  if (plan.prefix_bytes + plan.suffix_bytes > 0) {
+    if (!a->workspace) return DSV4_ERR_SCRATCH;
+    if (!aligned16(a->workspace)) return DSV4_ERR_ALIGN;
   }
   const int64_t rows = static_cast<int64_t>(a->b) * a->s_q * a->h_q;
-  int32_t* prefix_list = plan.dense ? nullptr : static_cast<int32_t*>(a->workspace);
-  int32_t* suffix_list = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(a->workspace) + plan.prefix_bytes);
+  const int64_t plen = static_cast<int64_t>(a->prefix_pages) * a->page_block_size;
+  const int64_t slen = static_cast<int64_t>(a->max_pages) * a->page_block_size;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if ((e = dsv4::launch_shared_lists(*a, prefix_list, suffix_list, st))) return cuda_fail(e);
-  if (plan.dense && (e = dsv4::launch_prefix_attn(*a, a->workspace, info.sms, st))) return cuda_fail(e);
+  int32_t* lists = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(a->workspace) + plan.prefix_bytes);
+  dsv4::SharedSetup setup{};
+  if (plan.form == FORM_DENSE) dsv4::prefix_attn_place(plen, a->workspace, setup);
+  if (plan.form == FORM_LISTS && plen > 0) setup.prefix_list = static_cast<int32_t*>(a->workspace);
+  if (plan.form == FORM_JOINED) {
+    setup.joined = lists;
+    setup.lens = lists + static_cast<int64_t>(a->b) * a->s_q * (plen + slen);
+  } else if (slen > 0) {
+    setup.suffix_lists = lists;
+  }
+  if ((e = dsv4::launch_shared_setup(*a, setup, st))) return cuda_fail(e);
+
+  if (plan.form == FORM_JOINED) {
+    Dsv4DecodeArgs d{};
+    d.b = a->b; d.s_q = a->s_q; d.h_q = a->h_q; d.d_qk = a->d_qk; d.d_v = a->d_v;
+    d.topk = static_cast<int>(plen + slen);
+    d.kv_format = a->kv_format; d.num_blocks = a->num_blocks; d.page_block_size = a->page_block_size;
+    d.n_splits = plan.suffix_splits;
+    d.flags = DSV4_FLAG_MASK_INVALID | DSV4_FLAG_ZERO_LENGTH_EMPTY;
+    d.sm_scale = a->sm_scale;
+    d.q = a->q; d.kv = a->kv; d.indices = setup.joined; d.topk_length = setup.lens; d.attn_sink = a->attn_sink;
+    d.out = a->out; d.lse = a->lse; d.o_accum = a->o_accum; d.lse_accum = a->lse_accum;
+    d.stride_q_h = a->d_qk;
+    d.stride_q_s = static_cast<int64_t>(a->h_q) * a->d_qk;
+    d.stride_q_b = d.stride_q_s * a->s_q;
+    d.stride_kv_block = a->stride_kv_block;
+    d.stride_indices_s = d.topk;
+    d.stride_indices_b = static_cast<int64_t>(d.topk) * a->s_q;
+    d.stride_o_b = a->stride_o_b; d.stride_o_s = a->stride_o_s; d.stride_o_h = a->stride_o_h;
+    d.stride_lse_b = a->stride_lse_b; d.stride_lse_s = a->stride_lse_s; d.stride_lse_h = a->stride_lse_h;
+    return dsv4_sparse_decode(&d, stream);
+  }
+  if (plan.form == FORM_DENSE && (e = dsv4::launch_prefix_attn(*a, setup, info.sms, st))) return cuda_fail(e);
 
   dsv4::AttnParams p{};
   p.cluster = 1;
@@ -427,13 +490,13 @@ int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* a, void* stream) {
     return want_simple(a->flags) ? dsv4::launch_simple_attn(p, a->kv_format, a->d_qk, st)
                                  : dsv4::launch_sm100_attn(p, a->kv_format, a->d_qk, st);
   };
-  if (plan.prefix_sets > 0 && !plan.dense) {
+  if (plan.prefix_sets > 0 && plan.form == FORM_LISTS) {
     // the rows of all requests as the heads of one: each block of 64 rows walks the prefix once
     p.n_req = p.s_q = 1;
     p.h_q = static_cast<int>(rows);
     p.topk = a->prefix_pages * a->page_block_size;
     p.n_splits = plan.prefix_sets;
-    p.indices = prefix_list;
+    p.indices = setup.prefix_list;
     p.topk_length = a->prefix_length;
     p.o_accum = a->o_accum;
     p.lse_accum = a->lse_accum;
@@ -445,7 +508,7 @@ int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* a, void* stream) {
     p.h_q = a->h_q;
     p.topk = a->max_pages * a->page_block_size;
     p.n_splits = plan.suffix_splits;
-    p.indices = suffix_list;
+    p.indices = setup.suffix_lists;
     p.topk_length = a->suffix_length;
     p.stride_q_s = static_cast<int64_t>(a->h_q) * a->d_qk;
     p.stride_q_b = p.stride_q_s * a->s_q;
@@ -461,7 +524,7 @@ int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* a, void* stream) {
   c.out = a->out; c.lse = a->lse;
   c.stride_o_b = a->stride_o_b; c.stride_o_s = a->stride_o_s; c.stride_o_h = a->stride_o_h;
   c.stride_lse_b = a->stride_lse_b; c.stride_lse_s = a->stride_lse_s; c.stride_lse_h = a->stride_lse_h;
-  e = dsv4::launch_combine(c, st);
+  e = dsv4::launch_join_sets(c, st);
   return e ? cuda_fail(e) : DSV4_OK;
 }
 

@@ -41,16 +41,28 @@ cudaError_t launch_gather_dequant(const void* kv, int64_t stride, int kv_format,
 constexpr int SLOT_MAP_MAX_REQUESTS = 16384;     // both sums of a request list in shared memory
 cudaError_t launch_slot_maps(const Dsv4SlotMapArgs& a, cudaStream_t st);
 cudaError_t launch_page_indices(const Dsv4PageIndicesArgs& a, cudaStream_t st);
-// Token indices of the first length[0] tokens of one table row (`prefix`), and of every
-// request's own tokens as each of its s_q query tokens sees them (`suffix`, one list of
-// max_pages * page tokens per query token).  A null `prefix` leaves that part out.
-cudaError_t launch_shared_lists(const Dsv4SharedPrefixArgs& a, int32_t* prefix, int32_t* suffix, cudaStream_t st);
+
+// Set-up of a shared-prefix decode (shared_prefix_sm100.cu), one launch: what is not null of
+//   rows, valid    the prefix as BF16 rows, and a bit per token (prefix_attn_place says where),
+//   prefix_list    token indices of the prefix,
+//   suffix_lists   of every query token's own tokens, a list of max_pages * page entries each,
+//   joined, lens   both one after the other, prefix_pages * page entries more each, and the
+//                  requests' list lengths.
+struct SharedSetup {
+  void* rows;
+  uint32_t* valid;
+  int32_t *prefix_list, *suffix_lists, *joined, *lens;
+};
+cudaError_t launch_shared_setup(const Dsv4SharedPrefixArgs& a, const SharedSetup& out, cudaStream_t st);
+// Joins partial sets of BF16 outputs (like launch_combine, for few sets and many rows).
+cudaError_t launch_join_sets(const Dsv4CombineArgs& a, cudaStream_t st);
 
 // Attention of many rows over a shared prefix, into the first prefix_attn_sets partial sets
 // (shared_prefix_sm100.cu).
 int prefix_attn_sets(int64_t rows, int num_sms);
 int64_t prefix_attn_workspace(int64_t tokens, int d_qk);       // bytes
-cudaError_t launch_prefix_attn(const Dsv4SharedPrefixArgs& a, void* workspace, int num_sms, cudaStream_t st);
+void prefix_attn_place(int64_t tokens, void* workspace, SharedSetup& out);
+cudaError_t launch_prefix_attn(const Dsv4SharedPrefixArgs& a, const SharedSetup& rows, int num_sms, cudaStream_t st);
 cudaError_t read_prefix_error(int* value, bool reset);
 
 // Dense attention over packed sequences (dense_attn_sm100.cu).

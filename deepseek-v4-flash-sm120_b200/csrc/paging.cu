@@ -20,6 +20,7 @@
 
 #include "attn_params.cuh"
 #include "launchers.h"
+#include "paging.cuh"
 
 namespace dsv4 {
 namespace {
@@ -160,30 +161,6 @@ slot_maps_kernel(const Dsv4SlotMapArgs a) {
   }
 }
 
-// Division of n < 2^31 by a constant: (umulhi(mul, n) + n) >> shift.
-struct FastDiv {
-  uint32_t mul, shift, d;
-};
-FastDiv fast_div(uint32_t d) {
-  uint32_t l = 0;
-  while ((1ull << l) < d) ++l;
-  const uint64_t m = ((1ull << 32) * ((1ull << l) - d)) / d + 1;
-  return FastDiv{static_cast<uint32_t>(m), l, d};
-}
-__device__ __forceinline__ uint32_t div_by(uint32_t n, const FastDiv& f) {
-  return (__umulhi(f.mul, n) + n) >> f.shift;
-}
-
-__device__ __forceinline__ int slot_of(const int32_t* table, int max_pages, const FastDiv& page, int pos) {
-  if (pos < 0) return -1;
-  const uint32_t col = div_by(static_cast<uint32_t>(pos), page);
-  if (col >= static_cast<uint32_t>(max_pages)) return -1;
-  const int id = __ldg(table + col);
-  if (id < 0) return -1;
-  const long long s = static_cast<long long>(id) * page.d + (static_cast<uint32_t>(pos) - col * page.d);
-  return s > MAX_I32 ? -1 : static_cast<int>(s);
-}
-
 // threadIdx.x walks a row, threadIdx.y and the grid the rows.
 template <bool VEC>
 __global__ void __launch_bounds__(256)
@@ -223,52 +200,10 @@ page_indices_kernel(const Dsv4PageIndicesArgs a, const FastDiv page) {
   }
 }
 
-// Index lists of a batch behind a shared prefix.  The first `prefix_ctas` CTAs write the
-// prefix's list, the others one query token's list each.  Only entries below the length are
-// written: nothing reads the others.
-__global__ void __launch_bounds__(256)
-shared_lists_kernel(const Dsv4SharedPrefixArgs a, const FastDiv page, int prefix_ctas, int32_t* prefix, int32_t* suffix) {
-  grid_dependency_wait();
-  const int n_tok = a.num_blocks * a.page_block_size;
-  auto entry = [&](const int32_t* table, int pages, int pos) {
-    const int s = slot_of(table, pages, page, pos);
-    return s < n_tok ? s : -1;
-  };
-  if (static_cast<int>(blockIdx.x) < prefix_ctas) {
-    const int n = min(max(*a.prefix_length, 0), a.prefix_pages * a.page_block_size);
-    for (int j = blockIdx.x * 256 + threadIdx.x; j < n; j += prefix_ctas * 256)
-      prefix[j] = entry(a.prefix_table, a.prefix_pages, j);
-    return;
-  }
-  const int row = blockIdx.x - prefix_ctas, r = row / a.s_q, s = row % a.s_q;
-  const int width = a.max_pages * a.page_block_size;
-  const int n = min(max(a.suffix_length[r], 0), width);
-  const int sees = n - (a.s_q - 1 - s);
-  for (int j = threadIdx.x; j < n; j += 256)
-    suffix[static_cast<int64_t>(row) * width + j] =
-        j < sees ? entry(a.block_table + r * a.stride_table, a.max_pages, j) : -1;
-}
-
 constexpr int MAX_DEVICES = 64;
 std::mutex g_paging_mu;
 
 }  // namespace
-
-cudaError_t launch_shared_lists(const Dsv4SharedPrefixArgs& a, int32_t* prefix, int32_t* suffix, cudaStream_t st) {
-  const int64_t n = static_cast<int64_t>(a.prefix_pages) * a.page_block_size;
-  const int prefix_ctas = prefix == nullptr ? 0 : static_cast<int>(n < 64 * 1024 ? (n + 1023) / 1024 : 64);
-  const int rows = a.max_pages > 0 ? a.b * a.s_q : 0;
-  if (prefix_ctas + rows == 0) return cudaSuccess;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(prefix_ctas + rows);
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  cfg.attrs = attr;
-  cfg.numAttrs = add_overlap_attribute(attr);
-  return cudaLaunchKernelEx(&cfg, shared_lists_kernel, a, fast_div(static_cast<uint32_t>(a.page_block_size)),
-                            prefix_ctas, prefix, suffix);
-}
 
 cudaError_t launch_slot_maps(const Dsv4SlotMapArgs& a, cudaStream_t st) {
   const size_t smem = 2 * (static_cast<size_t>(a.b) + 1) * sizeof(int);

@@ -1,7 +1,7 @@
 // Attention of many query rows over one prefix: the shared part of a batch's decode.
 //
 // The rows of all requests and heads (b * s_q * h_q of them) see the same tokens, so the FP8
-// rows of the prefix are converted to BF16 once (prefix_rows_kernel), and the products run
+// rows of the prefix are converted to BF16 once (shared_setup_kernel), and the products run
 // over blocks of 128 query rows as a dense attention with d_qk 576 or 512 and V the first 512
 // columns of the same rows.
 //
@@ -31,6 +31,7 @@
 
 #include "attn_params.cuh"
 #include "launchers.h"
+#include "paging.cuh"
 #include "sm100_ptx.cuh"
 #include "tensor_map.h"
 
@@ -511,26 +512,60 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
 }
 
-// FP8 rows of the prefix -> BF16 rows [tokens, d_qk], and a bit per token that says whether it
-// exists; rows that do not are zero.  Whole tiles of 128 tokens are written.  Bound by memory:
-// 644 (584) B in and 1152 (1024) B out per token; a warp has four tokens in flight.
+// One launch for what the attention kernels read besides the cache.  CTAs [0, row_ctas): FP8 rows
+// of the prefix -> BF16 rows [tokens, d_qk], and a bit per token that says whether it exists; rows
+// that do not are zero.  Whole tiles of 128 tokens are written.  Bound by memory: 644 (584) B in
+// and 1152 (1024) B out per token; a warp has four tokens in flight.  CTAs [row_ctas, +list_ctas):
+// token indices of the prefix.  The others: one query token's list each, of its own tokens or of
+// the prefix and those.  List entries behind a length are not written: nothing reads them.
 template <int FMT>
 __global__ void __launch_bounds__(256)
-prefix_rows_kernel(const Dsv4SharedPrefixArgs a, __nv_bfloat16* rows, uint32_t* valid) {
+shared_setup_kernel(const Dsv4SharedPrefixArgs a, const SharedSetup out, const FastDiv page, int row_ctas, int list_ctas) {
   using T = KvTraits<FMT>;
   grid_dependency_wait();
-  const int len = min(max(*a.prefix_length, 0), a.prefix_pages * a.page_block_size);
+  const int prefix = a.prefix_pages > 0 ? min(max(*a.prefix_length, 0), a.prefix_pages * a.page_block_size) : 0;
+  const int n_tok = a.num_blocks * a.page_block_size;
+  auto entry = [&](const int32_t* table, int pages, int pos) {
+    const int s = slot_of(table, pages, page, pos);
+    return s < n_tok ? s : -1;
+  };
+  if (static_cast<int>(blockIdx.x) >= row_ctas) {
+    int x = blockIdx.x - row_ctas;
+    if (x < list_ctas) {
+      for (int j = x * 256 + threadIdx.x; j < prefix; j += list_ctas * 256)
+        out.prefix_list[j] = entry(a.prefix_table, a.prefix_pages, j);
+      return;
+    }
+    x -= list_ctas;
+    const int r = x / a.s_q, s = x % a.s_q;
+    const int width = a.max_pages * a.page_block_size;
+    const int own = a.max_pages > 0 ? min(max(a.suffix_length[r], 0), width) : 0;
+    const int sees = own - (a.s_q - 1 - s);
+    const int32_t* table = a.block_table + r * a.stride_table;
+    if (out.joined != nullptr) {
+      int32_t* list = out.joined + static_cast<int64_t>(x) * (a.prefix_pages * a.page_block_size + width);
+      for (int j = threadIdx.x; j < prefix; j += 256) list[j] = entry(a.prefix_table, a.prefix_pages, j);
+      for (int j = threadIdx.x; j < own; j += 256) list[prefix + j] = j < sees ? entry(table, a.max_pages, j) : -1;
+      if (s == 0 && threadIdx.x == 0) out.lens[r] = prefix + own;
+    } else {
+      int32_t* list = out.suffix_lists + static_cast<int64_t>(x) * width;
+      for (int j = threadIdx.x; j < own; j += 256) list[j] = j < sees ? entry(table, a.max_pages, j) : -1;
+    }
+    return;
+  }
+
   const int tok0 = blockIdx.x * 32;
-  if (tok0 >= (len + TILE - 1) / TILE * TILE) return;
+  if (tok0 >= (prefix + TILE - 1) / TILE * TILE) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // every warp knows where the CTA's 32 tokens live: lane i looks up token i
   const int tok = tok0 + lane;
+  const int col = static_cast<int>(div_by(static_cast<uint32_t>(tok), page));
   int id = -1;
-  if (tok < len) id = __ldg(a.prefix_table + tok / a.page_block_size);
+  if (tok < prefix) id = __ldg(a.prefix_table + col);
   const bool live = id >= 0 && id < a.num_blocks;
   const uint32_t word = __ballot_sync(0xffffffffu, live);
-  if (threadIdx.x == 0) valid[blockIdx.x] = word;
-  const int off = live ? tok % a.page_block_size : 0;
+  if (threadIdx.x == 0) out.valid[blockIdx.x] = word;
+  const int off = tok - col * a.page_block_size;
 
   const uint8_t* kv = static_cast<const uint8_t*>(a.kv);
   uint4 latent[4], rope[4];
@@ -538,22 +573,22 @@ prefix_rows_kernel(const Dsv4SharedPrefixArgs a, __nv_bfloat16* rows, uint32_t* 
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int i = warp * 4 + k;
-    const int page = __shfl_sync(0xffffffffu, id, i), at = __shfl_sync(0xffffffffu, off, i);
+    const int pg = __shfl_sync(0xffffffffu, id, i), at = __shfl_sync(0xffffffffu, off, i);
     latent[k] = rope[k] = make_uint4(0, 0, 0, 0);
     scale[k] = 127;
     if ((word >> i) & 1u) {
-      const uint8_t* pg = kv + static_cast<int64_t>(page) * a.stride_kv_block;
-      const uint8_t* row = pg + static_cast<int64_t>(at) * T::ROW_BYTES;
+      const uint8_t* base = kv + static_cast<int64_t>(pg) * a.stride_kv_block;
+      const uint8_t* row = base + static_cast<int64_t>(at) * T::ROW_BYTES;
       if (lane < T::D_NOPE / 16) {
         latent[k] = __ldg(reinterpret_cast<const uint4*>(row) + lane);
-        scale[k] = __ldg(pg + static_cast<int64_t>(a.page_block_size) * T::ROW_BYTES + at * T::SLOTS + lane * 16 / T::TILE);
+        scale[k] = __ldg(base + static_cast<int64_t>(a.page_block_size) * T::ROW_BYTES + at * T::SLOTS + lane * 16 / T::TILE);
       }
       if (lane < 8) rope[k] = __ldg(reinterpret_cast<const uint4*>(row + T::D_NOPE) + lane);
     }
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    uint4* dst = reinterpret_cast<uint4*>(rows + static_cast<int64_t>(tok0 + warp * 4 + k) * T::D_QK);
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out.rows) + static_cast<int64_t>(tok0 + warp * 4 + k) * T::D_QK);
     if (lane < T::D_NOPE / 16) {
       const ScalePair c = scale_pair(scale[k]);
       const bool two = scale[k] > MAX_ONE_MULTIPLY_SCALE;
@@ -566,6 +601,70 @@ prefix_rows_kernel(const Dsv4SharedPrefixArgs a, __nv_bfloat16* rows, uint32_t* 
       dst[2 * lane + 1] = make_uint4(o[4], o[5], o[6], o[7]);
     }
     if (lane < 8) dst[T::D_NOPE / 8 + lane] = rope[k];
+  }
+}
+
+// Joins few partial sets of many rows: one warp per (row, head), which has the whole 2 KB of four
+// sets in flight; sets in order, so that the result does not depend on timing.
+__global__ void __launch_bounds__(256)
+join_sets_kernel(const Dsv4CombineArgs a) {
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = static_cast<int64_t>(a.n_rows) * a.h_q;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (item >= rows) return;
+  const int row = static_cast<int>(item / a.h_q), h = static_cast<int>(item - static_cast<int64_t>(row) * a.h_q);
+  float e = -INFINITY;
+  if (lane < a.n_splits) e = a.lse_accum[lane * rows + item];
+  const bool failed = __any_sync(0xffffffffu, e != e);
+  float m = e;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  if (failed) m = NAN;
+  const float w = e == -INFINITY ? 0.f : expf(e - m);
+  float l = w;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  const bool has_sink = a.attn_sink != nullptr;
+  float lse_v, ml_v;
+  const float f = finalize_row(MODE_DECODE, m, l, has_sink, has_sink ? a.attn_sink[h] : 0.f, lse_v, ml_v);
+  float acc[16];
+#pragma unroll
+  for (int q = 0; q < 16; ++q) acc[q] = 0.f;
+  // lane: columns 8 * lane .. +8 of each half of the row
+  const float4* src = reinterpret_cast<const float4*>(a.o_accum + item * D_V) + 2 * lane;
+  for (int s0 = 0; s0 < a.n_splits; s0 += 4) {
+    float4 v[4][4];
+    float ws[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      ws[j] = s0 + j < a.n_splits ? __shfl_sync(0xffffffffu, w, s0 + j) : 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        v[j][q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (ws[j] != 0.f)                        // (a set without weight may hold anything)
+          v[j][q] = __ldg(src + (s0 + j) * rows * (D_V / 4) + (q >> 1) * 64 + (q & 1));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        acc[4 * q] = fmaf(ws[j], v[j][q].x, acc[4 * q]);
+        acc[4 * q + 1] = fmaf(ws[j], v[j][q].y, acc[4 * q + 1]);
+        acc[4 * q + 2] = fmaf(ws[j], v[j][q].z, acc[4 * q + 2]);
+        acc[4 * q + 3] = fmaf(ws[j], v[j][q].w, acc[4 * q + 3]);
+      }
+  }
+  const int bi = row / a.s_q, si = row % a.s_q;
+  if (lane == 0) a.lse[bi * a.stride_lse_b + si * a.stride_lse_s + h * a.stride_lse_h] = lse_v;
+  __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + bi * a.stride_o_b + si * a.stride_o_s + h * a.stride_o_h;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint32_t o[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) o[q] = pack_bf16x2(acc[8 * half + 2 * q] * f, acc[8 * half + 2 * q + 1] * f);
+    *reinterpret_cast<uint4*>(dst + half * 256 + 8 * lane) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -620,32 +719,57 @@ int64_t prefix_attn_workspace(int64_t tokens, int d_qk) {
   return round_up(padded / 8, 256) + padded * d_qk * 2;
 }
 
-cudaError_t launch_prefix_attn(const Dsv4SharedPrefixArgs& a, void* workspace, int num_sms, cudaStream_t st) {
-  const int64_t tokens = static_cast<int64_t>(a.prefix_pages) * a.page_block_size, padded = round_up(tokens, TILE);
-  uint32_t* valid = static_cast<uint32_t*>(workspace);
-  __nv_bfloat16* rows = reinterpret_cast<__nv_bfloat16*>(static_cast<uint8_t*>(workspace) + round_up(padded / 8, 256));
+void prefix_attn_place(int64_t tokens, void* workspace, SharedSetup& out) {
+  out.valid = static_cast<uint32_t*>(workspace);
+  out.rows = static_cast<uint8_t*>(workspace) + round_up(round_up(tokens, TILE) / 8, 256);
+}
+
+cudaError_t launch_shared_setup(const Dsv4SharedPrefixArgs& a, const SharedSetup& out, cudaStream_t st) {
+  const int64_t tokens = static_cast<int64_t>(a.prefix_pages) * a.page_block_size;
+  const int row_ctas = out.rows != nullptr ? static_cast<int>(round_up(tokens, TILE) / 32) : 0;
+  const int list_ctas = out.prefix_list == nullptr ? 0 : static_cast<int>(tokens < 64 * 1024 ? (tokens + 1023) / 1024 : 64);
+  const int lists = out.suffix_lists != nullptr || out.joined != nullptr ? a.b * a.s_q : 0;
+  if (row_ctas + list_ctas + lists == 0) return cudaSuccess;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(padded / 32));
+  cfg.gridDim = dim3(static_cast<unsigned>(row_ctas) + list_ctas + lists);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   cfg.attrs = attr;
   cfg.numAttrs = add_overlap_attribute(attr);
-  cudaError_t e = a.kv_format == DSV4_KV_V32 ? cudaLaunchKernelEx(&cfg, prefix_rows_kernel<DSV4_KV_V32>, a, rows, valid)
-                                             : cudaLaunchKernelEx(&cfg, prefix_rows_kernel<DSV4_KV_MODEL1>, a, rows, valid);
-  if (e) return e;
+  const FastDiv page = fast_div(static_cast<uint32_t>(a.page_block_size));
+  return a.kv_format == DSV4_KV_V32
+             ? cudaLaunchKernelEx(&cfg, shared_setup_kernel<DSV4_KV_V32>, a, out, page, row_ctas, list_ctas)
+             : cudaLaunchKernelEx(&cfg, shared_setup_kernel<DSV4_KV_MODEL1>, a, out, page, row_ctas, list_ctas);
+}
+
+cudaError_t launch_join_sets(const Dsv4CombineArgs& a, cudaStream_t st) {
+  if (a.n_splits > 32) return launch_combine(a, st);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(a.n_rows) * a.h_q + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  cfg.attrs = attr;
+  cfg.numAttrs = add_overlap_attribute(attr);
+  return cudaLaunchKernelEx(&cfg, join_sets_kernel, a);
+}
+
+cudaError_t launch_prefix_attn(const Dsv4SharedPrefixArgs& a, const SharedSetup& setup, int num_sms, cudaStream_t st) {
+  const int64_t tokens = static_cast<int64_t>(a.prefix_pages) * a.page_block_size, padded = round_up(tokens, TILE);
+  cudaError_t e;
   PrefixParams p;
   p.rows = a.b * a.s_q * a.h_q;
   p.sets = prefix_attn_sets(p.rows, num_sms);
   p.max_tokens = static_cast<int>(tokens);
   p.length = a.prefix_length;
-  p.valid = valid;
+  p.valid = setup.valid;
   p.sm_scale = a.sm_scale;
   p.o_accum = a.o_accum;
   p.lse_accum = a.lse_accum;
   if ((e = make_map_16bit(&p.mq, true, a.q, p.rows, 1, a.d_qk, a.d_qk, a.d_qk, ROWS, 1))) return e;
-  if ((e = make_map_16bit(&p.mk, true, rows, static_cast<int>(padded), 1, a.d_qk, a.d_qk, a.d_qk, ROWS, 1))) return e;
-  if ((e = make_map_16bit(&p.mv, true, rows, static_cast<int>(padded), 1, a.d_qk, a.d_qk, a.d_qk, TILE, 1))) return e;
+  if ((e = make_map_16bit(&p.mk, true, setup.rows, static_cast<int>(padded), 1, a.d_qk, a.d_qk, a.d_qk, ROWS, 1))) return e;
+  if ((e = make_map_16bit(&p.mv, true, setup.rows, static_cast<int>(padded), 1, a.d_qk, a.d_qk, a.d_qk, TILE, 1))) return e;
   return a.d_qk == 576 ? launch_attn<576>(p, num_sms / 2, st) : launch_attn<512>(p, num_sms / 2, st);
 }
 

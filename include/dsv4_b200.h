@@ -61,7 +61,13 @@ enum Dsv4Flags {
    * (csrc/sm120/decode/sparse_decode_kernel.cuh:373-375).  Default (flag clear)
    * follows the reference's torch oracle, which raises such a length to one
    * (tests/reference.py:108-109).                                                      */
-  DSV4_FLAG_ZERO_LENGTH_EMPTY = 8
+  DSV4_FLAG_ZERO_LENGTH_EMPTY = 8,
+  /* dsv4_shared_prefix_decode only (test hooks): the form of the call, which is otherwise
+   * chosen from its sizes.  LISTS: prefix and own tokens as two index lists; JOINED: as one
+   * list per query token; DENSE: the prefix converted once and attended by all rows together. */
+  DSV4_FLAG_SHARED_LISTS = 16,
+  DSV4_FLAG_SHARED_JOINED = 32,
+  DSV4_FLAG_SHARED_DENSE = 64
 };
 
 /* ---------------------------------------------------------------------------
@@ -279,15 +285,15 @@ int dsv4_sparse_prefill(const Dsv4PrefillArgs* args, void* cuda_stream);
  *
  * q rows are dense: stride_q_h = d_qk, [b, s_q, h_q] contiguous.  Scratch, sized by
  * dsv4_shared_prefix_scratch(args): o_accum fp32 [sets, b, s_q, h_q, 512], lse_accum fp32
- * [sets, b, s_q, h_q], workspace bytes.  num_blocks * page_block_size < 2^31; sm_scale is
- * positive and finite.                                                                      */
+ * [sets, b, s_q, h_q], workspace bytes.  num_blocks * page_block_size and
+ * (prefix_pages + max_pages) * page_block_size < 2^31; sm_scale is positive and finite.     */
 typedef struct Dsv4SharedPrefixArgs {
   int32_t b, s_q, h_q, d_qk, d_v;
   int32_t kv_format;            /* DSV4_KV_MODEL1 or DSV4_KV_V32                 */
   int32_t num_blocks, page_block_size;
   int32_t prefix_pages, max_pages;
   int32_t prefix_splits, suffix_splits;   /* 0: chosen by the library             */
-  int32_t flags;                /* DSV4_FLAG_IMPL_SIMPLE                          */
+  int32_t flags;                /* DSV4_FLAG_IMPL_SIMPLE, DSV4_FLAG_SHARED_*      */
   float sm_scale;
   const void* q;                /* BF16 [b, s_q, h_q, d_qk]                       */
   const void* kv;               /* bytes [num_blocks, stride_kv_block]            */

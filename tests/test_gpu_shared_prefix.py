@@ -15,6 +15,7 @@ from deepseek_v4_kernel import ops
 
 pytestmark = pytest.mark.gpu
 SCORES, U = 8e-4, 2.0 ** -8
+FORMS = [0, N.FLAG_SHARED_LISTS, N.FLAG_SHARED_JOINED, N.FLAG_SHARED_DENSE]      # as chosen, and each of the three
 LAYOUTS = {"V32": (512, 128, 4, 4), "MODEL1": (448, 64, 7, 8)}
 
 
@@ -107,30 +108,35 @@ class Batch:
 
 
 @pytest.mark.parametrize("layout", ["V32", "MODEL1"])
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("b,s_q,h_q", [(1, 1, 1), (4, 1, 16), (3, 2, 20), (5, 1, 64), (2, 3, 128), (17, 1, 8), (9, 1, 48)])
-def test_batches(layout, b, s_q, h_q):
+def test_batches(layout, b, s_q, h_q, form):
     suffix = [(37 * r) % 201 for r in range(b)]
     x = Batch(layout, b, s_q, h_q, 1000, suffix, 64, seed=b, sink=b % 2 == 0)
-    x.check(x.call())
+    x.check(x.call(flags=form))
 
 
 @pytest.mark.parametrize("prefix", [0, 1, 63, 64, 65, 127, 128, 129, 2049])
 @pytest.mark.parametrize("page", [16, 48, 64, 256])
-def test_prefix_lengths_and_pages(prefix, page):
+@pytest.mark.parametrize("form", FORMS[1:])
+def test_prefix_lengths_and_pages(prefix, page, form):
     x = Batch("V32", 6, 1, 32, prefix, [0, 1, 2, 127, 128, 300], page, seed=prefix)
-    x.check(x.call())
+    x.check(x.call(flags=form))
 
 
 @pytest.mark.parametrize("layout", ["V32", "MODEL1"])
-def test_rows_that_see_nothing(layout):
+@pytest.mark.parametrize("form", FORMS)
+def test_rows_that_see_nothing(layout, form):
     for sink in (False, True):
         x = Batch(layout, 3, 2, 16, 0, [0, 1, 5], 64, sink=sink)
-        x.check(x.call())
-        got = x.call()
+        got = x.call(flags=form)
+        x.check(got)
+        x.prefix_table = torch.zeros(3, dtype=torch.int32, device="cuda")      # a table, but no token of it
+        x.check(x.call(flags=form))
         assert (got[0][0] == 0).all() and (got[0][1, 0] == 0).all()
     x = Batch(layout, 3, 1, 16, 0, [0, 0, 0], 64, sink=True)
     x.table = x.table[:, :0]
-    got = x.call()
+    got = x.call(flags=form)
     assert (got[0] == 0).all() and torch.equal(got[1], x.sink.view(1, 16, 1).expand(3, 16, 1))
 
 
@@ -141,17 +147,41 @@ def test_splits(prefix_splits, suffix_splits):
     x.check(x.call(prefix_splits=prefix_splits, suffix_splits=suffix_splits))
 
 
-def test_many_rows():
+@pytest.mark.parametrize("form", FORMS)
+def test_many_rows(form):
     """More 64-row blocks than SMs, an odd number of them."""
     x = Batch("V32", 150, 1, 65, 700, [r % 4 for r in range(150)], 64)
-    x.check(x.call())
+    x.check(x.call(flags=form))
     x = Batch("MODEL1", 80, 2, 128, 300, [r % 7 for r in range(80)], 64)
-    x.check(x.call())
+    x.check(x.call(flags=form))
 
 
-def test_long_prefix():
-    x = Batch("V32", 12, 1, 64, 20000, [100 * r for r in range(12)], 64)
-    x.check(x.call())
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("layout", ["V32", "MODEL1"])
+def test_long_prefix(form, layout):
+    x = Batch(layout, 12, 1, 64, 20000, [100 * r for r in range(12)], 64)
+    x.check(x.call(flags=form))
+
+
+def test_references_are_raised_along_the_prefix():
+    """Scores that grow along the prefix: both softmax groups raise the references again and again."""
+    x = Batch("V32", 5, 1, 64, 4000, [30] * 5, 64, seed=4)
+    tok = torch.arange(4000, device="cuda")
+    where = x.prefix_table.long()[tok // 64] * 64 + tok % 64
+    g = torch.Generator(device="cuda").manual_seed(9)
+    base = torch.randn(1, 512, device="cuda", generator=g)
+    grow = (base * torch.linspace(0.0, 3.0, 4000, device="cuda")[:, None]).bfloat16()
+    ops.kv_store(grow, torch.randn(4000, 64, device="cuda", generator=g).bfloat16(), where, x.kv)
+    x.q[..., :512] = (base * torch.linspace(-1.0, 1.0, 5, device="cuda").view(5, 1, 1, 1)).bfloat16()
+    out, mag, lse = x.definition()
+    # 576 products and partial sums, each rounded to 2^-24 of at most sum |q k| = 512 * 3 / 24 * E[base^2]
+    slack = 2 * 577 * 2.0 ** -24 * 3 * float((base * base).sum()) / 24 + SCORES
+    for form in FORMS:
+        got = x.call(flags=form)
+        torch.cuda.synchronize()
+        assert K.device_status() == 0
+        assert ((got[0].double() - out).abs() <= U * (mag + out.abs()) + 2 * slack * mag).all()
+        assert ((got[1].double() - lse).abs() <= slack + 2e-6 * lse.abs()).all()
 
 
 def test_cross_check_kernels_agree():
@@ -175,23 +205,28 @@ def test_equal_to_one_list_per_request():
     x.check(want[:2])
 
 
-def test_padded_page_stride_and_pages_beyond_4_gib():
+@pytest.mark.parametrize("form", FORMS[1:])
+def test_padded_page_stride_and_pages_beyond_4_gib(form):
     x = Batch("V32", 3, 1, 16, 130, [5, 64, 100], 64, pad=48)
-    x.check(x.call())
+    x.check(x.call(flags=form))
     before = (1 << 32) // (64 * 644) + 9
     x = Batch("V32", 3, 1, 16, 130, [5, 64, 100], 64, blocks_before=before)
     assert int(x.prefix_table.min()) * 64 * 644 > 1 << 32
-    x.check(x.call())
+    x.check(x.call(flags=form))
 
 
-def test_pages_outside_the_cache_are_masked():
+@pytest.mark.parametrize("form", FORMS[1:])
+def test_pages_outside_the_cache_are_masked(form):
     x = Batch("V32", 3, 1, 16, 200, [70, 64, 130], 16)
     x.prefix_table[3], x.prefix_table[5], x.prefix_table[6] = -1, x.kv.size(0), 2 ** 31 - 1
     x.table[0, 1], x.table[2, 0], x.table[1, 3] = -5, 2 ** 30, x.kv.size(0) + 7
-    x.check(x.call())
+    x.check(x.call(flags=form))
+    x.prefix_table.fill_(-1)                         # no token of the prefix at all
+    x.check(x.call(flags=form))
 
 
-def test_lengths_that_lie_are_clamped():
+@pytest.mark.parametrize("form", FORMS[1:])
+def test_lengths_that_lie_are_clamped(form):
     x = Batch("V32", 4, 1, 16, 128, [64, 32, 16, 16], 16)
     x.table[:, 4] = x.table[:, 0]                    # the column behind the pages: filled rows again
     for r, s in enumerate([64, 32, 16, 16]):
@@ -199,16 +234,17 @@ def test_lengths_that_lie_are_clamped():
     for p, s in ((2 ** 31 - 1, [2 ** 31 - 1, 70, 80, 1000]), (-4, [-1, -2 ** 31, 0, 3])):
         x.prefix_length.fill_(p)
         x.suffix_length.copy_(torch.tensor(s, dtype=torch.int32))
-        x.check(x.call(), x.definition(p, s))
+        x.check(x.call(flags=form), x.definition(p, s))
 
 
-def test_captured_and_replayed_with_other_lengths():
+@pytest.mark.parametrize("form", FORMS[1:])
+def test_captured_and_replayed_with_other_lengths(form):
     x = Batch("V32", 6, 1, 64, 1000, [200, 100, 3, 0, 64, 65], 64)
-    x.call()
+    x.call(flags=form)
     torch.cuda.synchronize()
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
-        got = x.call()
+        got = x.call(flags=form)
     for p, s in ((1000, x.suffix), (0, [1, 100, 3, 0, 64, 65]), (777, [0] * 6), (1, [200, 1, 3, 0, 64, 2])):
         x.prefix_length.fill_(p)
         x.suffix_length.copy_(torch.tensor(s, dtype=torch.int32))
@@ -216,15 +252,16 @@ def test_captured_and_replayed_with_other_lengths():
         x.check(got, x.definition(p, s))
 
 
-def test_streams_at_once_and_repeatability():
+@pytest.mark.parametrize("form", FORMS[1:])
+def test_streams_at_once_and_repeatability(form):
     x = Batch("V32", 8, 1, 64, 3000, [100] * 8, 64)
-    first = x.call()
+    first = x.call(flags=form)
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(3)]
     results = []
     for i in range(9):
         with torch.cuda.stream(streams[i % 3]):
-            results.append(x.call())
+            results.append(x.call(flags=form))
     torch.cuda.synchronize()
     for r in results:
         assert all(torch.equal(a, b) for a, b in zip(r, first))

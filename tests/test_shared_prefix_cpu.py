@@ -32,7 +32,8 @@ def shared_args(**kw):
     (dict(s_q=0), 2), (dict(h_q=0), 2), (dict(d_v=256), 2), (dict(num_blocks=0), 2), (dict(page_block_size=0), 2),
     (dict(prefix_pages=-1), 2), (dict(max_pages=-1), 2), (dict(prefix_splits=-1), 2), (dict(suffix_splits=65), 2),
     (dict(num_blocks=1 << 26), 2), (dict(prefix_pages=1 << 26), 2), (dict(max_pages=1 << 26), 2),
-    (dict(b=1 << 20, s_q=1 << 12), 2), (dict(b=1 << 20), 2), (dict(stride_table=-1), 2), (dict(d_qk=512), 3),
+    (dict(b=1 << 20, s_q=1 << 12), 2), (dict(b=1 << 20), 2), (dict(stride_table=-1), 2), (dict(sm_scale=0.0), 2), (dict(sm_scale=-1.0), 2), (dict(sm_scale=float("nan")), 2),
+    (dict(sm_scale=float("inf")), 2), (dict(prefix_pages=(1 << 25) - 1, max_pages=9), 2), (dict(d_qk=512), 3),
     (dict(kv_format=N.KV_MODEL1), 3), (dict(kv_format=N.KV_BF16), 3), (dict(stride_kv_block=64 * 644 - 16), 3),
     (dict(stride_kv_block=64 * 644 + 8), 4), (dict(kv=8), 4), (dict(q=2), 4), (dict(out=8), 4), (dict(stride_o_h=516), 4)])
 def test_entry_refuses(kw, code):
