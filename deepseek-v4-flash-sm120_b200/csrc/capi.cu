@@ -52,6 +52,7 @@ int current_device_is_sm100() {
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 
 int check_paged(int kv_format, int d_qk, int page_block, int64_t stride_block, const void* kv) {
   int per_tok;
@@ -426,11 +427,11 @@ int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* a, void* stream) {
   const int sets = plan.prefix_sets + plan.suffix_splits;
   if (sets > 0 && (plan.form != FORM_JOINED || sets > 1)) {
     if (!a->o_accum || !a->lse_accum) return DSV4_ERR_SCRATCH;
-    if (!aligned16(a->o_accum)) return DSV4_ERR_ALIGN;
+    if (!aligned32(a->o_accum)) return DSV4_ERR_ALIGN;
   }
   if (plan.prefix_bytes + plan.suffix_bytes > 0) {
     if (!a->workspace) return DSV4_ERR_SCRATCH;
-    if (!aligned16(a->workspace)) return DSV4_ERR_ALIGN;
+    if (!aligned32(a->workspace)) return DSV4_ERR_ALIGN;
   }
   const int64_t rows = static_cast<int64_t>(a->b) * a->s_q * a->h_q;
   const int64_t plen = static_cast<int64_t>(a->prefix_pages) * a->page_block_size;
@@ -582,7 +583,7 @@ int dsv4_dense_prefill(const Dsv4DensePrefillArgs* a, void* stream) {
   }
   if (a->n_splits > 1) {
     if (!a->o_accum || !a->stat_accum) return DSV4_ERR_SCRATCH;
-    if (!aligned16(a->o_accum) || (reinterpret_cast<uintptr_t>(a->stat_accum) & 7u)) return DSV4_ERR_ALIGN;
+    if (!aligned32(a->o_accum) || (reinterpret_cast<uintptr_t>(a->stat_accum) & 7u)) return DSV4_ERR_ALIGN;
   }
   int rc = current_device_is_sm100();
   if (rc) return rc;

@@ -105,6 +105,7 @@ struct DenseParams {
   int chunks;                    // head chunks: h_q / pack
   int slots;                     // row-tile pairs, upper bound over all sequences
   int n_splits;
+  int sectors;                   // rows of the output start on 32 bytes
   float sm_scale;
   const int32_t *cu_q, *cu_k;
   const float* sink;
@@ -700,15 +701,25 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     }
     if (!live || fail) continue;
     if (RANGES) {
-      float4* d = reinterpret_cast<float4*>(p.o_accum + acc + 32 * k);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) d[q] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
+      for (int q = 0; q < 32; q += 8)
+        st_global_32(p.o_accum + acc + 32 * k + q, __float_as_uint(f[q]), __float_as_uint(f[q + 1]),
+                     __float_as_uint(f[q + 2]), __float_as_uint(f[q + 3]), __float_as_uint(f[q + 4]),
+                     __float_as_uint(f[q + 5]), __float_as_uint(f[q + 6]), __float_as_uint(f[q + 7]));
     } else {
-      uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + t * p.stride_o_t + h * p.stride_o_h + 32 * k);
+      uint16_t* d = static_cast<uint16_t*>(p.out) + t * p.stride_o_t + h * p.stride_o_h + 32 * k;
+      uint32_t o2[16];
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        d[q] = make_uint4(pack2<BF16>(f[8 * q], f[8 * q + 1]), pack2<BF16>(f[8 * q + 2], f[8 * q + 3]),
-                          pack2<BF16>(f[8 * q + 4], f[8 * q + 5]), pack2<BF16>(f[8 * q + 6], f[8 * q + 7]));
+      for (int q = 0; q < 16; ++q) o2[q] = pack2<BF16>(f[2 * q], f[2 * q + 1]);
+      if (p.sectors) {
+#pragma unroll
+        for (int q = 0; q < 16; q += 8)
+          st_global_32(d + 2 * q, o2[q], o2[q + 1], o2[q + 2], o2[q + 3], o2[q + 4], o2[q + 5], o2[q + 6], o2[q + 7]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 16; q += 4)
+          *reinterpret_cast<uint4*>(d + 2 * q) = make_uint4(o2[q], o2[q + 1], o2[q + 2], o2[q + 3]);
+      }
     }
   }
   tc_fence_before_sync();
@@ -873,6 +884,7 @@ cudaError_t launch_dense_prefill(const Dsv4DensePrefillArgs& a, cudaStream_t st)
   p.stride_o_t = a.stride_o_t; p.stride_o_h = a.stride_o_h;
   p.stride_ml_t = a.stride_ml_t; p.stride_lse_t = a.stride_lse_t;
   p.o_accum = a.o_accum; p.stat_accum = a.stat_accum;
+  p.sectors = ((reinterpret_cast<uintptr_t>(a.out) | (a.stride_o_t * 2) | (a.stride_o_h * 2)) & 31) == 0;
   cudaError_t e;
   if ((e = make_map_16bit(&p.mq, bf16, a.q, a.t_q, a.h_q, a.d_qk, a.stride_q_t, a.stride_q_h, p.tok_tile, p.pack))) return e;
   // a batch without any key still needs legal maps: nothing is loaded through them

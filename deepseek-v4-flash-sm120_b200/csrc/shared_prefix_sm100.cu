@@ -486,11 +486,11 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
           if (lane == 0) arrive_leader(bar(&ctrl.o_free));
         }
         if (row < p.rows && !fail) {
-          float4* d = reinterpret_cast<float4*>(dst + 32 * k);
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            d[q] = make_float4(__uint_as_float(o[4 * q]) * f, __uint_as_float(o[4 * q + 1]) * f,
-                               __uint_as_float(o[4 * q + 2]) * f, __uint_as_float(o[4 * q + 3]) * f);
+          for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
+#pragma unroll
+          for (int q = 0; q < 32; q += 8)
+            st_global_32(dst + 32 * k + q, o[q], o[q + 1], o[q + 2], o[q + 3], o[q + 4], o[q + 5], o[q + 6], o[q + 7]);
         }
       }
     }

@@ -285,7 +285,7 @@ int dsv4_sparse_prefill(const Dsv4PrefillArgs* args, void* cuda_stream);
  *
  * q rows are dense: stride_q_h = d_qk, [b, s_q, h_q] contiguous.  Scratch, sized by
  * dsv4_shared_prefix_scratch(args): o_accum fp32 [sets, b, s_q, h_q, 512], lse_accum fp32
- * [sets, b, s_q, h_q], workspace bytes.  num_blocks * page_block_size and
+ * [sets, b, s_q, h_q], workspace bytes (o_accum and workspace aligned to 32).  num_blocks * page_block_size and
  * (prefix_pages + max_pages) * page_block_size < 2^31; sm_scale is positive and finite.     */
 typedef struct Dsv4SharedPrefixArgs {
   int32_t b, s_q, h_q, d_qk, d_v;
@@ -339,7 +339,8 @@ int dsv4_shared_prefix_scratch(const Dsv4SharedPrefixArgs* args, int num_sms, in
  * in elements, multiples of 8, positive (k and v of several tokens or heads cannot be
  * broadcast views); pointers are 16-byte aligned; the last dimension is dense.  sm_scale is
  * positive and finite.  n_splits > 1 cuts every sequence's keys into that many ranges and
- * needs o_accum [2 n_splits, t_q, h_q, d_v] and stat_accum [2 n_splits, t_q, h_q, 2].       */
+ * needs o_accum [2 n_splits, t_q, h_q, d_v] (32-byte aligned) and stat_accum
+ * [2 n_splits, t_q, h_q, 2].                                                                */
 enum Dsv4Dtype { DSV4_DTYPE_BF16 = 0, DSV4_DTYPE_FP16 = 1 };
 typedef struct Dsv4DensePrefillArgs {
   int32_t b, t_q, t_k, h_q, h_kv, d_qk, d_v;
