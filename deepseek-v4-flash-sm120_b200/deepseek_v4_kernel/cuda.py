@@ -11,7 +11,6 @@ fallback path: without the native library this module cannot be imported.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
 from typing import Optional, Tuple
@@ -45,9 +44,15 @@ def _stream(index: int) -> int:
     return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
-def _current(index: int):
-    """Context that makes device `index` current; nothing when it is already."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
+def _queue(fn, args, index: int, what: str) -> None:
+    """Call a C entry on the current stream of device `index`, with that device current."""
+    if torch.cuda.current_device() == index:
+        rc = fn(C.byref(args), _stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(C.byref(args), _stream(index))
+    if rc:
+        N.check(rc, what)
 
 
 def _int32(name, t, index, dim, dense_rows=False) -> None:
@@ -305,33 +310,32 @@ def shared_prefix_decode_fwd(q, kv, prefix_table, prefix_length, block_table, su
     if attn_sink is not None and not (attn_sink.dtype == torch.float32 and attn_sink.numel() == h_q
                                       and attn_sink.is_contiguous() and attn_sink.get_device() == idx):
         raise RuntimeError("attn_sink must be contiguous float32 [h_q]")
-    with _current(idx):
-        out = q.new_empty((b, s_q, h_q, 512))
-        lse = q.new_empty((b, h_q, s_q), dtype=torch.float32)
-        if b == 0:
-            return out, lse
-        a = N.SharedPrefixArgs()
-        a.b, a.s_q, a.h_q, a.d_qk, a.d_v, a.kv_format = b, s_q, h_q, d_qk, 512, fmt
-        a.num_blocks, a.page_block_size = num_blocks, page_block
-        a.prefix_pages, a.max_pages = prefix_table.numel(), block_table.size(1)
-        a.prefix_splits, a.suffix_splits, a.flags, a.sm_scale = prefix_splits, suffix_splits, flags, float(sm_scale)
-        sets, nbytes = C.c_int32(0), C.c_int64(0)
-        N.check(N.lib.dsv4_shared_prefix_scratch(C.byref(a), num_sms(q.device), C.byref(sets), C.byref(nbytes)),
-                "dsv4_shared_prefix_scratch")
-        # one allocation: partial outputs, their log-sum-exps, workspace
-        rows = sets.value * b * s_q * h_q
-        lse_at, work_at = rows * 2048, rows * 2048 + (rows * 4 + 255) // 256 * 256
-        scratch = q.new_empty((work_at + nbytes.value,), dtype=torch.uint8)
-        at = scratch.data_ptr()
-        a.o_accum, a.lse_accum, a.workspace = at, at + lse_at, at + work_at
-        a.q, a.kv, a.attn_sink = q.data_ptr(), kv.data_ptr(), _ptr(attn_sink)
-        a.prefix_table, a.prefix_length = prefix_table.data_ptr(), prefix_length.data_ptr()
-        a.block_table, a.suffix_length = block_table.data_ptr(), suffix_length.data_ptr()
-        a.out, a.lse = out.data_ptr(), lse.data_ptr()
-        a.stride_kv_block, a.stride_table = kv_strides[0], block_table.stride(0)
-        a.stride_o_b, a.stride_o_s, a.stride_o_h = s_q * h_q * 512, h_q * 512, 512
-        a.stride_lse_b, a.stride_lse_h, a.stride_lse_s = h_q * s_q, s_q, 1
-        N.check(N.lib.dsv4_shared_prefix_decode(C.byref(a), _stream(idx)), "dsv4_shared_prefix_decode")
+    out = q.new_empty((b, s_q, h_q, 512))
+    lse = q.new_empty((b, h_q, s_q), dtype=torch.float32)
+    if b == 0:
+        return out, lse
+    a = N.SharedPrefixArgs()
+    a.b, a.s_q, a.h_q, a.d_qk, a.d_v, a.kv_format = b, s_q, h_q, d_qk, 512, fmt
+    a.num_blocks, a.page_block_size = num_blocks, page_block
+    a.prefix_pages, a.max_pages = prefix_table.numel(), block_table.size(1)
+    a.prefix_splits, a.suffix_splits, a.flags, a.sm_scale = prefix_splits, suffix_splits, flags, float(sm_scale)
+    sets, nbytes = C.c_int32(0), C.c_int64(0)
+    N.check(N.lib.dsv4_shared_prefix_scratch(C.byref(a), num_sms(q.device), C.byref(sets), C.byref(nbytes)),
+            "dsv4_shared_prefix_scratch")
+    # one allocation: partial outputs, their log-sum-exps, workspace
+    rows = sets.value * b * s_q * h_q
+    lse_at, work_at = rows * 2048, rows * 2048 + (rows * 4 + 255) // 256 * 256
+    scratch = q.new_empty((work_at + nbytes.value,), dtype=torch.uint8)
+    at = scratch.data_ptr()
+    a.o_accum, a.lse_accum, a.workspace = at, at + lse_at, at + work_at
+    a.q, a.kv, a.attn_sink = q.data_ptr(), kv.data_ptr(), _ptr(attn_sink)
+    a.prefix_table, a.prefix_length = prefix_table.data_ptr(), prefix_length.data_ptr()
+    a.block_table, a.suffix_length = block_table.data_ptr(), suffix_length.data_ptr()
+    a.out, a.lse = out.data_ptr(), lse.data_ptr()
+    a.stride_kv_block, a.stride_table = kv_strides[0], block_table.stride(0)
+    a.stride_o_b, a.stride_o_s, a.stride_o_h = s_q * h_q * 512, h_q * 512, 512
+    a.stride_lse_b, a.stride_lse_h, a.stride_lse_s = h_q * s_q, s_q, 1
+    _queue(N.lib.dsv4_shared_prefix_decode, a, idx, "dsv4_shared_prefix_decode")
     return out, lse
 
 
@@ -381,28 +385,27 @@ def dense_prefill_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, sm_scale, causal: boo
     if out is not None and not (out.dtype == dtype and out.shape == (t_q, h_q, d_v) and out.get_device() == idx
                                 and out.stride(2) == 1):
         raise RuntimeError("out must be [t_q, h_q, d_v] of q's type, dense in the last dim")
-    with _current(idx):
-        if out is None:
-            out = q.new_empty((t_q, h_q, d_v))
-        stats = q.new_empty((2, t_q, h_q), dtype=torch.float32)
-        a = N.DensePrefillArgs()
-        if n_splits is None:
-            n_splits = N.lib.dsv4_plan_dense_splits(t_q, t_k, b, h_q, h_kv, num_sms(q.device))
-        a.b, a.t_q, a.t_k, a.h_q, a.h_kv, a.d_qk, a.d_v = b, t_q, t_k, h_q, h_kv, d_qk, d_v
-        a.dtype, a.causal, a.n_splits, a.sm_scale = _DENSE_DTYPES[dtype], int(bool(causal)), n_splits, float(sm_scale)
-        a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-        a.cu_seqlens_q, a.cu_seqlens_k = cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr()
-        at = stats.data_ptr()
-        a.attn_sink, a.max_logits, a.lse = _ptr(attn_sink), at, at + 4 * t_q * h_q
-        if n_splits > 1:
-            rows = 2 * n_splits * t_q * h_q          # two partial sets a range
-            scratch = q.new_empty((rows * (d_v + 2),), dtype=torch.float32)
-            a.o_accum, a.stat_accum = scratch.data_ptr(), scratch.data_ptr() + rows * d_v * 4
-        a.stride_q_t, a.stride_q_h, a.stride_k_t, a.stride_k_h = sq[0], sq[1], sk[0], sk[1]
-        a.stride_v_t, a.stride_v_h = sv[0], sv[1]
-        a.stride_o_t, a.stride_o_h, _ = out.stride()
-        a.stride_ml_t = a.stride_lse_t = h_q
-        N.check(N.lib.dsv4_dense_prefill(C.byref(a), _stream(idx)), "dsv4_dense_prefill")
+    if out is None:
+        out = q.new_empty((t_q, h_q, d_v))
+    stats = q.new_empty((2, t_q, h_q), dtype=torch.float32)
+    a = N.DensePrefillArgs()
+    if n_splits is None:
+        n_splits = N.lib.dsv4_plan_dense_splits(t_q, t_k, b, h_q, h_kv, num_sms(q.device))
+    a.b, a.t_q, a.t_k, a.h_q, a.h_kv, a.d_qk, a.d_v = b, t_q, t_k, h_q, h_kv, d_qk, d_v
+    a.dtype, a.causal, a.n_splits, a.sm_scale = _DENSE_DTYPES[dtype], int(bool(causal)), n_splits, float(sm_scale)
+    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    a.cu_seqlens_q, a.cu_seqlens_k = cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr()
+    at = stats.data_ptr()
+    a.attn_sink, a.max_logits, a.lse = _ptr(attn_sink), at, at + 4 * t_q * h_q
+    if n_splits > 1:
+        rows = 2 * n_splits * t_q * h_q          # two partial sets a range
+        scratch = q.new_empty((rows * (d_v + 2),), dtype=torch.float32)
+        a.o_accum, a.stat_accum = scratch.data_ptr(), scratch.data_ptr() + rows * d_v * 4
+    a.stride_q_t, a.stride_q_h, a.stride_k_t, a.stride_k_h = sq[0], sq[1], sk[0], sk[1]
+    a.stride_v_t, a.stride_v_h = sv[0], sv[1]
+    a.stride_o_t, a.stride_o_h, _ = out.stride()
+    a.stride_ml_t = a.stride_lse_t = h_q
+    _queue(N.lib.dsv4_dense_prefill, a, idx, "dsv4_dense_prefill")
     max_logits, lse = stats.unbind(0)
     return out, max_logits, lse
 
@@ -486,19 +489,18 @@ def build_slot_maps(block_table, cached_lens, new_lens, free_pages, page_block: 
         raise RuntimeError("page_block >= 1 and n_slots >= 0 expected")
     if b > 16384:
         raise RuntimeError("at most 16384 requests")
-    with _current(idx):
-        slots = cached_lens.new_empty((n_slots,), dtype=torch.int64)
-        ints = cached_lens.new_empty((n_slots + 2 * b + 3,))
-        a = N.SlotMapArgs()
-        a.b, a.max_pages, a.page_block_size, a.n_slots = b, max_pages, page_block, n_slots
-        a.n_free = free_pages.numel()
-        a.block_table, a.stride_table = block_table.data_ptr(), block_table.stride(0) if b > 1 else max_pages
-        a.cached_lens, a.new_lens, a.free_pages = cached_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr()
-        a.slots, at = slots.data_ptr(), ints.data_ptr()
-        a.positions, a.cu_new, a.cu_total = at, at + 4 * n_slots, at + 4 * (n_slots + b + 1)
-        a.n_taken = at + 4 * (n_slots + 2 * b + 2)
-        N.check(N.lib.dsv4_build_slot_maps(C.byref(a), _stream(idx)), "dsv4_build_slot_maps")
-    return (slots,) + torch.split_with_sizes(ints, (n_slots, b + 1, b + 1, 1))
+    slots = cached_lens.new_empty((n_slots,), dtype=torch.int64)
+    ints = cached_lens.new_empty((n_slots + 2 * b + 3,))
+    a = N.SlotMapArgs()
+    a.b, a.max_pages, a.page_block_size, a.n_slots = b, max_pages, page_block, n_slots
+    a.n_free = free_pages.numel()
+    a.block_table, a.stride_table = block_table.data_ptr(), block_table.stride(0) if b > 1 else max_pages
+    a.cached_lens, a.new_lens, a.free_pages = cached_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr()
+    a.slots, at = slots.data_ptr(), ints.data_ptr()
+    a.positions, a.cu_new, a.cu_total = at, at + 4 * n_slots, at + 4 * (n_slots + b + 1)
+    a.n_taken = at + 4 * (n_slots + 2 * b + 2)
+    _queue(N.lib.dsv4_build_slot_maps, a, idx, "dsv4_build_slot_maps")
+    return (slots,) + torch.unsafe_split_with_sizes(ints, (n_slots, b + 1, b + 1, 1))
 
 
 def page_indices(block_table, positions, page_block: int, cu_seqlens=None) -> torch.Tensor:
@@ -533,18 +535,17 @@ def page_indices(block_table, positions, page_block: int, cu_seqlens=None) -> to
         _int32("cu_seqlens", cu_seqlens, idx, 1)
         if cu_seqlens.numel() != b + 1:
             raise RuntimeError(f"cu_seqlens must have {b + 1} entries")
-    with _current(idx):
-        out = positions.new_empty(positions.shape)
-        a = N.PageIndicesArgs()
-        a.n_rows, a.topk, a.b, a.s_q = n_rows, topk, b, max(s_q, 1)
-        a.max_pages, a.page_block_size = max_pages, page_block
-        a.block_table, a.positions, a.indices = block_table.data_ptr(), flat.data_ptr(), out.data_ptr()
-        a.cu_seqlens = _ptr(cu_seqlens)
-        a.stride_table = block_table.stride(0)
-        a.stride_positions = topk if n_rows <= 1 else flat.stride(-2)
-        if s_q > 1 and flat is not positions:
-            a.stride_positions = flat.stride(0)
-        N.check(N.lib.dsv4_page_indices(C.byref(a), _stream(idx)), "dsv4_page_indices")
+    out = positions.new_empty(positions.shape)
+    a = N.PageIndicesArgs()
+    a.n_rows, a.topk, a.b, a.s_q = n_rows, topk, b, max(s_q, 1)
+    a.max_pages, a.page_block_size = max_pages, page_block
+    a.block_table, a.positions, a.indices = block_table.data_ptr(), flat.data_ptr(), out.data_ptr()
+    a.cu_seqlens = _ptr(cu_seqlens)
+    a.stride_table = block_table.stride(0)
+    a.stride_positions = topk if n_rows <= 1 else flat.stride(-2)
+    if s_q > 1 and flat is not positions:
+        a.stride_positions = flat.stride(0)
+    _queue(N.lib.dsv4_page_indices, a, idx, "dsv4_page_indices")
     return out
 
 
