@@ -380,7 +380,7 @@ static SharedPlan plan_shared(const Dsv4SharedPrefixArgs* a, int num_sms) {
 static int check_shared(const Dsv4SharedPrefixArgs* a) {
   if (!a) return DSV4_ERR_NULL;
   if (a->b < 0 || a->s_q < 1 || a->h_q < 1 || a->num_blocks < 1 || a->page_block_size < 1 || a->d_v != dsv4::D_V ||
-      !(a->sm_scale > 0.0f) || !(a->sm_scale <= 3.0e38f) || a->prefix_pages < 0 || a->max_pages < 0 || a->prefix_splits < 0 || a->suffix_splits < 0 ||
+      !(a->sm_scale > 0.0f) || !(a->sm_scale <= 1.0e38f) || a->prefix_pages < 0 || a->max_pages < 0 || a->prefix_splits < 0 || a->suffix_splits < 0 ||
       a->prefix_splits > 64 || a->suffix_splits > 64)
     return DSV4_ERR_SHAPE;
   const int64_t most = 0x7fffffff;
@@ -560,7 +560,7 @@ int dsv4_dense_prefill(const Dsv4DensePrefillArgs* a, void* stream) {
   if (!a) return DSV4_ERR_NULL;
   if (a->b < 0 || a->t_q < 0 || a->t_k < 0 || a->h_q < 1 || a->h_kv < 1 || a->h_q % a->h_kv ||
       a->n_splits < 1 || a->n_splits > dsv4::DENSE_MAX_SPLITS || !(a->sm_scale > 0.0f) ||
-      !(a->sm_scale <= 3.0e38f) || dsv4::dense_ctas(a->t_q, a->b, a->h_q, a->h_kv) > 0x7fffffff)
+      !(a->sm_scale <= 1.0e38f) || dsv4::dense_ctas(a->t_q, a->b, a->h_q, a->h_kv) > 0x7fffffff)
     return DSV4_ERR_SHAPE;
   if (!((a->d_qk == 64 && a->d_v == 64) || (a->d_qk == 128 && a->d_v == 128) ||
         (a->d_qk == 192 && a->d_v == 128)))

@@ -325,8 +325,15 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   const int split = blockIdx.z;
   const Work w = find_work<RANGES>(p, slot, split);
   const bool twin = RANGES && w.twin;
+  auto give_back = [&]() {                // TMEM of a CTA that leaves before the others have seen it
+    if (warp != WARP_LOOK) return;
+    tc_fence_before_sync();
+    __syncwarp();
+    tc_fence_after_sync();
+    tmem_dealloc(*reinterpret_cast<volatile uint32_t*>(&ctrl.tmem), TMEM_COLS);
+  };
   if (!w.any) {
-    if (warp == WARP_LOOK) tmem_dealloc(ctrl.tmem, TMEM_COLS);
+    give_back();
     return;
   }
   const int head0 = chunk * p.pack;
@@ -349,7 +356,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
         for (int c = 0; c < DV / 8; ++c) d[c] = make_uint4(0, 0, 0, 0);
       }
     }
-    if (warp == WARP_LOOK) tmem_dealloc(ctrl.tmem, TMEM_COLS);
+    give_back();
     return;
   }
 

@@ -523,7 +523,7 @@ def page_indices(block_table, positions, page_block: int, cu_seqlens=None) -> to
     if not 1 <= page_block < 2 ** 31:
         raise RuntimeError("page_block >= 1 expected")
     topk = positions.size(-1)
-    flat, s_q, n_rows = positions, 1, positions.size(0)
+    flat, s_q, n_rows, stride = positions, 1, positions.size(0), topk
     if cu_seqlens is None:
         if n_rows != b:
             raise RuntimeError(f"positions must be [{b}, s_q, topk]")
@@ -531,10 +531,13 @@ def page_indices(block_table, positions, page_block: int, cu_seqlens=None) -> to
         n_rows = b * s_q
         if not positions.is_contiguous():
             flat = positions.reshape(n_rows, topk)       # a view when the rows have one stride
+            stride = flat.stride(0)
     else:
         _int32("cu_seqlens", cu_seqlens, idx, 1)
         if cu_seqlens.numel() != b + 1:
             raise RuntimeError(f"cu_seqlens must have {b + 1} entries")
+        if n_rows > 1:
+            stride = positions.stride(0)
     out = positions.new_empty(positions.shape)
     a = N.PageIndicesArgs()
     a.n_rows, a.topk, a.b, a.s_q = n_rows, topk, b, max(s_q, 1)
@@ -542,9 +545,7 @@ def page_indices(block_table, positions, page_block: int, cu_seqlens=None) -> to
     a.block_table, a.positions, a.indices = block_table.data_ptr(), flat.data_ptr(), out.data_ptr()
     a.cu_seqlens = _ptr(cu_seqlens)
     a.stride_table = block_table.stride(0)
-    a.stride_positions = topk if n_rows <= 1 else flat.stride(-2)
-    if s_q > 1 and flat is not positions:
-        a.stride_positions = flat.stride(0)
+    a.stride_positions = stride
     _queue(N.lib.dsv4_page_indices, a, idx, "dsv4_page_indices")
     return out
 

@@ -286,7 +286,7 @@ int dsv4_sparse_prefill(const Dsv4PrefillArgs* args, void* cuda_stream);
  * q rows are dense: stride_q_h = d_qk, [b, s_q, h_q] contiguous.  Scratch, sized by
  * dsv4_shared_prefix_scratch(args): o_accum fp32 [sets, b, s_q, h_q, 512], lse_accum fp32
  * [sets, b, s_q, h_q], workspace bytes (o_accum and workspace aligned to 32).  num_blocks * page_block_size and
- * (prefix_pages + max_pages) * page_block_size < 2^31; sm_scale is positive and finite.     */
+ * (prefix_pages + max_pages) * page_block_size < 2^31; sm_scale is in (0, 1e38].            */
 typedef struct Dsv4SharedPrefixArgs {
   int32_t b, s_q, h_q, d_qk, d_v;
   int32_t kv_format;            /* DSV4_KV_MODEL1 or DSV4_KV_V32                 */
@@ -338,7 +338,7 @@ int dsv4_shared_prefix_scratch(const Dsv4SharedPrefixArgs* args, int num_sms, in
  * (d_qk, d_v) is (64, 64), (128, 128) or (192, 128); q, k, v, out of one type.  Strides are
  * in elements, multiples of 8, positive (k and v of several tokens or heads cannot be
  * broadcast views); pointers are 16-byte aligned; the last dimension is dense.  sm_scale is
- * positive and finite.  n_splits > 1 cuts every sequence's keys into that many ranges and
+ * positive and at most 1e38.  n_splits > 1 cuts every sequence's keys into that many ranges and
  * needs o_accum [2 n_splits, t_q, h_q, d_v] (32-byte aligned) and stat_accum
  * [2 n_splits, t_q, h_q, 2].                                                                */
 enum Dsv4Dtype { DSV4_DTYPE_BF16 = 0, DSV4_DTYPE_FP16 = 1 };

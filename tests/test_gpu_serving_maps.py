@@ -156,6 +156,24 @@ def test_page_indices_packed(cu):
     assert ops.page_indices(table.cuda(), wide[:, 5:41], 16, ints(cu)).tolist() == want
 
 
+def test_page_indices_of_views():
+    gen = torch.Generator().manual_seed(3)
+    table, pos = torch.randint(0, 99, (4, 20), generator=gen).int(), torch.randint(-1, 330, (4, 3, 40), generator=gen).int()
+    want = torch.tensor(plain_indices(table, pos.view(12, 40), [r for r in range(4) for _ in range(3)], 16)).view(4, 3, 40)
+    dev = pos.cuda()
+    for s in range(3):                               # one query token of several, and the same with an odd stride of size 1
+        assert ops.page_indices(table.cuda(), dev[:, s:s + 1], 16).tolist() == want[:, s:s + 1].tolist()
+        one = dev[:, s].contiguous().as_strided((4, 1, 40), (40, 7, 1))
+        assert ops.page_indices(table.cuda(), one, 16).tolist() == want[:, s:s + 1].tolist()
+    assert ops.page_indices(table.cuda(), dev[:, :, 4:36], 16).tolist() == want[:, :, 4:36].tolist()
+    assert ops.page_indices(table.cuda(), dev.transpose(0, 1).contiguous().transpose(0, 1), 16).tolist() == want.tolist()
+    assert ops.page_indices(table.cuda(), dev[:1].expand(4, 3, 40), 16).tolist() == \
+        torch.tensor(plain_indices(table, pos[:1].expand(4, 3, 40).reshape(12, 40), [r for r in range(4) for _ in range(3)], 16)).view(4, 3, 40).tolist()
+    wide = torch.full((4, 30), -5, dtype=torch.int32, device="cuda")
+    wide[:, 3:23] = table.cuda()
+    assert ops.page_indices(wide[:, 3:23], dev, 16).tolist() == want.tolist()
+
+
 def test_page_indices_that_do_not_fit():
     table = ints([[I32_MAX, I32_MAX // 64, 33554431, 33554432]])
     pos = ints([[[0, 64, 127, 128, 191, 192, 193, 255, 256, I32_MAX]]])
