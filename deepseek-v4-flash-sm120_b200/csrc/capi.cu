@@ -324,11 +324,13 @@ int dsv4_sparse_prefill(const Dsv4PrefillArgs* a, void* stream) {
 // How a shared-prefix decode is done, and its scratch.
 //   JOINED  one list per query token, of the prefix and its own tokens, for the sparse kernel:
 //           reads the prefix once per request, but is two or three short launches;
-//   DENSE   the prefix by launch_prefix_attn, the own tokens by the sparse kernel, joined;
+//   DENSE   the prefix by launch_prefix_attn, with the own tokens where their table is not too
+//           wide, else those by the sparse kernel, joined;
 //   LISTS   the same with the prefix by the sparse kernel too, as one list for all rows.
 enum SharedForm { FORM_JOINED, FORM_DENSE, FORM_LISTS };
 struct SharedPlan {
   SharedForm form;
+  bool own;                                // DENSE: the own tokens in the same pass
   int prefix_sets, suffix_splits;          // partial sets of the two parts (JOINED: splits in the second)
   int64_t prefix_bytes, suffix_bytes;      // of the workspace: the prefix's part, then the lists
 };
@@ -336,7 +338,7 @@ static SharedForm choose_form(const Dsv4SharedPrefixArgs* a, int64_t rows, int64
   const bool by_list = a->prefix_splits > 0 || a->suffix_splits > 0 || want_simple(a->flags);
   if (by_list || plen + slen == 0 || (a->flags & DSV4_FLAG_SHARED_LISTS)) return FORM_LISTS;
   if (plen == 0 || (a->flags & DSV4_FLAG_SHARED_JOINED)) return FORM_JOINED;
-  if (a->flags & DSV4_FLAG_SHARED_DENSE) return FORM_DENSE;
+  if ((a->flags & DSV4_FLAG_SHARED_DENSE) && dsv4::prefix_attn_fits(*a, false)) return FORM_DENSE;
   // JOINED up to four tiles of 128 tokens an SM (for blocks of up to 64 rows) and lists of 16384
   // tokens (microseconds, JOINED / DENSE / LISTS, tokens a request x requests x heads: 2100 x 4 x
   // 16: 18 / 35 / 33; 2100 x 16 x 64: 27 / 40 / 41; 4100 x 16 x 64, 528 tiles: 37 / 43 / 49;
@@ -346,7 +348,7 @@ static SharedForm choose_form(const Dsv4SharedPrefixArgs* a, int64_t rows, int64
   // LISTS up to 128 rows: converting the whole prefix costs more than reading its FP8 rows twice
   // (30100 x 4 x 16, 64 rows: 49 DENSE, 41 LISTS; 10100 x 4 x 32: 41 and 39; 4100 x 8 x 64, 512
   // rows: 39 and 41; 33000 x 64 x 64: 269 and 667).
-  return rows > 128 ? FORM_DENSE : FORM_LISTS;
+  return rows > 128 && dsv4::prefix_attn_fits(*a, false) ? FORM_DENSE : FORM_LISTS;
 }
 
 static SharedPlan plan_shared(const Dsv4SharedPrefixArgs* a, int num_sms) {
@@ -363,8 +365,17 @@ static SharedPlan plan_shared(const Dsv4SharedPrefixArgs* a, int num_sms) {
     return p;
   }
   if (p.form == FORM_DENSE) {
+    // In the same pass the own tokens are converted to BF16 rows like the prefix's, which pays while
+    // those rows stay in L2, up to 131072 tokens that the table can hold; and a tile of them is of use
+    // to its request's rows alone, of which a block of 128 rows wants 16 (microseconds, same pass /
+    // own launch; requests x heads, prefix, own: 64 x 64, 32768, 64 to 2048: 219 / 244; 64 x 64, 2048,
+    // 64 to 2048: 61 / 91; 16 x 128, 8192, 4096 to 8192: 101 / 135; 64 x 16, 8192, 64 to 512: 53 /
+    // 58.  Beyond: 64 x 16, 32768, 1024 to 2048: 130 / 121; 64 x 64, 8192, 2048 to 4096: 168 / 162;
+    // 256 x 64, 1024, 1100: 217 / 184; 128 x 8, 32768, 64 to 512: 108 / 102).
+    p.own = slen > 0 && a->b * ((slen + 127) / 128 * 128) <= 131072 && a->s_q * a->h_q >= 16 && dsv4::prefix_attn_fits(*a, true);
     p.prefix_sets = dsv4::prefix_attn_sets(rows, num_sms);
-    p.prefix_bytes = dsv4::prefix_attn_workspace(plen, a->d_qk);
+    p.prefix_bytes = dsv4::prefix_attn_workspace(*a, p.own);
+    if (p.own) return p;
   } else if (plen > 0) {
     p.prefix_sets = a->prefix_splits > 0 ? a->prefix_splits
                                          : dsv4_plan_splits(1, 1, static_cast<int>(rows), static_cast<int>(plen), 0, num_sms);
@@ -439,12 +450,12 @@ int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* a, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int32_t* lists = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(a->workspace) + plan.prefix_bytes);
   dsv4::SharedSetup setup{};
-  if (plan.form == FORM_DENSE) dsv4::prefix_attn_place(plen, a->workspace, setup);
+  if (plan.form == FORM_DENSE) dsv4::prefix_attn_place(*a, plan.own, setup);
   if (plan.form == FORM_LISTS && plen > 0) setup.prefix_list = static_cast<int32_t*>(a->workspace);
   if (plan.form == FORM_JOINED) {
     setup.joined = lists;
     setup.lens = lists + static_cast<int64_t>(a->b) * a->s_q * (plen + slen);
-  } else if (slen > 0) {
+  } else if (slen > 0 && !plan.own) {
     setup.suffix_lists = lists;
   }
   if ((e = dsv4::launch_shared_setup(*a, setup, st))) return cuda_fail(e);

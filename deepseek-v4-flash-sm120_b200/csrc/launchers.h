@@ -43,14 +43,19 @@ cudaError_t launch_slot_maps(const Dsv4SlotMapArgs& a, cudaStream_t st);
 cudaError_t launch_page_indices(const Dsv4PageIndicesArgs& a, cudaStream_t st);
 
 // Set-up of a shared-prefix decode (shared_prefix_sm100.cu), one launch: what is not null of
-//   rows, valid    the prefix as BF16 rows, and a bit per token (prefix_attn_place says where),
+//   rows, valid    the prefix as BF16 rows and, when own_padded is not 0, each request's own
+//                  tokens (`padded` rows, then own_padded for each), and a bit per row: it exists,
+//   unfit          a bit per row of own tokens: its latent part is not finite, and zeros stand there,
+//   starts         where the tiles of the row blocks start (prefix_attn_place sets these six),
 //   prefix_list    token indices of the prefix,
 //   suffix_lists   of every query token's own tokens, a list of max_pages * page entries each,
 //   joined, lens   both one after the other, prefix_pages * page entries more each, and the
 //                  requests' list lengths.
 struct SharedSetup {
   void* rows;
-  uint32_t* valid;
+  uint32_t *valid, *unfit;
+  int32_t* starts;
+  int padded, own_padded;
   int32_t *prefix_list, *suffix_lists, *joined, *lens;
 };
 cudaError_t launch_shared_setup(const Dsv4SharedPrefixArgs& a, const SharedSetup& out, cudaStream_t st);
@@ -60,8 +65,10 @@ cudaError_t launch_join_sets(const Dsv4CombineArgs& a, cudaStream_t st);
 // Attention of many rows over a shared prefix, into the first prefix_attn_sets partial sets
 // (shared_prefix_sm100.cu).
 int prefix_attn_sets(int64_t rows, int num_sms);
-int64_t prefix_attn_workspace(int64_t tokens, int d_qk);       // bytes
-void prefix_attn_place(int64_t tokens, void* workspace, SharedSetup& out);
+// `own`: with the requests' own tokens.  Do the sizes fit, and how many bytes of workspace?
+bool prefix_attn_fits(const Dsv4SharedPrefixArgs& a, bool own);
+int64_t prefix_attn_workspace(const Dsv4SharedPrefixArgs& a, bool own);
+void prefix_attn_place(const Dsv4SharedPrefixArgs& a, bool own, SharedSetup& out);
 cudaError_t launch_prefix_attn(const Dsv4SharedPrefixArgs& a, const SharedSetup& rows, int num_sms, cudaStream_t st);
 cudaError_t read_prefix_error(int* value, bool reset);
 

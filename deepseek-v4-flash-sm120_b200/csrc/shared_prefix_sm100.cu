@@ -23,10 +23,20 @@
 // Q K^T of tile t + 1 and P V of tile t - 1 while the exponentials of tile t are formed.  K is
 // recycled in groups of blocks as Q K^T passes them, V in halves of its columns.
 //
-// Work is cut evenly: row blocks x tiles form one line that is divided among the clusters; a
-// cluster's share is one or more segments (a range of tiles of one row block), each leaving a
-// normalised 32-bit partial and its log-sum-exp.  The segments of a row block are its sets
-// 0, 1, ...; the last one marks the sets that are not used with -inf.
+// The requests' own tokens can be attended in the same pass: the tiles of every request with rows
+// in a block follow the prefix's, seen by that request's rows only.  That wastes most of such a
+// tile's products, but saves a launch that is as long as its longest request (64 requests of 64
+// to 2048 own tokens: 45 us; here 6 % more tiles, and 11 us more of conversion).
+//
+// Work is cut evenly: the tiles of all row blocks form one line that is divided among the
+// clusters; a cluster's share is one or more segments (a range of tiles of one row block), each
+// leaving a normalised 32-bit partial and its log-sum-exp.  The segments of a row block are its
+// sets 0, 1, ...; the last one marks the sets that are not used with -inf.
+//
+// Measured (64 requests x 64 heads, a prefix of 32768 of d_qk 576, 64 to 2048 own tokens): 194 us,
+// 1.5 PFLOP/s for the prefix alone, tensor pipe 86 % busy at an SM clock of 1.55 GHz that the power
+// limit sets.  Bound by the tensor cores at that clock; around it conversion 25 us (6.9 TB/s with
+// rows that stay in L2) and the join 12 us (2 KB a row and set read, 1 KB a row written).
 #include <mutex>
 
 #include "attn_params.cuh"
@@ -84,9 +94,13 @@ static_assert(prefix_smem_bytes<576>() <= 232448, "227 KB a CTA");
 
 struct PrefixParams {
   CUtensorMap mq, mk, mv;        // query rows; token rows in boxes of 64 and of 128
-  int rows, sets, max_tokens;
-  const int32_t* length;         // [1]
-  const uint32_t* valid;         // one bit a token
+  int rows, sets, blocks;        // query rows, partial sets, blocks of 128 rows
+  int max_tokens, padded;        // of the prefix: tokens, and rows of the workspace
+  int own_max, own_padded;       // of each request's own tokens; 0: attended elsewhere
+  int b, s_q, h_q;
+  const int32_t *length, *own;   // [1], [b]
+  const int32_t* starts;         // [blocks + 2]: where a block's tiles start; the most of a block
+  const uint32_t *valid, *unfit; // one bit a row of the workspace: it exists; it is not finite
   float sm_scale;
   float *o_accum, *lse_accum;    // [sets][rows][512], [sets][rows]
 };
@@ -148,32 +162,67 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&t);
 }
 
-// This cluster's share of the line of row blocks x tiles, segment by segment.
+// How many own tokens request r has.
+__device__ __forceinline__ int own_tokens(const PrefixParams& p, int r) { return min(max(__ldg(p.own + r), 0), p.own_max); }
+
+// This cluster's share of the line of tiles, segment by segment.  Used by whole warps.
 struct Share {
-  int tiles;                     // of a row block
-  int64_t per, at, end;          // tiles of a cluster; where it is, where it ends
-  int block, first, count, set;  // the current segment
+  int blocks, prefix_tiles;
+  int per, at, end;              // tiles of a cluster; where it is, where it ends
+  int block, first, count, set;  // the current segment: tiles [first, first + count) of a block,
+  int shared;                    // of which the first `shared` are the prefix's
   bool last;                     // it ends its row block
   __device__ __forceinline__ Share(const PrefixParams& p, int cluster, int clusters) {
-    const int len = min(max(*p.length, 0), p.max_tokens);
-    tiles = (len + TILE - 1) / TILE;
-    const int64_t line = static_cast<int64_t>(tiles) * ((p.rows + 2 * ROWS - 1) / (2 * ROWS));
-    per = max((line + clusters - 1) / clusters, static_cast<int64_t>(MIN_TILES));
-    at = min(cluster * per, line);
-    end = min(at + per, line);
+    const int len = __ldg(p.length), line = __ldg(p.starts + p.blocks), most = __ldg(p.starts + p.blocks + 1);
+    blocks = p.blocks;
+    prefix_tiles = (min(max(len, 0), p.max_tokens) + TILE - 1) / TILE;
+    // an even share, but no block in more than p.sets segments: its tiles / per + 1 at most
+    per = max(max((line + clusters - 1) / clusters, (most + p.sets - 2) / (p.sets - 1)), MIN_TILES);
+    at = static_cast<int>(min(static_cast<int64_t>(cluster) * per, static_cast<int64_t>(line)));
+    end = static_cast<int>(min(static_cast<int64_t>(at) + per, static_cast<int64_t>(line)));
   }
-  __device__ __forceinline__ bool next() {
+  __device__ __forceinline__ bool next(const int32_t* starts) {
     if (at >= end) return false;
-    block = static_cast<int>(at / tiles);
-    first = static_cast<int>(at - static_cast<int64_t>(block) * tiles);
-    count = static_cast<int>(min(end - at, static_cast<int64_t>(tiles - first)));
+    // the last block that starts at or before `at`, 32 candidates at a time
+    const int lane = threadIdx.x & 31;
+    int lo = 0, n = blocks;
+    while (n > 1) {
+      const int step = (n + 31) / 32;
+      const bool below = lane * step < n && __ldg(starts + lo + lane * step) <= at;
+      const int hit = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
+      n = min(step, n - hit * step);
+      lo += hit * step;
+    }
+    block = lo;
+    const int begin = __ldg(starts + lo), tiles = __ldg(starts + lo + 1) - begin;
+    first = at - begin;
+    count = min(end - at, tiles - first);
+    shared = min(count, max(prefix_tiles - first, 0));
     // segments of this block before this one: shares that begin in it, and the one it begins in
-    const int64_t begin = static_cast<int64_t>(block) * tiles;
-    set = static_cast<int>(at / per - begin / per);
+    set = at / per - begin / per;
     last = first + count == tiles;
     at += count;
     return true;
   }
+};
+
+// The tiles of own tokens of a block one after the other, from the `skip`-th on: of each request
+// with rows in the block.  The roles walk them in loops of their own behind the prefix's, whose
+// loops stay as short as they can be: with one loop for both the prefix's tiles took 18 % longer.
+struct OwnTile {
+  int req, own, len;             // the request, which tile of its tokens, and how many it has
+  __device__ __forceinline__ OwnTile(const PrefixParams& p, int block, int skip) {
+    req = block * 2 * ROWS / (p.s_q * p.h_q) - 1;
+    own = len = 0;
+    for (; skip >= 0; --skip) step(p);
+  }
+  __device__ __forceinline__ void step(const PrefixParams& p) {
+    if (++own * TILE < len) return;
+    own = 0;
+    for (len = 0; len == 0 && req + 1 < p.b;) len = own_tokens(p, ++req);
+  }
+  // first row of the workspace
+  __device__ __forceinline__ int row(const PrefixParams& p) const { return p.padded + req * p.own_padded + own * TILE; }
 };
 
 template <int DQK>
@@ -241,19 +290,16 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
       // ======================= Q and K ======================================================
       const uint32_t elected = elect_one();
       int n = 0;
-      while (ok && w.next()) {
-        for (int i = 0; i < w.count && ok; ++i, ++n) {
-          if (i == 0) {
-            // Q is free once every product of the segment before is done
-            for (int g = 0; g < C::GROUPS; ++g) wait(&ctrl.k_empty[g], (n & 1) ^ 1, ERR_SLOT);
-            if (!ok) break;
-            if (elected) {
-              if (rank == 0) mbar_expect_tx(bar(&ctrl.q_land), 2 * C::Q_BYTES);
-              for (int c = 0; c < C::NB; ++c)
-                load_pair(sQ + c * QK_BLOCK, &p.mq, 64 * c, 0, w.block * 2 * ROWS + rank * ROWS, of_leader(bar(&ctrl.q_land)));
-            }
-          }
-          const int tok = (w.first + i) * TILE + rank * ROWS;
+      while (__all_sync(0xffffffffu, ok) && w.next(p.starts)) {
+        // Q is free once every product of the segment before is done
+        for (int g = 0; g < C::GROUPS; ++g) wait(&ctrl.k_empty[g], (n & 1) ^ 1, ERR_SLOT);
+        if (ok && elected) {
+          if (rank == 0) mbar_expect_tx(bar(&ctrl.q_land), 2 * C::Q_BYTES);
+          for (int c = 0; c < C::NB; ++c)
+            load_pair(sQ + c * QK_BLOCK, &p.mq, 64 * c, 0, w.block * 2 * ROWS + rank * ROWS, of_leader(bar(&ctrl.q_land)));
+        }
+        auto load = [&](int tok) {
+          tok += rank * ROWS;
           for (int g = 0; g < C::GROUPS; ++g) {
             wait(&ctrl.k_empty[g], (n & 1) ^ 1, ERR_SLOT);
             if (!ok) break;
@@ -263,15 +309,24 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
                 load_pair(sK + c * QK_BLOCK, &p.mk, 64 * c, 0, tok, of_leader(bar(&ctrl.k_land[g])));
             }
           }
+          ++n;
+        };
+        int i = 0;
+        for (; i < w.shared && ok; ++i) load((w.first + i) * TILE);
+        if (i < w.count) {
+          OwnTile tile(p, w.block, w.first + i - w.prefix_tiles);
+          for (; i < w.count && ok; ++i) {
+            load(tile.row(p));
+            tile.step(p);
+          }
         }
       }
     } else if (warp == WARP_LOAD_V) {
       // ======================= V ============================================================
       const uint32_t elected = elect_one();
       int n = 0;
-      while (ok && w.next()) {
-        for (int i = 0; i < w.count && ok; ++i, ++n) {
-          const int tok = (w.first + i) * TILE;
+      while (__all_sync(0xffffffffu, ok) && w.next(p.starts)) {
+        auto load = [&](int tok) {
           for (int h = 0; h < 2; ++h) {
             wait(&ctrl.v_empty[h], (n & 1) ^ 1, ERR_SLOT);
             if (!ok) break;
@@ -280,6 +335,16 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
               for (int c = 0; c < 2; ++c)
                 load_pair(sV + (2 * h + c) * V_BLOCK, &p.mv, 256 * h + 128 * rank + 64 * c, 0, tok, of_leader(bar(&ctrl.v_land[h])));
             }
+          }
+          ++n;
+        };
+        int i = 0;
+        for (; i < w.shared && ok; ++i) load((w.first + i) * TILE);
+        if (i < w.count) {
+          OwnTile tile(p, w.block, w.first + i - w.prefix_tiles);
+          for (; i < w.count && ok; ++i) {
+            load(tile.row(p));
+            tile.step(p);
           }
         }
       }
@@ -292,7 +357,7 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
       const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0) + COL_S;
       const uint32_t elected = elect_one();
       int n = 0, seg = 0;
-      while (ok && w.next()) {
+      while (__all_sync(0xffffffffu, ok) && w.next(p.starts)) {
         wait(&ctrl.q_land, seg & 1, ERR_Q);
         ++seg;
         const int count = __shfl_sync(0xffffffffu, w.count, 0);
@@ -323,7 +388,7 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
       const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0) + COL_O;
       const uint32_t elected = elect_one();
       int n = 0, seg = 0;
-      while (ok && w.next()) {
+      while (__all_sync(0xffffffffu, ok) && w.next(p.starts)) {
         wait(&ctrl.o_free, (seg & 1) ^ 1, ERR_FREE);     // the segment before has been read out
         ++seg;
         const int count = __shfl_sync(0xffffffffu, w.count, 0);
@@ -360,20 +425,16 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
     };
     const int64_t total_tiles = w.end - w.at;
     int n = 0;
-    while (w.next()) {
+    while (w.next(p.starts)) {
       if (tid < ROWS) ctrl.ref[tid] = -INFINITY;
       bar_sync(BAR_BOTH, SOFTMAX_THREADS);
       float m_ref = -INFINITY, l = 0.f;            // l is relative to m_ref
-      const uint2* bits = reinterpret_cast<const uint2*>(p.valid) + w.first * 2 + half;
       const int mine = (n & 1) == group ? 0 : 1;   // this group's first tile of the segment
-      uint2 ahead = make_uint2(0u, 0u);
-      if (mine < w.count) ahead = __ldg(bits + 2 * mine);
       const int n0 = n;                            // tiles of the segments before
-#pragma unroll 1
-      for (int i = mine; i < w.count; i += 2) {
+      const int row = w.block * 2 * ROWS + rank * ROWS + r;
+      // Tile i of the segment; of this thread's 64 tokens its row sees those whose bits are set.
+      auto attend = [&](int i, uint2 seen) {
         n = n0 + i;
-        const uint2 seen = ahead;
-        if (i + 2 < w.count) ahead = __ldg(bits + 2 * (i + 2));
         wait(&ctrl.s_full[group], (n >> 1) & 1, ERR_S);
         tc_fence_after_sync();
         uint32_t x[64];
@@ -453,6 +514,44 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) arrive_leader(bar(&ctrl.p_full));
+      };
+      // bits are fetched a tile ahead
+      const uint2* bits = reinterpret_cast<const uint2*>(p.valid) + w.first * 2 + half;
+      int i = mine;
+      uint2 ahead = make_uint2(0u, 0u);
+      if (i < w.shared) ahead = __ldg(bits + 2 * i);
+#pragma unroll 1
+      for (; i < w.shared; i += 2) {
+        const uint2 seen = ahead;
+        if (i + 2 < w.shared) ahead = __ldg(bits + 2 * (i + 2));
+        attend(i, seen);
+      }
+      if (i < w.count) {
+        const int rows_of_req = p.s_q * p.h_q, my_req = row / rows_of_req, unseen = p.s_q - 1 - row % rows_of_req / p.h_q;
+        OwnTile tile(p, w.block, w.first + i - w.prefix_tiles);
+        auto own_bits = [&]() {
+          const int64_t at = tile.row(p) >> 5;
+          uint2 v = __ldg(reinterpret_cast<const uint2*>(p.valid + at) + half);
+          // of this row's request, up to its own place
+          const int sees = tile.req == my_req ? tile.len - unseen - tile.own * TILE - 64 * half : 0;
+          if (sees < 64) v.y &= sees <= 32 ? 0u : (1u << (sees - 32)) - 1u;
+          if (sees < 32) v.x &= sees <= 0 ? 0u : (1u << sees) - 1u;
+          // the setup has zeroed what is not finite, for the rows that do not see it
+          const uint2 unfit = __ldg(reinterpret_cast<const uint2*>(p.unfit + at) + half);
+          if (((unfit.x & v.x) | (unfit.y & v.y)) != 0u) l = NAN;
+          return v;
+        };
+        ahead = own_bits();
+#pragma unroll 1
+        for (; i < w.count; i += 2) {
+          const uint2 seen = ahead;
+          if (i + 2 < w.count) {
+            tile.step(p);
+            tile.step(p);
+            ahead = own_bits();
+          }
+          attend(i, seen);
+        }
       }
       n = n0 + w.count;
       // ---- the segment's partial ------------------------------------------------------------
@@ -465,7 +564,6 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
       wait(&ctrl.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1, ERR_O);
       tc_fence_after_sync();
       const bool fail = *reinterpret_cast<volatile int*>(&ctrl.fail) != 0;
-      const int row = w.block * 2 * ROWS + rank * ROWS + r;
       const bool none = total == 0.f;
       const float f = none ? 0.f : 1.f / total;
       if (group == 0 && half == 0 && row < p.rows) {
@@ -494,12 +592,12 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
         }
       }
     }
-    // no tile at all: nobody else writes the sets of these rows
-    if (w.tiles == 0) {
-      const int clusters = gridDim.x >> 1;
-      for (int64_t i = static_cast<int64_t>(blockIdx.x) * SOFTMAX_THREADS + tid; i < static_cast<int64_t>(p.sets) * p.rows;
-           i += static_cast<int64_t>(2 * clusters) * SOFTMAX_THREADS)
-        p.lse_accum[i] = -INFINITY;
+    // blocks without any tile: nobody else marks the sets of their rows
+    for (int k = blockIdx.x >> 1; k < p.blocks; k += gridDim.x >> 1) {
+      if (__ldg(p.starts + k) != __ldg(p.starts + k + 1)) continue;
+      const int row = k * 2 * ROWS + rank * ROWS + tid;
+      if (tid < ROWS && row < p.rows)
+        for (int i = 0; i < p.sets; ++i) p.lse_accum[static_cast<int64_t>(i) * p.rows + row] = -INFINITY;
     }
   }
   grid_launch_dependents();
@@ -512,10 +610,63 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
 }
 
+// Is one of two BF16 numbers an infinity or NaN?
+__device__ __forceinline__ bool not_finite(uint32_t two) {
+  return (two & 0x7f80u) == 0x7f80u || (two & 0x7f800000u) == 0x7f800000u;
+}
+
+// starts[k]: tiles of the row blocks before block k (the prefix's, and of the own tokens of every
+// request with rows in the block); then their sum, and the most tiles of a block.  One CTA of 256.
+__device__ __forceinline__ void block_starts(const Dsv4SharedPrefixArgs& a, const SharedSetup& out, int prefix) {
+  __shared__ int part[8], top[8];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rows_of_req = a.s_q * a.h_q, rows = a.b * rows_of_req, blocks = (rows + 2 * ROWS - 1) / (2 * ROWS);
+  const int prefix_tiles = (prefix + TILE - 1) / TILE;
+  int carry = 0, most = 0;
+  for (int k0 = 0; k0 < blocks; k0 += 256) {
+    const int k = k0 + tid;
+    int n = 0;
+    if (k < blocks) {
+      n = prefix_tiles;
+      if (out.own_padded > 0)
+        for (int r = k * 2 * ROWS / rows_of_req; r <= (min((k + 1) * 2 * ROWS, rows) - 1) / rows_of_req; ++r)
+          n += (min(max(a.suffix_length[r], 0), a.max_pages * a.page_block_size) + TILE - 1) / TILE;
+    }
+    most = max(most, n);
+    int sum = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += o;
+    }
+    if (lane == 31) part[warp] = sum;
+    __syncthreads();
+    int before = carry, all = carry;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i < warp) before += part[i];
+      all += part[i];
+    }
+    if (k < blocks) out.starts[k] = before + sum - n;
+    carry = all;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+  if (lane == 0) top[warp] = most;
+  __syncthreads();
+  if (tid == 0) {
+    for (int i = 1; i < 8; ++i) most = max(most, top[i]);
+    out.starts[blocks] = carry;
+    out.starts[blocks + 1] = most;
+  }
+}
+
 // One launch for what the attention kernels read besides the cache.  CTAs [0, row_ctas): FP8 rows
-// of the prefix -> BF16 rows [tokens, d_qk], and a bit per token that says whether it exists; rows
-// that do not are zero.  Whole tiles of 128 tokens are written.  Bound by memory: 644 (584) B in
-// and 1152 (1024) B out per token; a warp has four tokens in flight.  CTAs [row_ctas, +list_ctas):
+// of the prefix, and of every request's own tokens, -> BF16 rows [tokens, d_qk], and a bit per
+// token that says whether it exists; rows that do not are zero.  Whole tiles of 128 tokens are
+// written.  Bound by memory: 644 (584) B in and 1152 (1024) B out per token; a warp has four
+// tokens in flight.  One CTA: where the row blocks' tiles start.  CTAs [row_ctas, +list_ctas):
 // token indices of the prefix.  The others: one query token's list each, of its own tokens or of
 // the prefix and those.  List entries behind a length are not written: nothing reads them.
 template <int FMT>
@@ -531,6 +682,13 @@ shared_setup_kernel(const Dsv4SharedPrefixArgs a, const SharedSetup out, const F
   };
   if (static_cast<int>(blockIdx.x) >= row_ctas) {
     int x = blockIdx.x - row_ctas;
+    if (out.starts != nullptr) {
+      if (x == 0) {
+        block_starts(a, out, prefix);
+        return;
+      }
+      --x;
+    }
     if (x < list_ctas) {
       for (int j = x * 256 + threadIdx.x; j < prefix; j += list_ctas * 256)
         out.prefix_list[j] = entry(a.prefix_table, a.prefix_pages, j);
@@ -554,18 +712,34 @@ shared_setup_kernel(const Dsv4SharedPrefixArgs a, const SharedSetup out, const F
     return;
   }
 
-  const int tok0 = blockIdx.x * 32;
-  if (tok0 >= (prefix + TILE - 1) / TILE * TILE) return;
+  // 32 rows of the workspace: of the prefix, or behind those of a request's own tokens
+  const int row0 = blockIdx.x * 32;
+  int tok0 = row0, len = prefix;
+  const int32_t* table = a.prefix_table;
+  const bool own = row0 >= out.padded;
+  if (own) {
+    const int r = (row0 - out.padded) / out.own_padded;
+    tok0 = (row0 - out.padded) - r * out.own_padded;
+    len = min(max(a.suffix_length[r], 0), a.max_pages * a.page_block_size);
+    table = a.block_table + r * a.stride_table;
+  }
+  if (tok0 >= (len + TILE - 1) / TILE * TILE) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // every warp knows where the CTA's 32 tokens live: lane i looks up token i
   const int tok = tok0 + lane;
   const int col = static_cast<int>(div_by(static_cast<uint32_t>(tok), page));
   int id = -1;
-  if (tok < prefix) id = __ldg(a.prefix_table + col);
+  if (tok < len) id = __ldg(table + col);
   const bool live = id >= 0 && id < a.num_blocks;
   const uint32_t word = __ballot_sync(0xffffffffu, live);
   if (threadIdx.x == 0) out.valid[blockIdx.x] = word;
   const int off = tok - col * a.page_block_size;
+
+  // A tile of own tokens is multiplied with the rows of other requests too, with weights of zero;
+  // so that zero times it is zero, a row whose values are not finite is written as zeros and noted
+  // (the values are the first 512 numbers: of MODEL1 the rotary part too).
+  __shared__ uint32_t noted[8];
+  uint32_t unfit = 0;
 
   const uint8_t* kv = static_cast<const uint8_t*>(a.kv);
   uint4 latent[4], rope[4];
@@ -588,24 +762,46 @@ shared_setup_kernel(const Dsv4SharedPrefixArgs a, const SharedSetup out, const F
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out.rows) + static_cast<int64_t>(tok0 + warp * 4 + k) * T::D_QK);
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out.rows) + static_cast<int64_t>(row0 + warp * 4 + k) * T::D_QK);
+    uint32_t o[8] = {};
     if (lane < T::D_NOPE / 16) {
       const ScalePair c = scale_pair(scale[k]);
       const bool two = scale[k] > MAX_ONE_MULTIPLY_SCALE;
-      uint32_t o[8];
       dequant4(latent[k].x, c, two, o[0], o[1]);
       dequant4(latent[k].y, c, two, o[2], o[3]);
       dequant4(latent[k].z, c, two, o[4], o[5]);
       dequant4(latent[k].w, c, two, o[6], o[7]);
+    }
+    if (own) {
+      bool wild = false;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) wild |= not_finite(o[q]);
+      if (T::D_NOPE < D_V) wild |= not_finite(rope[k].x) || not_finite(rope[k].y) || not_finite(rope[k].z) || not_finite(rope[k].w);
+      if (__any_sync(0xffffffffu, wild)) {
+        unfit |= 1u << (warp * 4 + k);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) o[q] = 0;
+        rope[k] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    if (lane < T::D_NOPE / 16) {
       dst[2 * lane] = make_uint4(o[0], o[1], o[2], o[3]);
       dst[2 * lane + 1] = make_uint4(o[4], o[5], o[6], o[7]);
     }
     if (lane < 8) dst[T::D_NOPE / 8 + lane] = rope[k];
   }
+  if (!own) return;
+  if (lane == 0) noted[warp] = unfit;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const uint32_t all = __reduce_or_sync(0xffffffffu, lane < 8 ? noted[lane] : 0u);
+    if (lane == 0) out.unfit[blockIdx.x] = all;
+  }
 }
 
-// Joins few partial sets of many rows: one warp per (row, head), which has the whole 2 KB of four
-// sets in flight; sets in order, so that the result does not depend on timing.
+// Joins the partial sets of many rows: one warp per (row, head), which has the whole 2 KB of four
+// sets in flight; sets in order, so that the result does not depend on timing.  NaN in any of a
+// row's log-sum-exps makes the row NaN.
 __global__ void __launch_bounds__(256)
 join_sets_kernel(const Dsv4CombineArgs a) {
   grid_dependency_wait();
@@ -614,15 +810,23 @@ join_sets_kernel(const Dsv4CombineArgs a) {
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (item >= rows) return;
   const int row = static_cast<int>(item / a.h_q), h = static_cast<int>(item - static_cast<int64_t>(row) * a.h_q);
-  float e = -INFINITY;
-  if (lane < a.n_splits) e = a.lse_accum[lane * rows + item];
-  const bool failed = __any_sync(0xffffffffu, e != e);
-  float m = e;
+  auto lse_of = [&](int set) { return set < a.n_splits ? a.lse_accum[set * rows + item] : -INFINITY; };
+  float m = -INFINITY;
+  bool failed = false;
+  for (int s = lane; s < a.n_splits; s += 32) {
+    const float e = lse_of(s);
+    failed |= e != e;
+    m = fmaxf(m, e);
+  }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  if (failed) m = NAN;
-  const float w = e == -INFINITY ? 0.f : expf(e - m);
-  float l = w;
+  if (__any_sync(0xffffffffu, failed)) m = NAN;
+  auto weight_of = [&](int set) {
+    const float e = lse_of(set);
+    return e == -INFINITY ? 0.f : expf(e - m);
+  };
+  float l = 0.f;
+  for (int s = lane; s < a.n_splits; s += 32) l += weight_of(s);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
   const bool has_sink = a.attn_sink != nullptr;
@@ -633,12 +837,14 @@ join_sets_kernel(const Dsv4CombineArgs a) {
   for (int q = 0; q < 16; ++q) acc[q] = 0.f;
   // lane: columns 8 * lane .. +8 of each half of the row
   const float4* src = reinterpret_cast<const float4*>(a.o_accum + item * D_V) + 2 * lane;
+  float w = 0.f;
   for (int s0 = 0; s0 < a.n_splits; s0 += 4) {
+    if ((s0 & 31) == 0) w = weight_of(s0 + lane);
     float4 v[4][4];
     float ws[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      ws[j] = s0 + j < a.n_splits ? __shfl_sync(0xffffffffu, w, s0 + j) : 0.f;
+      ws[j] = __shfl_sync(0xffffffffu, w, (s0 + j) & 31);       // (0 behind the last set)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         v[j][q] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -707,31 +913,61 @@ int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 }  // namespace
 
-// A share is at least line / clusters long, so at most clusters / blocks of them lie in a row
-// block, and two more reach into it.
+// Enough for even shares of even blocks (a share is at least line / clusters long, so at most
+// clusters / blocks of them lie in a row block, and two reach into it), and one more for uneven ones.
 int prefix_attn_sets(int64_t rows, int num_sms) {
   const int64_t blocks = (rows + 2 * ROWS - 1) / (2 * ROWS), clusters = num_sms / 2;
-  return static_cast<int>((clusters + blocks - 1) / blocks + 1);
+  return static_cast<int>((clusters + blocks - 1) / blocks + 2);
 }
 
-int64_t prefix_attn_workspace(int64_t tokens, int d_qk) {
-  const int64_t padded = round_up(tokens, TILE);
-  return round_up(padded / 8, 256) + padded * d_qk * 2;
+namespace {
+struct Places {
+  int64_t padded, own_padded, rows, blocks, unfit, starts, values, bytes;
+};
+Places places(const Dsv4SharedPrefixArgs& a, bool own) {
+  Places x;
+  x.padded = round_up(static_cast<int64_t>(a.prefix_pages) * a.page_block_size, TILE);
+  x.own_padded = own ? round_up(static_cast<int64_t>(a.max_pages) * a.page_block_size, TILE) : 0;
+  x.rows = x.padded + x.own_padded * a.b;
+  x.blocks = (static_cast<int64_t>(a.b) * a.s_q * a.h_q + 2 * ROWS - 1) / (2 * ROWS);
+  x.unfit = round_up(x.rows / 8, 256);                         // two sets of bits first
+  x.starts = 2 * x.unfit;
+  x.values = x.starts + round_up((x.blocks + 2) * 4, 256);
+  x.bytes = x.values + x.rows * a.d_qk * 2;
+  return x;
+}
+}  // namespace
+
+int64_t prefix_attn_workspace(const Dsv4SharedPrefixArgs& a, bool own) { return places(a, own).bytes; }
+
+bool prefix_attn_fits(const Dsv4SharedPrefixArgs& a, bool own) {
+  const Places x = places(a, own);
+  const int64_t most = 0x7fffffff - 65536;
+  // rows, and the tiles of all blocks (a request's are counted in each block that it has rows in),
+  // as 32-bit numbers with room for what is added to them
+  return x.rows <= most && x.blocks * (x.padded / TILE) + (x.blocks + a.b) * (x.own_padded / TILE) <= most;
 }
 
-void prefix_attn_place(int64_t tokens, void* workspace, SharedSetup& out) {
-  out.valid = static_cast<uint32_t*>(workspace);
-  out.rows = static_cast<uint8_t*>(workspace) + round_up(round_up(tokens, TILE) / 8, 256);
+void prefix_attn_place(const Dsv4SharedPrefixArgs& a, bool own, SharedSetup& out) {
+  const Places x = places(a, own);
+  uint8_t* base = static_cast<uint8_t*>(a.workspace);
+  out.valid = reinterpret_cast<uint32_t*>(base);
+  out.unfit = reinterpret_cast<uint32_t*>(base + x.unfit);
+  out.starts = reinterpret_cast<int32_t*>(base + x.starts);
+  out.rows = base + x.values;
+  out.padded = static_cast<int>(x.padded);
+  out.own_padded = static_cast<int>(x.own_padded);
 }
 
 cudaError_t launch_shared_setup(const Dsv4SharedPrefixArgs& a, const SharedSetup& out, cudaStream_t st) {
   const int64_t tokens = static_cast<int64_t>(a.prefix_pages) * a.page_block_size;
-  const int row_ctas = out.rows != nullptr ? static_cast<int>(round_up(tokens, TILE) / 32) : 0;
+  const int row_ctas = out.rows != nullptr ? static_cast<int>((out.padded + static_cast<int64_t>(out.own_padded) * a.b) / 32) : 0;
   const int list_ctas = out.prefix_list == nullptr ? 0 : static_cast<int>(tokens < 64 * 1024 ? (tokens + 1023) / 1024 : 64);
   const int lists = out.suffix_lists != nullptr || out.joined != nullptr ? a.b * a.s_q : 0;
-  if (row_ctas + list_ctas + lists == 0) return cudaSuccess;
+  const int starts = out.starts != nullptr ? 1 : 0;
+  if (row_ctas + list_ctas + lists + starts == 0) return cudaSuccess;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(row_ctas) + list_ctas + lists);
+  cfg.gridDim = dim3(static_cast<unsigned>(row_ctas) + starts + list_ctas + lists);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -744,6 +980,8 @@ cudaError_t launch_shared_setup(const Dsv4SharedPrefixArgs& a, const SharedSetup
 }
 
 cudaError_t launch_join_sets(const Dsv4CombineArgs& a, cudaStream_t st) {
+  // Many sets are those of few rows: the combine kernel has a CTA for each row (256 rows of 39 sets:
+  // the whole call 52 us with it, 63 with a warp per row).
   if (a.n_splits > 32) return launch_combine(a, st);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(a.n_rows) * a.h_q + 7) / 8));
@@ -756,20 +994,30 @@ cudaError_t launch_join_sets(const Dsv4CombineArgs& a, cudaStream_t st) {
 }
 
 cudaError_t launch_prefix_attn(const Dsv4SharedPrefixArgs& a, const SharedSetup& setup, int num_sms, cudaStream_t st) {
-  const int64_t tokens = static_cast<int64_t>(a.prefix_pages) * a.page_block_size, padded = round_up(tokens, TILE);
   cudaError_t e;
   PrefixParams p;
   p.rows = a.b * a.s_q * a.h_q;
+  p.blocks = (p.rows + 2 * ROWS - 1) / (2 * ROWS);
   p.sets = prefix_attn_sets(p.rows, num_sms);
-  p.max_tokens = static_cast<int>(tokens);
+  p.max_tokens = a.prefix_pages * a.page_block_size;
+  p.padded = setup.padded;
+  p.own_padded = setup.own_padded;
+  p.own_max = setup.own_padded > 0 ? a.max_pages * a.page_block_size : 0;
+  p.b = a.b;
+  p.s_q = a.s_q;
+  p.h_q = a.h_q;
   p.length = a.prefix_length;
+  p.own = a.suffix_length;
+  p.starts = setup.starts;
   p.valid = setup.valid;
+  p.unfit = setup.unfit;
   p.sm_scale = a.sm_scale;
   p.o_accum = a.o_accum;
   p.lse_accum = a.lse_accum;
+  const int tokens = setup.padded + setup.own_padded * a.b;
   if ((e = make_map_16bit(&p.mq, true, a.q, p.rows, 1, a.d_qk, a.d_qk, a.d_qk, ROWS, 1))) return e;
-  if ((e = make_map_16bit(&p.mk, true, setup.rows, static_cast<int>(padded), 1, a.d_qk, a.d_qk, a.d_qk, ROWS, 1))) return e;
-  if ((e = make_map_16bit(&p.mv, true, setup.rows, static_cast<int>(padded), 1, a.d_qk, a.d_qk, a.d_qk, TILE, 1))) return e;
+  if ((e = make_map_16bit(&p.mk, true, setup.rows, tokens, 1, a.d_qk, a.d_qk, a.d_qk, ROWS, 1))) return e;
+  if ((e = make_map_16bit(&p.mv, true, setup.rows, tokens, 1, a.d_qk, a.d_qk, a.d_qk, TILE, 1))) return e;
   return a.d_qk == 576 ? launch_attn<576>(p, num_sms / 2, st) : launch_attn<512>(p, num_sms / 2, st);
 }
 

@@ -237,6 +237,44 @@ def test_lengths_that_lie_are_clamped(form):
         x.check(x.call(flags=form), x.definition(p, s))
 
 
+@pytest.mark.parametrize("layout", ["V32", "MODEL1"])
+@pytest.mark.parametrize("form", FORMS)
+def test_tokens_that_are_not_finite_reach_the_rows_that_see_them_alone(layout, form):
+    x = Batch(layout, 7, 2, 16, 700, [40, 0, 129, 1, 300, 64, 2], 64, seed=3)
+    want = x.definition()
+    spoilt = torch.zeros(7, 2, dtype=torch.bool, device="cuda")
+    for r, at, where in ((0, 39, "latent"), (2, 127, "latent"), (4, 299, "rope"), (6, 0, "latent")):
+        page, at = int(x.table[r, at // 64]), at % 64
+        spoilt[r] |= torch.arange(2, device="cuda") >= 1 - (x.suffix[r] - 1 - 64 * (0, 0, 1, 0, 4, 0, 0)[r] - at)
+        if where == "latent":                              # 2^128 times the codes: infinities of both signs
+            x.arena[page, 64 * (x.d + 128) + at * x.slots + 1] = 255
+        else:
+            x.arena[page, at * (x.d + 128) + x.d:][:2] = 0xff
+    out, lse = x.call(flags=form)
+    if form == N.FLAG_SHARED_DENSE:
+        assert torch.isnan(out[spoilt]).all() and torch.isnan(lse.transpose(1, 2)[spoilt]).all()
+    fine = ~spoilt
+    off = (out.double() - want[0]).abs() / (U * (want[1] + want[0].abs()) + SCORES * want[1] + 1e-30)
+    assert float(off[fine].max()) <= 1
+    assert ((lse.double() - want[2]).abs().transpose(1, 2)[fine] <= SCORES + 2e-6 * want[2].abs().transpose(1, 2)[fine]).all()
+
+
+@pytest.mark.parametrize("form", FORMS[1:])
+@pytest.mark.parametrize("pages", [300, 600])
+def test_wide_tables_of_short_requests(pages, form):
+    """A table that could hold far more own tokens than there are."""
+    x = Batch("V32", 5, 2, 48, 700, [300, 0, 1, 129, 64], 64, seed=4, sink=True)
+    x.table = torch.cat([x.table, torch.full((5, pages), 2 ** 30, dtype=torch.int32, device="cuda")], 1)
+    x.check(x.call(flags=form))
+
+
+@pytest.mark.parametrize("s_q,h_q", [(1, 8), (1, 24), (3, 16), (2, 64), (5, 40)])
+def test_blocks_that_hold_parts_of_requests(s_q, h_q):
+    suffix = [(53 * r * r) % 700 for r in range(23)]
+    x = Batch("V32", 23, s_q, h_q, 3000, suffix, 64, seed=h_q)
+    x.check(x.call(flags=N.FLAG_SHARED_DENSE))
+
+
 @pytest.mark.parametrize("form", FORMS[1:])
 def test_captured_and_replayed_with_other_lengths(form):
     x = Batch("V32", 6, 1, 64, 1000, [200, 100, 3, 0, 64, 65], 64)
