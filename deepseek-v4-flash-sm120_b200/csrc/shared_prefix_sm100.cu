@@ -262,12 +262,17 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
                  ::"r"(smem_u32(&ctrl.tmem)), "r"(TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
-  grid_dependency_wait();
+  if (warp == WARP_LOAD_K && lane == 0) {
+    tma_prefetch_map(&p.mq);
+    tma_prefetch_map(&p.mk);
+    tma_prefetch_map(&p.mv);
+  }
   tc_fence_before_sync();
   __syncthreads();
   cluster_sync();                                // the other CTA's barriers and TMEM are there too
   tc_fence_after_sync();
   const uint32_t tmem = ctrl.tmem;
+  grid_dependency_wait();
   Share w(p, blockIdx.x >> 1, gridDim.x >> 1);
   // A role whose bounded wait gives up records it and waits for nothing any more; what it does
   // from then on is of no use, but every barrier of the CTA is still walked.
@@ -674,6 +679,7 @@ __global__ void __launch_bounds__(256)
 shared_setup_kernel(const Dsv4SharedPrefixArgs a, const SharedSetup out, const FastDiv page, int row_ctas, int list_ctas) {
   using T = KvTraits<FMT>;
   grid_dependency_wait();
+  grid_launch_dependents();        // the next kernel sets itself up meanwhile, and waits for this one
   const int prefix = a.prefix_pages > 0 ? min(max(*a.prefix_length, 0), a.prefix_pages * a.page_block_size) : 0;
   const int n_tok = a.num_blocks * a.page_block_size;
   auto entry = [&](const int32_t* table, int pages, int pos) {
