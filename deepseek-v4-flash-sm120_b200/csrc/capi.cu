@@ -1,6 +1,7 @@
 // extern "C" entry points: argument validation, translation to the kernel-side
 // parameter block, dispatch.  Allocates nothing and never synchronises.
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -544,34 +545,31 @@ int dsv4_plan_dense_splits(int t_q, int t_k, int b, int h_q, int h_kv, int num_s
   if (t_q < 1 || t_k < 1 || b < 1 || h_q < 1 || h_kv < 1 || h_q % h_kv || num_sms < 1) return 1;
   const int64_t ctas = dsv4::dense_ctas(t_q, b, h_q, h_kv);
   const double tiles = static_cast<double>(t_k) / b / 128.0;           // of a sequence, on average
-  if (ctas >= num_sms || tiles <= 2.0) return 1;
-  // In microseconds, fitted to calls of 1 to 60 sequences on a B200: a CTA starts and ends in 5,
+  if (tiles <= 2.0) return 1;
+  // In microseconds, fitted to calls of 1 to 200 sequences on a B200: a CTA starts and ends in 5,
   // streams a tile of 128 keys in 1 (64 to 80 KB, what its buffers keep in flight), and the
-  // GPU's memory gives a tile in 0.0105; joining costs 3 and 0.15 a range.  The lengths are on
-  // the device: the longest sequence is taken to be three times the average one, and a plan of
-  // more CTAs than SMs to end 15 % unevenly.  (One sequence of 8000 keys, 64 heads on one: 78 us
-  // uncut, 23 in 8 ranges; 8 of 1000 to 16383 keys, 32 heads on 8: 105 and 61; 32 of 4096 fill
-  // the GPU: 95 uncut, 113 in 2.)
+  // GPU's memory gives a tile in 0.0105; a launch more costs 3, a range 0.6, and the partials are
+  // written and read at 4 TB/s.  The lengths are on the device: the longest sequence is taken to
+  // be eight times the average one.  (One sequence of 8000 keys, 64 heads on one: 78 us uncut, 22
+  // in ranges; 60 of 1 to 20000 keys, 8 heads of 64: 170 and 81; 32 of 4096, 32 heads on 8, which
+  // fill the GPU evenly: 95 and 102.)
   const double total = static_cast<double>(t_k) / 128.0;
-  const double longest = tiles * 3.0 < total ? tiles * 3.0 : total;
-  int best = 1;
-  double best_cost = 1e30;
-  for (int s = 1; s <= dsv4::DENSE_MAX_SPLITS && s <= tiles; ++s) {
-    const double at_once = ctas * s < num_sms ? static_cast<double>(ctas) * s : num_sms;
-    const double chain = 5.0 + longest / s;
-    const double streamed = ctas * tiles / at_once > ctas * tiles * 0.0105 ? ctas * tiles / at_once : ctas * tiles * 0.0105;
-    const double all = (ctas * s * 5.0 / num_sms + streamed) * (ctas * s > num_sms ? 1.15 : 1.0);
-    const double cost = (chain > all ? chain : all) + (s > 1 ? 3.0 + 0.15 * s : 0.0);
-    if (cost < best_cost - 1e-9) { best_cost = cost; best = s; }
-  }
-  return best;
+  const double longest = std::fmin(tiles * 8.0, total);
+  const double line = ctas * tiles, memory = line * 0.0105;
+  const double uncut = std::fmax(5.0 + longest, std::fmax((ctas * 5.0 + line) / num_sms, memory));
+  const double per = std::fmax(line / num_sms, std::sqrt(0.6 * longest));      // tiles of a range
+  const double used = ctas * std::fmax(tiles / per, 1.0);
+  const double partials = 2.0 * t_q * h_q * 128.0 * 4.0 * (tiles / per + 1.0) / 4.0e6;
+  const double cut = std::fmax(5.0 + per, std::fmax((used * 5.0 + line) / num_sms, memory + 5.0)) + 3.0 + 0.6 * longest / per + partials;
+  if (cut >= uncut) return 1;
+  return static_cast<int>(std::fmin(std::fmax(longest / per, 2.0), dsv4::DENSE_MAX_SPLITS));
 }
 
 int dsv4_dense_prefill(const Dsv4DensePrefillArgs* a, void* stream) {
   if (!a) return DSV4_ERR_NULL;
   if (a->b < 0 || a->t_q < 0 || a->t_k < 0 || a->h_q < 1 || a->h_kv < 1 || a->h_q % a->h_kv ||
       a->n_splits < 1 || a->n_splits > dsv4::DENSE_MAX_SPLITS || !(a->sm_scale > 0.0f) ||
-      !(a->sm_scale <= 1.0e38f) || dsv4::dense_ctas(a->t_q, a->b, a->h_q, a->h_kv) > 0x7fffffff)
+      !(a->sm_scale <= 1.0e38f) || dsv4::dense_ctas(a->t_q, a->b, a->h_q, a->h_kv) > 0x3fffffff)
     return DSV4_ERR_SHAPE;
   if (!((a->d_qk == 64 && a->d_v == 64) || (a->d_qk == 128 && a->d_v == 128) ||
         (a->d_qk == 192 && a->d_v == 128)))
@@ -598,7 +596,12 @@ int dsv4_dense_prefill(const Dsv4DensePrefillArgs* a, void* stream) {
   }
   int rc = current_device_is_sm100();
   if (rc) return rc;
-  cudaError_t e = dsv4::launch_dense_prefill(*a, static_cast<cudaStream_t>(stream));
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e) return cuda_fail(e);
+  DevInfo info;
+  if ((rc = device_info(dev, info))) return rc;
+  e = dsv4::launch_dense_prefill(*a, info.sms, static_cast<cudaStream_t>(stream));
   return e ? cuda_fail(e) : DSV4_OK;
 }
 

@@ -27,7 +27,7 @@
 // before the tensor core may read it: rows no one sees are cleared, and elements that are not
 // finite are cleared and handed by the epilogue to the rows that do see them.
 //
-// Few rows (single tokens over long contexts): the keys are cut into n_splits ranges, each
+// Few rows (single tokens over long contexts): the keys are cut into up to n_splits ranges, each
 // CTA leaves normalised 32-bit partials, and dense_combine_kernel joins them.  A CTA whose
 // second row tile would be empty then gives the first one's odd key tiles to the second
 // pipeline ("twin"), which halves its chain of products and softmaxes; a range therefore has
@@ -104,7 +104,10 @@ struct DenseParams {
   int pack, tok_tile;            // heads packed per row tile, tokens per row tile
   int chunks;                    // head chunks: h_q / pack
   int slots;                     // row-tile pairs, upper bound over all sequences
-  int n_splits;
+  int n_splits;                  // ranges of a sequence's keys, at most
+  int ctas;                      // of a launch with ranges
+  int items;                     // row-tile pairs x head chunks, upper bound
+  int sms;
   int sectors;                   // rows of the output start on 32 bytes
   float sm_scale;
   const int32_t *cu_q, *cu_k;
@@ -181,6 +184,8 @@ struct Work {
   bool twin;                     // ... or, both row tiles being the same, every second one from s on
   int look;                      // key tiles from this one on are seen only in part by some row
   bool any;
+  int chunk, split;              // heads, range
+  int last_set;                  // partial sets from here on are not written: this CTA marks them
 };
 
 // Keys of the sequence that token t sees: [0, reach).
@@ -192,9 +197,38 @@ __device__ __forceinline__ int reach_of(const DenseParams& p, const Work& w, int
 
 __device__ __forceinline__ int clamp_to(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
+// Which tiles the rows from w.t0 on see of the keys' tiles [first, end).
 template <bool RANGES>
-__device__ __forceinline__ Work find_work(const DenseParams& p, int slot, int split) {
+__device__ __forceinline__ void set_tiles(const DenseParams& p, Work& w, int first, int end) {
+  int tiles[2] = {0, 0};
+  if (w.any) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int a = w.t0 + s * p.tok_tile;
+      if (a < w.len_q)
+        tiles[s] = (reach_of(p, w, min(a + p.tok_tile, w.len_q) - 1) + TILE_N - 1) / TILE_N;
+    }
+  }
+  const int total = max(tiles[0], tiles[1]);
+  w.first = min(first, total);
+  end = min(end, total);
+  w.tiles = end - w.first;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) w.count[s] = max(min(tiles[s], end) - w.first, 0);
+  w.twin = RANGES && w.t0 + p.tok_tile >= w.len_q;
+  if (w.twin) {
+    w.count[0] = (w.tiles + 1) / 2;
+    w.count[1] = w.tiles / 2;
+  }
+  w.look = reach_of(p, w, w.t0) / TILE_N;
+}
+
+__device__ __forceinline__ Work find_work(const DenseParams& p, int block) {
   Work w;
+  // Slots last to first: in a causal sequence the late rows are the long ones.
+  w.chunk = block % p.chunks;
+  const int slot = p.slots - 1 - block / p.chunks;
+  w.split = w.last_set = 0;
   // Sequence s owns the slots from cu_q[s] / span + s on: at least ceil(len / span) of them.
   // Every warp looks for it 32 candidates at a time: the loads of a step do not wait for one
   // another (bisection took one memory latency a halving, up to 2 us of a short CTA's 8).
@@ -230,32 +264,88 @@ __device__ __forceinline__ Work find_work(const DenseParams& p, int slot, int sp
   const int64_t t0 = static_cast<int64_t>(slot - (w.q0 / span + lo)) * span;
   w.any = t0 >= 0 && t0 < w.len_q;
   w.t0 = static_cast<int>(w.any ? t0 : 0);
-  int tiles[2] = {0, 0};
-  if (w.any) {
+  set_tiles<false>(p, w, 0, 0x7fffffff);
+  return w;
+}
+
+// With ranges: the sequences are cut into ranges of about the same length, so that the grid ends
+// evenly whatever their lengths: the shortest length with which the launch's CTAs are enough (and
+// they are for line / (ctas - items) tiles, line being the sum of all items' tiles, since rounding
+// up costs every item less than one range more).  A range streams a tile in about 1 us and costs
+// 0.6 us to start and join, so below sqrt(0.6 tiles) shorter ranges gain nothing.  (As many ranges
+// for every sequence instead, microseconds: 8 of 1000 to 16383 keys, 32 heads on 8, 5 query tokens
+// each: 47, with this 39; 60 of 1 to 20000 keys, 8 heads of 64: 170 uncut and 100 in two, with this 82.)
+__device__ __forceinline__ Work find_range(const DenseParams& p, int block) {
+  Work w = {};
+  const int span = 2 * p.tok_tile, lane = threadIdx.x & 31;
+  int q0 = 0, len_q = 0, k0 = 0, len_k = 0;             // of sequence s0 + lane
+  int items = 0, tiles = 0, shortest = 1;               // its row-tile pairs x chunks, key tiles, shortest range
+  auto fetch = [&](int s0) {
+    const int s = min(s0 + lane, p.b - 1);
+    const int a = __ldg(p.cu_q + s), b = __ldg(p.cu_q + s + 1), c = __ldg(p.cu_k + s), d = __ldg(p.cu_k + s + 1);
+    q0 = clamp_to(a, 0, p.t_q);
+    len_q = s0 + lane < p.b ? clamp_to(b, q0, p.t_q) - q0 : 0;
+    k0 = clamp_to(c, 0, p.t_k);
+    len_k = clamp_to(d, k0, p.t_k) - k0;
+    items = (len_q + span - 1) / span * p.chunks;
+    tiles = (len_k + TILE_N - 1) / TILE_N;
+    shortest = max(max((tiles + p.n_splits - 1) / p.n_splits, static_cast<int>(ceilf(sqrtf(0.6f * tiles)))), 1);
+  };
+  auto parts_of = [&](int even) {
+    const int per = max(even, shortest);
+    return max((tiles + per - 1) / per, 1);
+  };
+  int64_t line = 0;
+  for (int s0 = 0; s0 < p.b; s0 += 32) {
+    fetch(s0);
+    line += static_cast<int64_t>(items) * tiles;
+  }
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int a = w.t0 + s * p.tok_tile;
-      if (a < w.len_q)
-        tiles[s] = (reach_of(p, w, min(a + p.tok_tile, w.len_q) - 1) + TILE_N - 1) / TILE_N;
+  for (int d = 16; d > 0; d >>= 1) line += __shfl_xor_sync(0xffffffffu, line, d);
+  const int room = p.ctas - p.items, most = 1 << 24;
+  // no shorter than an SM's share of the line: that would only add starts
+  int low = static_cast<int>(min((line + p.sms - 1) / p.sms, static_cast<int64_t>(most)));
+  int even = max(static_cast<int>(min((line + room - 1) / room, static_cast<int64_t>(most))), low);
+  while (low < even) {                                  // (only with fewer items than SMs; few steps)
+    const int mid = (low + even) / 2;
+    uint32_t count = 0;
+    for (int s0 = 0; s0 < p.b; s0 += 32) {
+      if (p.b > 32) fetch(s0);
+      count += static_cast<uint32_t>(min(static_cast<int64_t>(items) * parts_of(mid), static_cast<int64_t>(p.ctas) + 1));
     }
+    if (__reduce_add_sync(0xffffffffu, count) <= static_cast<uint32_t>(p.ctas)) even = mid;
+    else low = mid + 1;
   }
-  const int total = max(tiles[0], tiles[1]);
-  int end = total;
-  w.first = 0;
-  if (RANGES) {
-    const int per = (total + p.n_splits - 1) / p.n_splits;
-    w.first = min(split * per, total);
-    end = min(w.first + per, total);
-  }
-  w.tiles = end - w.first;
+  int64_t before = 0;                                   // CTAs of the sequences before s0
+  w.any = false;
+  for (int s0 = 0; s0 < p.b && !w.any; s0 += 32) {
+    if (p.b > 32) fetch(s0);
+    const int parts = parts_of(even), per = (tiles + parts - 1) / parts;
+    const int64_t mine = static_cast<int64_t>(items) * parts;
+    int64_t sum = mine;
 #pragma unroll
-  for (int s = 0; s < 2; ++s) w.count[s] = max(min(tiles[s], end) - w.first, 0);
-  w.twin = RANGES && w.t0 + p.tok_tile >= w.len_q;
-  if (w.twin) {
-    w.count[0] = (w.tiles + 1) / 2;
-    w.count[1] = w.tiles / 2;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += o;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, before + sum > block);
+    if (hit != 0) {
+      const int from = __ffs(hit) - 1;
+      const int r = block - static_cast<int>(before + __shfl_sync(0xffffffffu, sum - mine, from));
+      const int n = __shfl_sync(0xffffffffu, parts, from), len = __shfl_sync(0xffffffffu, per, from);
+      w.q0 = __shfl_sync(0xffffffffu, q0, from);
+      w.len_q = __shfl_sync(0xffffffffu, len_q, from);
+      w.k0 = __shfl_sync(0xffffffffu, k0, from);
+      w.len_k = __shfl_sync(0xffffffffu, len_k, from);
+      w.split = r % n;
+      w.chunk = r / n % p.chunks;
+      w.t0 = r / n / p.chunks * span;
+      w.last_set = w.split == n - 1 ? 2 * n : 2 * p.n_splits;
+      w.any = true;
+      set_tiles<true>(p, w, w.split * len, w.split * len + len);
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
   }
-  w.look = reach_of(p, w, w.t0) / TILE_N;
   return w;
 }
 
@@ -319,11 +409,9 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     tma_prefetch_map(lane == 0 ? &p.mq : lane == 1 ? &p.mk : &p.mv);
   }
   grid_dependency_wait();
-  // Slots last to first: in a causal sequence the late rows are the long ones.
-  const int chunk = blockIdx.x % p.chunks;
-  const int slot = p.slots - 1 - static_cast<int>(blockIdx.x / p.chunks);
-  const int split = blockIdx.z;
-  const Work w = find_work<RANGES>(p, slot, split);
+  Work w;
+  if constexpr (RANGES) w = find_range(p, blockIdx.x);
+  else w = find_work(p, blockIdx.x);
   const bool twin = RANGES && w.twin;
   auto give_back = [&]() {                // TMEM of a CTA that leaves before the others have seen it
     if (warp != WARP_LOOK) return;
@@ -336,7 +424,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     give_back();
     return;
   }
-  const int head0 = chunk * p.pack;
+  const int head0 = w.chunk * p.pack;
   const int kvh = head0 / (p.h_q / p.h_kv);
   const int n_tiles = w.tiles;
 
@@ -348,8 +436,8 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
       const int64_t t = w.q0 + tok;
       float f;
       if (RANGES) {                       // (a set without weight: its values are not read)
-        store_stats(p, 2 * split, t, h, -INFINITY, -INFINITY, 0.f, false, f);
-        store_stats(p, 2 * split + 1, t, h, -INFINITY, -INFINITY, 0.f, false, f);
+        for (int set = 2 * w.split; set < 2 * w.split + 2; ++set) store_stats(p, set, t, h, -INFINITY, -INFINITY, 0.f, false, f);
+        for (int set = w.last_set; set < 2 * p.n_splits; ++set) store_stats(p, set, t, h, -INFINITY, -INFINITY, 0.f, false, f);
       } else {
         store_stats(p, 0, t, h, -INFINITY, -INFINITY, 0.f, false, f);
         uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + t * p.stride_o_t + h * p.stride_o_h);
@@ -670,11 +758,13 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   const bool fail = !ok || *reinterpret_cast<volatile int*>(&ctrl.fail) != 0;
   const int64_t t = static_cast<int64_t>(w.q0) + tok;
   float factor = 0.f;
-  const int set = RANGES ? 2 * split + (twin ? s : 0) : 0;
+  const int set = RANGES ? 2 * w.split + (twin ? s : 0) : 0;
   if (live) {
     store_stats(p, set, t, h, m_raw, m_ref, l, fail, factor);
     float none;
     if (RANGES && !twin) store_stats(p, set + 1, t, h, -INFINITY, -INFINITY, 0.f, false, none);
+    if (RANGES && (!twin || s == 0))
+      for (int k = w.last_set; k < 2 * p.n_splits; ++k) store_stats(p, k, t, h, -INFINITY, -INFINITY, 0.f, false, none);
   }
   const bool nothing = m_ref == -INFINITY && l == l;
   const bool bad = *reinterpret_cast<volatile int*>(&ctrl.bad) != 0;
@@ -782,7 +872,8 @@ dense_combine_kernel(const __grid_constant__ DenseParams p) {
   const float* src = p.o_accum + item * DV + lane * PER;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    for (int s0 = 32 * k; s0 < min(sets, 32 * k + 32); s0 += 8) {
+    const int used = 32 - __clz(__ballot_sync(0xffffffffu, w[k] != 0.f));      // sets up to the last with weight
+    for (int s0 = 32 * k; s0 < 32 * k + used; s0 += 8) {
       float v[8][PER], ws[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -840,7 +931,7 @@ cudaError_t launch_one(const DenseParams& p, cudaStream_t st) {
     }
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.slots) * p.chunks, 1, p.n_splits);
+  cfg.gridDim = dim3(static_cast<unsigned>(RANGES ? p.ctas : p.items));
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -875,7 +966,11 @@ int64_t dense_ctas(int t_q, int b, int h_q, int h_kv) {
   return (static_cast<int64_t>(t_q) / (2 * (TILE_M / pack)) + b) * (h_q / pack);
 }
 
-cudaError_t launch_dense_prefill(const Dsv4DensePrefillArgs& a, cudaStream_t st) {
+// CTAs of a launch with ranges: one for every SM, or twice the uncut ones where those alone are
+// more than half of the SMs.
+int64_t dense_range_ctas(int64_t ctas, int num_sms) { return 2 * ctas > num_sms ? 2 * ctas : num_sms; }
+
+cudaError_t launch_dense_prefill(const Dsv4DensePrefillArgs& a, int num_sms, cudaStream_t st) {
   DenseParams p;
   const bool bf16 = a.dtype == DSV4_DTYPE_BF16;
   p.b = a.b; p.t_q = a.t_q; p.t_k = a.t_k; p.h_q = a.h_q; p.h_kv = a.h_kv; p.causal = a.causal;
@@ -884,6 +979,9 @@ cudaError_t launch_dense_prefill(const Dsv4DensePrefillArgs& a, cudaStream_t st)
   p.chunks = a.h_q / p.pack;
   p.slots = a.t_q / (2 * p.tok_tile) + a.b;
   p.n_splits = a.n_splits;
+  p.items = p.slots * p.chunks;
+  p.sms = num_sms;
+  p.ctas = static_cast<int>(dense_range_ctas(p.items, num_sms));
   p.sm_scale = a.sm_scale;
   p.cu_q = a.cu_seqlens_q; p.cu_k = a.cu_seqlens_k; p.sink = a.attn_sink;
   p.v = a.v; p.stride_v_t = a.stride_v_t; p.stride_v_h = a.stride_v_h;

@@ -338,9 +338,9 @@ int dsv4_shared_prefix_scratch(const Dsv4SharedPrefixArgs* args, int num_sms, in
  * (d_qk, d_v) is (64, 64), (128, 128) or (192, 128); q, k, v, out of one type.  Strides are
  * in elements, multiples of 8, positive (k and v of several tokens or heads cannot be
  * broadcast views); pointers are 16-byte aligned; the last dimension is dense.  sm_scale is
- * positive and at most 1e38.  n_splits > 1 cuts every sequence's keys into that many ranges and
- * needs o_accum [2 n_splits, t_q, h_q, d_v] (32-byte aligned) and stat_accum
- * [2 n_splits, t_q, h_q, 2].                                                                */
+ * positive and at most 1e38.  n_splits > 1 cuts the sequences' keys into ranges of about the
+ * same length, no sequence into more than n_splits (64 at most), and needs o_accum
+ * [2 n_splits, t_q, h_q, d_v] (32-byte aligned) and stat_accum [2 n_splits, t_q, h_q, 2].  */
 enum Dsv4Dtype { DSV4_DTYPE_BF16 = 0, DSV4_DTYPE_FP16 = 1 };
 typedef struct Dsv4DensePrefillArgs {
   int32_t b, t_q, t_k, h_q, h_kv, d_qk, d_v;
@@ -365,8 +365,9 @@ typedef struct Dsv4DensePrefillArgs {
 
 int dsv4_dense_prefill(const Dsv4DensePrefillArgs* args, void* cuda_stream);
 
-/* Key ranges for a dense prefill: a pure function of sizes and the SM count (stable under
- * graph capture); more than one only when the query rows alone leave SMs idle.             */
+/* n_splits for a dense prefill: a pure function of sizes and the SM count (stable under
+ * graph capture); more than one where the query rows alone would leave SMs idle, or are so
+ * few that cutting costs little and evens out sequences of different lengths.              */
 int dsv4_plan_dense_splits(int t_q, int t_k, int b, int h_q, int h_kv, int num_sms);
 
 /* ---------------------------------------------------------------------------

@@ -47,7 +47,7 @@ def test_entry_refuses_no_arguments_and_the_layout_of_the_block():
 def test_split_plan():
     plan = N.lib.dsv4_plan_dense_splits
     assert plan(8192, 8192, 1, 16, 16, 148) == 1                 # the rows fill the GPU
-    assert 1 < plan(8, 8 * 8192, 8, 32, 8, 148) <= 8             # 64 CTAs
+    assert 1 < plan(8, 8 * 8192, 8, 32, 8, 148) <= 148 // 8      # 8 chunks of heads
     assert plan(1, 100000, 1, 8, 8, 148) > 8                     # one token over a long context
     assert plan(1, 200, 1, 8, 8, 148) == 1                       # too short to cut
     for bad in ((0, 1, 1, 1, 1, 148), (1, 0, 1, 1, 1, 148), (1, 1, 0, 1, 1, 148), (1, 1, 1, 3, 2, 148), (1, 1, 1, 1, 1, 0)):

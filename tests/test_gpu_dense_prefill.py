@@ -137,6 +137,28 @@ def test_single_tokens_and_key_ranges(n_splits, d_qk, d_v):
     run(q, k, v, lq, lk, causal=False, n_splits=n_splits)
 
 
+@pytest.mark.parametrize("b", [31, 32, 33, 70, 300])
+@pytest.mark.parametrize("n_splits", [None, 2, 9, 64])
+def test_ranges_of_many_uneven_sequences(b, n_splits):
+    """More sequences than a warp has lanes; one of them holds most of the keys."""
+    lq = [(0, 1, 1, 2, 1)[r % 5] for r in range(b)]
+    lk = [(r * 37) % 400 if r != b - 2 else 9000 for r in range(b)]
+    q, k, v = make(lq, lk, 4, 1, 64, 64, BF16, seed=b)
+    run(q, k, v, lq, lk, n_splits=n_splits)
+
+
+@pytest.mark.parametrize("n_splits", [None, 6])
+def test_ranges_with_bounds_that_do_not_cover_the_tensors(n_splits):
+    """Rows of no sequence stay as they are; bounds beyond the tensors are clamped."""
+    q, k, v = make([40], [5000], 8, 2, 128, 128, BF16, seed=8)
+    cq, ck = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([3, 4, 6], [10, 2000, 1 << 30]))
+    out = torch.full_like(q, 7.0)
+    got = K.dense_prefill_fwd(q, k, v, cq, ck, 0.1, True, None, out, n_splits=n_splits)
+    check((got[0][3:6], got[1][3:6], got[2][3:6]),
+          definition(q[3:6], k[10:], v[10:], [1, 2], [1990, 3000], 0.1, True, None), BF16)
+    assert (out[:3] == 7).all() and (out[6:] == 7).all()
+
+
 def test_key_ranges_of_long_rows():
     lq, lk = [300, 17], [1300, 900]
     q, k, v = make(lq, lk, 6, 3, 128, 128, BF16, seed=6)
