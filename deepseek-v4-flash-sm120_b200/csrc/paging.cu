@@ -11,11 +11,14 @@
 // itself (8 B a request out of L2, cheaper than a second launch or a grid-wide hand-over),
 // keeps both sums in shared memory and finds its tokens' requests by bisection there.  A new
 // page's id comes from the free list in both places that need it (its table entry and its
-// tokens' slots), so no CTA reads an entry another one writes.
+// tokens' slots), so no CTA reads an entry another one writes.  Measured: 64 requests of one token
+// 2.7 us in a graph; 301 prompts of 1 to 2048 tokens: 7 us from cold caches (launch, and four
+// dependent reads of about 0.8 us).
 //
 // page_indices_kernel.  slot = table[r][pos / P] * P + pos % P per list entry: 4 B in, 4 B
 // out, bound by memory for prefill lists.  16-byte loads and stores where rows allow, the
-// division by a multiplication prepared on the host.
+// division by a multiplication prepared on the host.  Measured: 8192 x 2048 entries 23.7 us,
+// 5.7 TB/s (0.87 of a copy's rate); 64 x 2048 entries 2.7 us in a graph.
 #include <mutex>
 
 #include "attn_params.cuh"
