@@ -569,7 +569,7 @@ int dsv4_dense_prefill(const Dsv4DensePrefillArgs* a, void* stream) {
   if (!a) return DSV4_ERR_NULL;
   if (a->b < 0 || a->t_q < 0 || a->t_k < 0 || a->h_q < 1 || a->h_kv < 1 || a->h_q % a->h_kv ||
       a->n_splits < 1 || a->n_splits > dsv4::DENSE_MAX_SPLITS || !(a->sm_scale > 0.0f) ||
-      !(a->sm_scale <= 1.0e38f) || dsv4::dense_ctas(a->t_q, a->b, a->h_q, a->h_kv) > 0x3fffffff)
+      !(a->sm_scale <= 1.0e38f) || dsv4::dense_ctas(a->t_q, a->b, a->h_q, a->h_kv) > (a->n_splits > 1 ? 1 << 24 : 0x7fffffff))
     return DSV4_ERR_SHAPE;
   if (!((a->d_qk == 64 && a->d_v == 64) || (a->d_qk == 128 && a->d_v == 128) ||
         (a->d_qk == 192 && a->d_v == 128)))

@@ -37,8 +37,9 @@
 // PFLOP/s of the products that are not masked (0.76 of a matrix product's rate), 327 us under the
 // power limit; tensor pipe 64 % busy, bound by the 128 exponentials, sums and conversions of
 // each thread and tile beside it.  Packed prompts, 24 heads on 4, (128, 128): 253 us and 55 %.
-// Single tokens, 8 contexts of 1000 to 16383, 32 heads on 8: 28 us for 99 MB (3.6 TB/s), of
-// which 5 us are the start and the end of a CTA.
+// Single tokens, 8 contexts of 1000 to 16383, 32 heads on 8: 18 us a CTA for 99 MB, of which 13 us
+// stream at memory's rate (with one unit of V less for twins 17) and 5 are its start and end; 31 us
+// with the joining launch.
 #include <cuda_fp16.h>
 
 #include <mutex>
@@ -79,24 +80,39 @@ template <int DQK, int DV> struct DCfg {
   static constexpr int K_SLOTS = DQK == 192 ? 4 : DQK == 128 ? 6 : 4;   // blocks of 64 columns
   static constexpr int K_STEP = DQK == 192 ? 1 : QB;      // blocks handed over together
   static constexpr int K_RING = K_SLOTS / K_STEP;
-  static constexpr int V_UNITS = DQK == 64 ? 4 : 2;                     // whole tiles
+  static constexpr int V_UNITS = DQK == 64 ? 4 : 2;                     // whole tiles; twins have one more
   // TMEM columns: O_s (d_v each), P_s (64 each), and what is left for scores: one tile that the
   // row tiles use in turn at d_v = 128, one each at d_v = 64.
   static constexpr int S_BUFS = DV == 64 ? 2 : 1;
   static constexpr uint32_t COL_S = 0, COL_P = 128 * S_BUFS, COL_O = COL_P + 128;
   static_assert(COL_O + 2 * DV <= TMEM_COLS, "512 columns");
+  static_assert(V_UNITS <= 4 && VB <= QB, "a unit fits where the second Q tile would be");
   static constexpr int Q_BYTES = 2 * QB * BLOCK_BYTES, K_BYTES = K_SLOTS * BLOCK_BYTES;
   static constexpr int V_UNIT_BYTES = VB * BLOCK_BYTES, V_BYTES = V_UNITS * V_UNIT_BYTES;
 };
 
+// The part of a sequence that a CTA works on.
+struct Work {
+  int q0, len_q, k0, len_k;      // rows of the packed tensors
+  int t0;                        // first query token of row tile 0, in the sequence
+  int first, tiles;              // key tiles [first, first + tiles)
+  int count[2];                  // of them row tile s takes the first count[s] ...
+  bool twin;                     // ... or, both row tiles being the same, every second one from s on
+  int look;                      // key tiles from this one on are seen only in part by some row
+  bool any;
+  int chunk, split;              // heads, range
+  int last_set;                  // partial sets from here on are not written: this CTA marks them
+};
+
 struct DenseCtrl {
   uint64_t q_full[2], s_full[2], s_free[2], p_full[2], o_done[2];
-  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
+  uint64_t k_full[4], k_empty[4], v_full[5], v_empty[5];
   // tiles that are looked over (the last ones) land on v_look instead of v_full, so that the
   // looking warps count only their own phases; v_clean hands them on
-  uint64_t v_look[4], v_clean[4];
+  uint64_t v_look[5], v_clean[5];
   uint32_t tmem;
   int fail, bad;
+  Work work;                     // with ranges: what the loading warp has found
 };
 
 template <int DQK, int DV> constexpr size_t dense_smem_bytes() {
@@ -182,19 +198,6 @@ __device__ __forceinline__ uint32_t abs_max2(uint32_t a, uint32_t b) {
   return d;
 }
 
-// The part of a sequence that a CTA works on.
-struct Work {
-  int q0, len_q, k0, len_k;      // rows of the packed tensors
-  int t0;                        // first query token of row tile 0, in the sequence
-  int first, tiles;              // key tiles [first, first + tiles)
-  int count[2];                  // of them row tile s takes the first count[s] ...
-  bool twin;                     // ... or, both row tiles being the same, every second one from s on
-  int look;                      // key tiles from this one on are seen only in part by some row
-  bool any;
-  int chunk, split;              // heads, range
-  int last_set;                  // partial sets from here on are not written: this CTA marks them
-};
-
 // Keys of the sequence that token t sees: [0, reach).
 __device__ __forceinline__ int reach_of(const DenseParams& p, const Work& w, int t) {
   if (!p.causal) return w.len_k;
@@ -275,6 +278,12 @@ __device__ __forceinline__ Work find_work(const DenseParams& p, int block) {
   return w;
 }
 
+__device__ __forceinline__ float root(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // With ranges: the sequences are cut into ranges of about the same length, so that the grid ends
 // evenly whatever their lengths: the shortest length with which the launch's CTAs are enough (and
 // they are for line / (ctas - items) tiles, line being the sum of all items' tiles, since rounding
@@ -296,46 +305,50 @@ __device__ __forceinline__ Work find_range(const DenseParams& p, int block) {
     len_k = clamp_to(d, k0, p.t_k) - k0;
     items = (len_q + span - 1) / span * p.chunks;
     tiles = (len_k + TILE_N - 1) / TILE_N;
-    shortest = max(max((tiles + p.n_splits - 1) / p.n_splits, static_cast<int>(ceilf(sqrtf(0.6f * tiles)))), 1);
+    shortest = max(static_cast<int>(ceilf(root(0.6f * tiles))), 1);
   };
+  // ceil(tiles / per), or a little less beyond 2^18 tiles, but never more: the factor outweighs what
+  // the quick division can be off
   auto parts_of = [&](int even) {
     const int per = max(even, shortest);
-    return max((tiles + per - 1) / per, 1);
+    return clamp_to(static_cast<int>(__fdividef(tiles + (per - 0.5f), per) * (1.f - 0x1p-20f)), 1, p.n_splits);
   };
-  int64_t line = 0;
+  // the line's length in floating point (64-bit divisions took a third of the time); the margin
+  // covers its roundings, so that `even` is never too short
+  float line = 0.f;
   for (int s0 = 0; s0 < p.b; s0 += 32) {
     fetch(s0);
-    line += static_cast<int64_t>(items) * tiles;
+    line += static_cast<float>(items) * static_cast<float>(tiles);
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) line += __shfl_xor_sync(0xffffffffu, line, d);
-  const int room = p.ctas - p.items, most = 1 << 24;
+  line *= 1.f + 0x1p-16f;
   // no shorter than an SM's share of the line: that would only add starts
-  int low = static_cast<int>(min((line + p.sms - 1) / p.sms, static_cast<int64_t>(most)));
-  int even = max(static_cast<int>(min((line + room - 1) / room, static_cast<int64_t>(most))), low);
+  int low = static_cast<int>(fminf(ceilf(line / p.sms), 0x1p24f));
+  int even = max(static_cast<int>(fminf(ceilf(line / (p.ctas - p.items)), 0x1p24f)), low);
   while (low < even) {                                  // (only with fewer items than SMs; few steps)
     const int mid = (low + even) / 2;
     uint32_t count = 0;
     for (int s0 = 0; s0 < p.b; s0 += 32) {
       if (p.b > 32) fetch(s0);
-      count += static_cast<uint32_t>(min(static_cast<int64_t>(items) * parts_of(mid), static_cast<int64_t>(p.ctas) + 1));
+      count += min(static_cast<uint32_t>(items * parts_of(mid)), static_cast<uint32_t>(p.ctas) + 1);
     }
     if (__reduce_add_sync(0xffffffffu, count) <= static_cast<uint32_t>(p.ctas)) even = mid;
     else low = mid + 1;
   }
-  int64_t before = 0;                                   // CTAs of the sequences before s0
+  uint32_t before = 0;                                  // CTAs of the sequences before s0
   w.any = false;
   for (int s0 = 0; s0 < p.b && !w.any; s0 += 32) {
     if (p.b > 32) fetch(s0);
     const int parts = parts_of(even), per = (tiles + parts - 1) / parts;
-    const int64_t mine = static_cast<int64_t>(items) * parts;
-    int64_t sum = mine;
+    const uint32_t mine = min(static_cast<uint32_t>(items * parts), static_cast<uint32_t>(p.ctas));
+    uint32_t sum = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int64_t o = __shfl_up_sync(0xffffffffu, sum, d);
+      const uint32_t o = __shfl_up_sync(0xffffffffu, sum, d);
       if (lane >= d) sum += o;
     }
-    const uint32_t hit = __ballot_sync(0xffffffffu, before + sum > block);
+    const uint32_t hit = __ballot_sync(0xffffffffu, before + sum > static_cast<uint32_t>(block));
     if (hit != 0) {
       const int from = __ffs(hit) - 1;
       const int r = block - static_cast<int>(before + __shfl_sync(0xffffffffu, sum - mine, from));
@@ -400,6 +413,8 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
       for (int i = 0; i < 4; ++i) {
         mbar_init(bar(&ctrl.k_full[i]), 1);
         mbar_init(bar(&ctrl.k_empty[i]), 1);
+      }
+      for (int i = 0; i < 5; ++i) {
         mbar_init(bar(&ctrl.v_full[i]), 1);
         mbar_init(bar(&ctrl.v_empty[i]), 1);
         mbar_init(bar(&ctrl.v_look[i]), 1);
@@ -417,9 +432,22 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   }
   grid_dependency_wait();
   Work w;
-  if constexpr (RANGES) w = find_range(p, blockIdx.x);
-  else w = find_work(p, blockIdx.x);
+  if constexpr (RANGES) {          // one warp looks: twelve would share four schedulers
+    if (warp == WARP_TMA) {
+      w = find_range(p, blockIdx.x);
+      if (lane == 0) ctrl.work = w;
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    w = ctrl.work;
+  } else {
+    w = find_work(p, blockIdx.x);
+  }
   const bool twin = RANGES && w.twin;
+  // twins share a Q tile; in the place of the second one they have one more unit of V
+  const int v_units = twin ? C::V_UNITS + 1 : C::V_UNITS;
+  auto v_at = [&](int vu) { return RANGES && vu == C::V_UNITS ? sQ + C::QB * BLOCK_BYTES : sV + vu * C::V_UNIT_BYTES; };
   auto give_back = [&]() {                // TMEM of a CTA that leaves before the others have seen it
     if (warp != WARP_LOOK) return;
     tc_fence_before_sync();
@@ -455,9 +483,11 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     return;
   }
 
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
+  if (!RANGES) {
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+  }
   const uint32_t tmem = ctrl.tmem;
   // A role whose bounded wait gives up records it and ends; the others then run into their
   // own limits, long after every copy and product in flight has finished.
@@ -476,7 +506,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
           mbar_expect_tx(bar(&ctrl.q_full[s]), q_bytes * C::QB);
           for (int c = 0; c < C::QB; ++c)
             tma_load_3d(sQ + (s * C::QB + c) * BLOCK_BYTES, &p.mq, 64 * c, head0,
-                        w.q0 + w.t0 + (twin ? 0 : s * p.tok_tile), bar(&ctrl.q_full[s]));
+                        w.q0 + w.t0 + s * p.tok_tile, bar(&ctrl.q_full[s]));
         };
         if (w.count[0] > 0) load_q(0);
         bool ok = true;
@@ -490,13 +520,13 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
               tma_load_3d(sK + (ks * C::K_STEP + d) * BLOCK_BYTES, &p.mk, 64 * (c + d), kvh, row, bar(&ctrl.k_full[ks]));
             if (++ks == C::K_RING) { ks = 0; kphase ^= 1; }
           }
-          if (i == 0 && w.count[1] > 0) load_q(1);
+          if (i == 0 && w.count[1] > 0 && !twin) load_q(1);
           if (!ok || !mbar_wait_fast(bar(&ctrl.v_empty[vu]), vphase ^ 1)) { gave_up(ERR_SLOT); break; }
           const uint32_t landed = bar(w.first + i >= w.look ? &ctrl.v_look[vu] : &ctrl.v_full[vu]);
           mbar_expect_tx(landed, C::V_UNIT_BYTES);
           for (int c = 0; c < C::VB; ++c)
-            tma_load_3d(sV + vu * C::V_UNIT_BYTES + c * BLOCK_BYTES, &p.mv, 64 * c, kvh, row, landed);
-          if (++vu == C::V_UNITS) { vu = 0; vphase ^= 1; }
+            tma_load_3d(v_at(vu) + c * BLOCK_BYTES, &p.mv, 64 * c, kvh, row, landed);
+          if (++vu == v_units) { vu = 0; vphase ^= 1; }
         }
       }
       __syncwarp();
@@ -534,7 +564,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
             if (!takes(s, i) || !ok) continue;
             const bool last = twin || s == 1 || i >= count1;     // nobody reads the tile's K after this
             const int j = nth(i);
-            if (j == 0) wait(&ctrl.q_full[s], 0, ERR_Q);
+            if (j == 0) wait(&ctrl.q_full[twin ? 0 : s], 0, ERR_Q);
             // the scores that were here have been read
             if (C::S_BUFS == 1) wait(&ctrl.s_free[0], (turn & 1) ^ 1, ERR_FREE);
             else wait(&ctrl.s_free[s], (j & 1) ^ 1, ERR_FREE);
@@ -549,7 +579,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
               const uint64_t d = dK + ((ks * C::K_STEP * BLOCK_BYTES) >> 4);
 #pragma unroll
               for (int k = 0; k < 4 * C::K_STEP; ++k)
-                umma_bf16_elect(tS, dQ + (((s * C::QB + c + (k >> 2)) * BLOCK_BYTES + (k & 3) * 32) >> 4),
+                umma_bf16_elect(tS, dQ + ((((twin ? 0 : s) * C::QB + c + (k >> 2)) * BLOCK_BYTES + (k & 3) * 32) >> 4),
                                 d + (((k >> 2) * BLOCK_BYTES + (k & 3) * 32) >> 4), idesc, (c | k) != 0, elected);
               if (last) umma_commit_elect(bar(&ctrl.k_empty[ks]), elected);
               if (++ks == C::K_RING) { ks = 0; kphase ^= 1; }
@@ -560,11 +590,13 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
       } else {
         constexpr uint32_t idesc = make_idesc_16(BF16, TILE_M, DV, 0, 1);
         const uint64_t dV = make_smem_desc(sV, BLOCK_BYTES, 1024, SWZ_128B);   // MN-major
+        const uint64_t dV_more = make_smem_desc(sQ + C::QB * BLOCK_BYTES, BLOCK_BYTES, 1024, SWZ_128B);
+        const int units = twin ? C::V_UNITS + 1 : C::V_UNITS;
         uint32_t clean_parity = 0;
 #pragma unroll 1
         for (int i = 0; i < tiles && ok; ++i) {
-          const int vu = i % C::V_UNITS, vphase = (i / C::V_UNITS) & 1;
-          const uint64_t d = dV + ((vu * C::V_UNIT_BYTES) >> 4);
+          const int vu = i % units, vphase = (i / units) & 1;
+          const uint64_t d = RANGES && vu == C::V_UNITS ? dV_more : dV + ((vu * C::V_UNIT_BYTES) >> 4);
           if (w.first + i >= w.look) {
             wait(&ctrl.v_clean[vu], (clean_parity >> vu) & 1, ERR_LOOK);
             clean_parity ^= 1u << vu;
@@ -593,7 +625,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
       const int seen = reach_of(p, w, min(w.t0 + 2 * p.tok_tile, w.len_q) - 1);
       uint32_t parity = 0;
       for (int i = max(w.look - w.first, 0); i < n_tiles; ++i) {
-        const int vu = i % C::V_UNITS;
+        const int vu = i % v_units;
         if (!mbar_wait_fast(bar(&ctrl.v_look[vu]), (parity >> vu) & 1)) {
           if (lane == 0) gave_up(ERR_V);
           break;
@@ -602,7 +634,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
         const int live = min(seen - (w.first + i) * TILE_N, TILE_N);   // rows of the tile that count
         // 32 chunks of 16 bytes (four rows of a block) at a time
         constexpr int BATCH = 8;
-        const uint32_t mine = sV + vu * C::V_UNIT_BYTES + lane * 16;
+        const uint32_t mine = v_at(vu) + lane * 16;
         uint32_t most = 0;                           // largest magnitude, pairwise; NaN stays
         for (int c0 = 0; c0 < C::V_UNIT_BYTES / 512; c0 += BATCH) {
           uint32_t x[BATCH][4];
