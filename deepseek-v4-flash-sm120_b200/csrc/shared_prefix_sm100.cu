@@ -576,8 +576,10 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
         if (w.last)
           for (int s = w.set + 1; s < p.sets; ++s) p.lse_accum[static_cast<int64_t>(s) * p.rows + row] = -INFINITY;
       }
-      // each group writes the 256 columns of one product
-      float* dst = p.o_accum + (static_cast<int64_t>(w.set) * p.rows + row) * D_V + group * 256 + half * 128;
+      // Each group writes the 256 columns of one product.  Four lanes exchange the blocks of 8
+      // columns of their rows first, so that they write 128 bytes of each row in turn.
+      const int j = lane & 3;
+      float* dst = p.o_accum + (static_cast<int64_t>(w.set) * p.rows + row - j) * D_V + group * 256 + half * 128 + 8 * j;
 #pragma unroll 1
       for (int k = 0; k < 4; ++k) {
         uint32_t o[32];
@@ -588,13 +590,28 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
           __syncwarp();
           if (lane == 0) arrive_leader(bar(&ctrl.o_free));
         }
-        if (row < p.rows && !fail) {
 #pragma unroll
-          for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
+        for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
+        // block i of lane j <-> block j of lane i
 #pragma unroll
-          for (int q = 0; q < 32; q += 8)
-            st_global_32(dst + 32 * k + q, o[q], o[q + 1], o[q + 2], o[q + 3], o[q + 4], o[q + 5], o[q + 6], o[q + 7]);
+        for (int bit = 1; bit < 4; bit <<= 1) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (i & bit) continue;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const bool up = (j & bit) != 0;
+              const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? o[8 * i + q] : o[8 * (i | bit) + q], bit);
+              if (up) o[8 * i + q] = got;
+              else o[8 * (i | bit) + q] = got;
+            }
+          }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (row - j + i < p.rows && !fail)
+            st_global_32(dst + i * D_V + 32 * k, o[8 * i], o[8 * i + 1], o[8 * i + 2], o[8 * i + 3], o[8 * i + 4],
+                         o[8 * i + 5], o[8 * i + 6], o[8 * i + 7]);
       }
     }
     // blocks without any tile: nobody else marks the sets of their rows
