@@ -577,7 +577,8 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
           for (int s = w.set + 1; s < p.sets; ++s) p.lse_accum[static_cast<int64_t>(s) * p.rows + row] = -INFINITY;
       }
       // Each group writes the 256 columns of one product.  Four lanes exchange the blocks of 8
-      // columns of their rows first, so that they write 128 bytes of each row in turn.
+      // columns of their rows first, so that they write 128 bytes of each row in turn (32 bytes at
+      // 32 places took 8200 clk a segment; 16 requests 80 us, with this 77).
       const int j = lane & 3;
       float* dst = p.o_accum + (static_cast<int64_t>(w.set) * p.rows + row - j) * D_V + group * 256 + half * 128 + 8 * j;
 #pragma unroll 1

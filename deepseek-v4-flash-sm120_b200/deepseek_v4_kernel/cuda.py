@@ -36,7 +36,8 @@ def _ptr(t: Optional[torch.Tensor]):
 
 # The serving operators below are called for a few microseconds of GPU work each, so their host
 # cost counts: checks that build no message unless they fail, no context for the current device,
-# and the stream as the plain handle.
+# the stream as the plain handle, and sizes as plain arguments of `new_empty` (a tuple of them
+# takes 0.4 us longer; two small tensors 1 us less than one and its views).
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
@@ -271,8 +272,8 @@ def sparse_prefill_fwd_fp8(q, kv, indices, sm_scale, d_v=512, attn_sink=None, to
 def shared_prefix_decode_fwd(q, kv, prefix_table, prefix_length, block_table, suffix_length, attn_sink, d_v,
                              sm_scale, *, prefix_splits: int = 0, suffix_splits: int = 0, flags: int = 0):
     """Decode of a batch whose requests share a long prefix: the prefix is attended once for
-    the rows of all requests together, every request's own tokens separately, and the two
-    parts are joined by their log-sum-exps.
+    the rows of all requests together, and joined with every request's own tokens by their
+    log-sum-exps.
 
       q [b, s_q, h_q, d_qk] bf16 (contiguous); kv [num_blocks, page_block, 1, bytes]
       fp8/uint8/int8 as for `sparse_decode_fwd`; prefix_table [prefix_pages] int32 and
@@ -284,7 +285,8 @@ def shared_prefix_decode_fwd(q, kv, prefix_table, prefix_length, block_table, su
     Query token s sees the whole prefix and suffix_length - (s_q - 1 - s) own tokens.  A row
     that sees nothing gives out 0 and lse = its sink, or -inf.  Tokens on pages outside the
     cache are masked.  The lengths stay on the device, so a captured call can be replayed
-    with others.  `prefix_splits` / `suffix_splits` / `flags` are test hooks.  No counterpart
+    with others; the scratch grows with what the two tables can hold, so they should be no
+    wider than needed.  `prefix_splits` / `suffix_splits` / `flags` are test hooks.  No counterpart
     in the reference."""
     if not (q.is_cuda and kv.get_device() == q.get_device()):
         raise RuntimeError("q and kv must be CUDA tensors of one device")
@@ -310,8 +312,8 @@ def shared_prefix_decode_fwd(q, kv, prefix_table, prefix_length, block_table, su
     if attn_sink is not None and not (attn_sink.dtype == torch.float32 and attn_sink.numel() == h_q
                                       and attn_sink.is_contiguous() and attn_sink.get_device() == idx):
         raise RuntimeError("attn_sink must be contiguous float32 [h_q]")
-    out = q.new_empty((b, s_q, h_q, 512))
-    lse = q.new_empty((b, h_q, s_q), dtype=torch.float32)
+    out = q.new_empty(b, s_q, h_q, 512)
+    lse = q.new_empty(b, h_q, s_q, dtype=torch.float32)
     if b == 0:
         return out, lse
     a = N.SharedPrefixArgs()
@@ -325,7 +327,7 @@ def shared_prefix_decode_fwd(q, kv, prefix_table, prefix_length, block_table, su
     # one allocation: partial outputs, their log-sum-exps, workspace
     rows = sets.value * b * s_q * h_q
     lse_at, work_at = rows * 2048, rows * 2048 + (rows * 4 + 255) // 256 * 256
-    scratch = q.new_empty((work_at + nbytes.value,), dtype=torch.uint8)
+    scratch = q.new_empty(work_at + nbytes.value, dtype=torch.uint8)
     at = scratch.data_ptr()
     a.o_accum, a.lse_accum, a.workspace = at, at + lse_at, at + work_at
     a.q, a.kv, a.attn_sink = q.data_ptr(), kv.data_ptr(), _ptr(attn_sink)
@@ -386,8 +388,9 @@ def dense_prefill_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, sm_scale, causal: boo
                                 and out.stride(2) == 1):
         raise RuntimeError("out must be [t_q, h_q, d_v] of q's type, dense in the last dim")
     if out is None:
-        out = q.new_empty((t_q, h_q, d_v))
-    stats = q.new_empty((2, t_q, h_q), dtype=torch.float32)
+        out = q.new_empty(t_q, h_q, d_v)
+    max_logits = q.new_empty(t_q, h_q, dtype=torch.float32)
+    lse = q.new_empty(t_q, h_q, dtype=torch.float32)
     a = N.DensePrefillArgs()
     if n_splits is None:
         n_splits = N.lib.dsv4_plan_dense_splits(t_q, t_k, b, h_q, h_kv, num_sms(q.device))
@@ -395,18 +398,16 @@ def dense_prefill_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, sm_scale, causal: boo
     a.dtype, a.causal, a.n_splits, a.sm_scale = _DENSE_DTYPES[dtype], int(bool(causal)), n_splits, float(sm_scale)
     a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     a.cu_seqlens_q, a.cu_seqlens_k = cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr()
-    at = stats.data_ptr()
-    a.attn_sink, a.max_logits, a.lse = _ptr(attn_sink), at, at + 4 * t_q * h_q
+    a.attn_sink, a.max_logits, a.lse = _ptr(attn_sink), max_logits.data_ptr(), lse.data_ptr()
     if n_splits > 1:
         rows = 2 * n_splits * t_q * h_q          # two partial sets a range
-        scratch = q.new_empty((rows * (d_v + 2),), dtype=torch.float32)
+        scratch = q.new_empty(rows * (d_v + 2), dtype=torch.float32)
         a.o_accum, a.stat_accum = scratch.data_ptr(), scratch.data_ptr() + rows * d_v * 4
     a.stride_q_t, a.stride_q_h, a.stride_k_t, a.stride_k_h = sq[0], sq[1], sk[0], sk[1]
     a.stride_v_t, a.stride_v_h = sv[0], sv[1]
     a.stride_o_t, a.stride_o_h, _ = out.stride()
     a.stride_ml_t = a.stride_lse_t = h_q
     _queue(N.lib.dsv4_dense_prefill, a, idx, "dsv4_dense_prefill")
-    max_logits, lse = stats.unbind(0)
     return out, max_logits, lse
 
 
@@ -489,8 +490,8 @@ def build_slot_maps(block_table, cached_lens, new_lens, free_pages, page_block: 
         raise RuntimeError("page_block >= 1 and n_slots >= 0 expected")
     if b > 16384:
         raise RuntimeError("at most 16384 requests")
-    slots = cached_lens.new_empty((n_slots,), dtype=torch.int64)
-    ints = cached_lens.new_empty((n_slots + 2 * b + 3,))
+    slots = cached_lens.new_empty(n_slots, dtype=torch.int64)
+    ints = cached_lens.new_empty(n_slots + 2 * b + 3)
     a = N.SlotMapArgs()
     a.b, a.max_pages, a.page_block_size, a.n_slots = b, max_pages, page_block, n_slots
     a.n_free = free_pages.numel()
@@ -538,7 +539,7 @@ def page_indices(block_table, positions, page_block: int, cu_seqlens=None) -> to
             raise RuntimeError(f"cu_seqlens must have {b + 1} entries")
         if n_rows > 1:
             stride = positions.stride(0)
-    out = positions.new_empty(positions.shape)
+    out = positions.new_empty(*positions.shape)
     a = N.PageIndicesArgs()
     a.n_rows, a.topk, a.b, a.s_q = n_rows, topk, b, max(s_q, 1)
     a.max_pages, a.page_block_size = max_pages, page_block
