@@ -290,7 +290,7 @@ __device__ __forceinline__ float root(float x) {
 // up costs every item less than one range more).  A range streams a tile in about 1 us and costs
 // 0.6 us to start and join, so below sqrt(0.6 tiles) shorter ranges gain nothing.  (As many ranges
 // for every sequence instead, microseconds: 8 of 1000 to 16383 keys, 32 heads on 8, 5 query tokens
-// each: 47, with this 39; 60 of 1 to 20000 keys, 8 heads of 64: 170 uncut and 100 in two, with this 82.)
+// each: 47, with this 35; 60 of 1 to 20000 keys, 8 heads of 64: 170 uncut and 100 in two, with this 80.)
 __device__ __forceinline__ Work find_range(const DenseParams& p, int block) {
   Work w = {};
   const int span = 2 * p.tok_tile, lane = threadIdx.x & 31;
@@ -313,19 +313,18 @@ __device__ __forceinline__ Work find_range(const DenseParams& p, int block) {
     const int per = max(even, shortest);
     return clamp_to(static_cast<int>(__fdividef(tiles + (per - 0.5f), per) * (1.f - 0x1p-20f)), 1, p.n_splits);
   };
-  // the line's length in floating point (64-bit divisions took a third of the time); the margin
-  // covers its roundings, so that `even` is never too short
+  // the line's length in floating point (64-bit divisions took a third of the time), rounded up so
+  // that `even` is never too short
   float line = 0.f;
   for (int s0 = 0; s0 < p.b; s0 += 32) {
     fetch(s0);
-    line += static_cast<float>(items) * static_cast<float>(tiles);
+    line = __fmaf_ru(static_cast<float>(items), static_cast<float>(tiles), line);
   }
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) line += __shfl_xor_sync(0xffffffffu, line, d);
-  line *= 1.f + 0x1p-16f;
+  for (int d = 16; d > 0; d >>= 1) line = __fadd_ru(line, __shfl_xor_sync(0xffffffffu, line, d));
   // no shorter than an SM's share of the line: that would only add starts
   int low = static_cast<int>(fminf(ceilf(line / p.sms), 0x1p24f));
-  int even = max(static_cast<int>(fminf(ceilf(line / (p.ctas - p.items)), 0x1p24f)), low);
+  int even = max(static_cast<int>(fminf(ceilf(__fdiv_ru(line, p.ctas - p.items)), 0x1p24f)), low);
   while (low < even) {                                  // (only with fewer items than SMs; few steps)
     const int mid = (low + even) / 2;
     uint32_t count = 0;
