@@ -572,7 +572,10 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
       const bool none = total == 0.f;
       const float f = none ? 0.f : 1.f / total;
       if (group == 0 && half == 0 && row < p.rows) {
-        p.lse_accum[static_cast<int64_t>(w.set) * p.rows + row] = fail ? NAN : none ? -INFINITY : logf(total) + ref * LN2;
+        // a row that failed, or is NaN, has to come out NaN whatever else is joined with it: +inf does
+        // so, being the maximum of the sets, where a NaN could be passed over
+        const float lse = logf(total) + ref * LN2;
+        p.lse_accum[static_cast<int64_t>(w.set) * p.rows + row] = fail || lse != lse ? INFINITY : none ? -INFINITY : lse;
         if (w.last)
           for (int s = w.set + 1; s < p.sets; ++s) p.lse_accum[static_cast<int64_t>(s) * p.rows + row] = -INFINITY;
       }

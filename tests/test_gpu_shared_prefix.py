@@ -259,6 +259,16 @@ def test_tokens_that_are_not_finite_reach_the_rows_that_see_them_alone(layout, f
     assert ((lse.double() - want[2]).abs().transpose(1, 2)[fine] <= SCORES + 2e-6 * want[2].abs().transpose(1, 2)[fine]).all()
 
 
+@pytest.mark.parametrize("b", [1, 4, 20])
+def test_a_row_of_one_set_that_is_not_finite(b):
+    """Nothing but the set with the NaN holds tokens; few rows have more than 32 sets."""
+    x = Batch("V32", b, 1, 16, 64, [40] * b, 64, seed=5)
+    x.arena[int(x.table[b - 1, 0]), 39 * (x.d + 128) + x.d:][:2] = 0xff
+    out, lse = x.call(flags=N.FLAG_SHARED_DENSE)
+    assert torch.isnan(out[b - 1]).all() and torch.isnan(lse[b - 1]).all()
+    assert torch.isfinite(out[:b - 1]).all() and torch.isfinite(lse[:b - 1]).all()
+
+
 @pytest.mark.parametrize("form", FORMS[1:])
 @pytest.mark.parametrize("pages", [300, 600])
 def test_wide_tables_of_short_requests(pages, form):
