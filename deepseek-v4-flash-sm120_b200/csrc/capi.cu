@@ -340,16 +340,19 @@ static SharedForm choose_form(const Dsv4SharedPrefixArgs* a, int64_t rows, int64
   if (by_list || plen + slen == 0 || (a->flags & DSV4_FLAG_SHARED_LISTS)) return FORM_LISTS;
   if (plen == 0 || (a->flags & DSV4_FLAG_SHARED_JOINED)) return FORM_JOINED;
   if ((a->flags & DSV4_FLAG_SHARED_DENSE) && dsv4::prefix_attn_fits(*a, false)) return FORM_DENSE;
-  // JOINED up to four tiles of 128 tokens an SM (for blocks of up to 64 rows) and lists of 16384
-  // tokens (microseconds, JOINED / DENSE / LISTS, tokens a request x requests x heads: 2100 x 4 x
-  // 16: 18 / 35 / 33; 2100 x 16 x 64: 27 / 40 / 41; 4100 x 16 x 64, 528 tiles: 37 / 43 / 49;
-  // 20100 x 8 x 8, 1264 tiles: 60 / 43 / 39; 30100 x 1 x 64: 53 / 53 / 43).
+  // JOINED up to 3 tiles of 128 tokens an SM, half as many where they are of more than 32 heads, and
+  // lists of 8000 tokens (microseconds, JOINED / DENSE / LISTS, prefix x query tokens x heads: 2000 x
+  // 4 x 16: 19 / 25 / 35; 512 x 57 x 20, 456 tiles: 21 / 29 / 33; 6000 x 16 x 8, 768 tiles: 41 / 31 /
+  // 35; 2000 x 3 x 64: 23 / 29 / 37; 1088 x 32 x 64, 288 tiles: 39 / 31 / 50; 16000 x 1 x 16: 31 / 26 /
+  // 31).  Over 600 drawn calls of up to 60 requests and 30000 tokens the rules here cost 0.6 % over
+  // the best form of each.
   const int64_t tiles = static_cast<int64_t>(a->b) * a->s_q * ((a->h_q + 63) / 64) * ((plen + slen + 127) / 128);
-  if (tiles <= 4 * num_sms && plen + slen <= 16384) return FORM_JOINED;
-  // LISTS up to 128 rows: converting the whole prefix costs more than reading its FP8 rows twice
-  // (30100 x 4 x 16, 64 rows: 49 DENSE, 41 LISTS; 10100 x 4 x 32: 41 and 39; 4100 x 8 x 64, 512
-  // rows: 39 and 41; 33000 x 64 x 64: 269 and 667).
-  return rows > 128 && dsv4::prefix_attn_fits(*a, false) ? FORM_DENSE : FORM_LISTS;
+  if (tiles * (a->h_q <= 32 ? 1 : 2) <= 3ll * num_sms && plen + slen <= 8000) return FORM_JOINED;
+  // LISTS for up to 64 rows behind a long prefix: converting it all costs more than reading its FP8
+  // rows once (1 x 16, 16000: 26 DENSE, 31 LISTS; 65536: 54 and 43; 262144: 154 and 98; two blocks of
+  // rows, 2 x 64, 65536: 58 and 68).
+  if (rows <= 64 && plen > 40000) return FORM_LISTS;
+  return dsv4::prefix_attn_fits(*a, false) ? FORM_DENSE : FORM_LISTS;
 }
 
 static SharedPlan plan_shared(const Dsv4SharedPrefixArgs* a, int num_sms) {
@@ -368,12 +371,14 @@ static SharedPlan plan_shared(const Dsv4SharedPrefixArgs* a, int num_sms) {
   if (p.form == FORM_DENSE) {
     // In the same pass the own tokens are converted to BF16 rows like the prefix's, which pays while
     // those rows stay in L2, up to 131072 tokens that the table can hold; and a tile of them is of use
-    // to its request's rows alone, of which a block of 128 rows wants 16 (microseconds, same pass /
-    // own launch; requests x heads, prefix, own: 64 x 64, 32768, 64 to 2048: 219 / 244; 64 x 64, 2048,
-    // 64 to 2048: 61 / 91; 16 x 128, 8192, 4096 to 8192: 101 / 135; 64 x 16, 8192, 64 to 512: 53 /
-    // 58.  Beyond: 64 x 16, 32768, 1024 to 2048: 130 / 121; 64 x 64, 8192, 2048 to 4096: 168 / 162;
-    // 256 x 64, 1024, 1100: 217 / 184; 128 x 8, 32768, 64 to 512: 108 / 102).
-    p.own = slen > 0 && a->b * ((slen + 127) / 128 * 128) <= 131072 && a->s_q * a->h_q >= 16 && dsv4::prefix_attn_fits(*a, true);
+    // to its request's rows alone: fewer where those are less than an eighth of a block's 128
+    // (microseconds, same pass / own launch; requests x heads, prefix, own: 64 x 64, 32768, 64 to
+    // 2048: 219 / 244; 64 x 64, 2048, 64 to 2048: 61 / 91; 16 x 128, 8192, 4096 to 8192: 101 / 135; 64
+    // x 16, 8192, 64 to 512: 53 / 58; 27 x 8, 10976, up to 1056: 37 / 45.  Beyond: 64 x 16, 32768, 1024
+    // to 2048: 130 / 121; 64 x 64, 8192, 2048 to 4096: 168 / 162; 256 x 64, 1024, 1100: 217 / 184;
+    // 128 x 8, 32768, 64 to 512: 108 / 102).
+    const int64_t most_own = a->s_q * a->h_q >= 16 ? 131072 : 49152;
+    p.own = slen > 0 && a->b * ((slen + 127) / 128 * 128) <= most_own && dsv4::prefix_attn_fits(*a, true);
     p.prefix_sets = dsv4::prefix_attn_sets(rows, num_sms);
     p.prefix_bytes = dsv4::prefix_attn_workspace(*a, p.own);
     if (p.own) return p;
