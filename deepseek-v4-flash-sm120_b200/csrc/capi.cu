@@ -340,14 +340,14 @@ static SharedForm choose_form(const Dsv4SharedPrefixArgs* a, int64_t rows, int64
   if (by_list || plen + slen == 0 || (a->flags & DSV4_FLAG_SHARED_LISTS)) return FORM_LISTS;
   if (plen == 0 || (a->flags & DSV4_FLAG_SHARED_JOINED)) return FORM_JOINED;
   if ((a->flags & DSV4_FLAG_SHARED_DENSE) && dsv4::prefix_attn_fits(*a, false)) return FORM_DENSE;
-  // JOINED up to 3 tiles of 128 tokens an SM, half as many where they are of more than 32 heads, and
-  // lists of 8000 tokens (microseconds, JOINED / DENSE / LISTS, prefix x query tokens x heads: 2000 x
+  // JOINED up to 4 tiles of 128 tokens an SM, half as many where they are of more than 32 heads, and
+  // lists of 4000 tokens (microseconds, JOINED / DENSE / LISTS, prefix x query tokens x heads: 2000 x
   // 4 x 16: 19 / 25 / 35; 512 x 57 x 20, 456 tiles: 21 / 29 / 33; 6000 x 16 x 8, 768 tiles: 41 / 31 /
   // 35; 2000 x 3 x 64: 23 / 29 / 37; 1088 x 32 x 64, 288 tiles: 39 / 31 / 50; 16000 x 1 x 16: 31 / 26 /
-  // 31).  Over 600 drawn calls of up to 60 requests and 30000 tokens the rules here cost 0.6 % over
+  // 31).  Over 200 drawn calls of up to 60 requests and 30000 tokens the rules here cost 0.8 % over
   // the best form of each.
   const int64_t tiles = static_cast<int64_t>(a->b) * a->s_q * ((a->h_q + 63) / 64) * ((plen + slen + 127) / 128);
-  if (tiles * (a->h_q <= 32 ? 1 : 2) <= 3ll * num_sms && plen + slen <= 8000) return FORM_JOINED;
+  if (tiles * (a->h_q <= 32 ? 1 : 2) <= 4ll * num_sms && plen + slen <= 4000) return FORM_JOINED;
   // LISTS for up to 64 rows behind a long prefix: converting it all costs more than reading its FP8
   // rows once (1 x 16, 16000: 26 DENSE, 31 LISTS; 65536: 54 and 43; 262144: 154 and 98; two blocks of
   // rows, 2 x 64, 65536: 58 and 68).
