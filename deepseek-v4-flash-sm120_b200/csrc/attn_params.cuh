@@ -90,10 +90,11 @@ __device__ __forceinline__ const int32_t* idx_row(const int32_t* base, int64_t s
 
 // Final (o, lse) fix-up shared by the non-split epilogue and the combine step.
 // l is the softmax denominator relative to m.  Returns the factor that turns the
-// un-normalised accumulator into the output and sets lse_out (and ml_out).
+// un-normalised accumulator into the output and sets lse_out (and ml_out).  A NaN score makes l
+// NaN and sets no reference (m may still be -inf): such a row is NaN, not empty.
 __device__ __forceinline__ float finalize_row(int mode, float m, float l, bool has_sink,
                                               float sink, float& lse_out, float& ml_out) {
-  if (l == 0.0f || m == -INFINITY) {
+  if (l == 0.0f || (m == -INFINITY && l == l)) {
     if (mode == MODE_PREFILL) { lse_out = INFINITY; ml_out = -INFINITY; }
     else { lse_out = has_sink ? sink : -INFINITY; ml_out = -INFINITY; }
     return 0.0f;

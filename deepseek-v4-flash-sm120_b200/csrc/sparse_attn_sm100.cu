@@ -638,7 +638,7 @@ __device__ __noinline__ void cluster_merge(const MergeOut p, Ctrl& ctrl, const M
       if (rank == 0 && tid < c.heads_here && !ctrl.fail)
         p.lse[c.bi * p.stride_lse_b + c.si * p.stride_lse_s + (c.head0 + tid) * p.stride_lse_h] = lse_v;
     } else {
-      const bool none = !(total > 0.f);
+      const bool none = total == 0.f;                    // (a NaN score: total and lse are NaN)
       f = none ? 0.f : 1.f / total;
       if (rank == 0 && tid < c.heads_here && !ctrl.fail)
         p.lse_accum[c.acc_slot0 + tid] = none ? -INFINITY : logf(total) + big * LN2;
@@ -1302,7 +1302,9 @@ sm100_attn_kernel(const AttnParams p) {
       const float m_nat = (mr <= NEG_HUGE) ? -INFINITY : mr * LN2;
       float f;
       if (split_out) {
-        const bool empty = !(l > 0.f) || m_nat == -INFINITY;
+        // nothing seen; a NaN score makes l NaN, whether or not a reference was set beside it, and
+        // the log-sum-exp says so: the set must not be passed over when the partials are joined
+        const bool empty = l == 0.f || (m_nat == -INFINITY && l == l);
         f = empty ? 0.f : 1.f / l;
         if (tid < heads_here) p.lse_accum[acc_slot0 + tid] = empty ? -INFINITY : logf(l) + m_nat;
       } else {

@@ -279,8 +279,8 @@ int dsv4_sparse_prefill(const Dsv4PrefillArgs* args, void* cuda_stream);
  * them (the last s_q tokens are the queries' own).  The products with the prefix are formed
  * once for the rows of all requests together; the two parts are joined by their
  * log-sum-exps.  Layouts, out, lse (sink-merged) and strides as dsv4_sparse_decode's; a row
- * that sees nothing gives out 0 and lse = its sink, or -inf.  Tokens of a page id outside
- * [0, num_blocks) are masked; lengths are clamped to the tables.  The lengths live on the
+ * that sees nothing gives out 0 and lse = its sink, or -inf; one that sees a NaN or +inf
+ * score is NaN.  Tokens of a page id outside [0, num_blocks) are masked; lengths are clamped to the tables.  The lengths live on the
  * device; launches depend on sizes only.
  *
  * q rows are dense: stride_q_h = d_qk, [b, s_q, h_q] contiguous.  Scratch, sized by
