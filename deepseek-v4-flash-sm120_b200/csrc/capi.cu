@@ -328,6 +328,9 @@ int dsv4_sparse_prefill(const Dsv4PrefillArgs* a, void* stream) {
 //   DENSE   the prefix by launch_prefix_attn, with the own tokens where their table is not too
 //           wide, else those by the sparse kernel, joined;
 //   LISTS   the same with the prefix by the sparse kernel too, as one list for all rows.
+// Scratch is sized by one call and used by another, so the plan depends on the sizes alone: it is
+// made for the 148 SMs of a B200 whatever the device has (the kernels take any number of sets).
+constexpr int PLAN_SMS = 148;
 enum SharedForm { FORM_JOINED, FORM_DENSE, FORM_LISTS };
 struct SharedPlan {
   SharedForm form;
@@ -335,7 +338,7 @@ struct SharedPlan {
   int prefix_sets, suffix_splits;          // partial sets of the two parts (JOINED: splits in the second)
   int64_t prefix_bytes, suffix_bytes;      // of the workspace: the prefix's part, then the lists
 };
-static SharedForm choose_form(const Dsv4SharedPrefixArgs* a, int64_t rows, int64_t plen, int64_t slen, int num_sms) {
+static SharedForm choose_form(const Dsv4SharedPrefixArgs* a, int64_t rows, int64_t plen, int64_t slen) {
   const bool by_list = a->prefix_splits > 0 || a->suffix_splits > 0 || want_simple(a->flags);
   if (by_list || plen + slen == 0 || (a->flags & DSV4_FLAG_SHARED_LISTS)) return FORM_LISTS;
   if (plen == 0 || (a->flags & DSV4_FLAG_SHARED_JOINED)) return FORM_JOINED;
@@ -347,7 +350,7 @@ static SharedForm choose_form(const Dsv4SharedPrefixArgs* a, int64_t rows, int64
   // 31).  Over 200 drawn calls of up to 60 requests and 30000 tokens the rules here cost 0.8 % over
   // the best form of each.
   const int64_t tiles = static_cast<int64_t>(a->b) * a->s_q * ((a->h_q + 63) / 64) * ((plen + slen + 127) / 128);
-  if (tiles * (a->h_q <= 32 ? 1 : 2) <= 4ll * num_sms && plen + slen <= 4000) return FORM_JOINED;
+  if (tiles * (a->h_q <= 32 ? 1 : 2) <= 4ll * PLAN_SMS && plen + slen <= 4000) return FORM_JOINED;
   // LISTS for up to 64 rows behind a long prefix: converting it all costs more than reading its FP8
   // rows once (1 x 16, 16000: 26 DENSE, 31 LISTS; 65536: 54 and 43; 262144: 154 and 98; two blocks of
   // rows, 2 x 64, 65536: 58 and 68).
@@ -355,16 +358,16 @@ static SharedForm choose_form(const Dsv4SharedPrefixArgs* a, int64_t rows, int64
   return dsv4::prefix_attn_fits(*a, false) ? FORM_DENSE : FORM_LISTS;
 }
 
-static SharedPlan plan_shared(const Dsv4SharedPrefixArgs* a, int num_sms) {
+static SharedPlan plan_shared(const Dsv4SharedPrefixArgs* a) {
   SharedPlan p{};
   const int64_t rows = static_cast<int64_t>(a->b) * a->s_q * a->h_q;
   const int64_t plen = static_cast<int64_t>(a->prefix_pages) * a->page_block_size;
   const int64_t slen = static_cast<int64_t>(a->max_pages) * a->page_block_size;
   const int64_t tokens = static_cast<int64_t>(a->b) * a->s_q;
   const int64_t most = 0x7fffffff;
-  p.form = choose_form(a, rows, plen, slen, num_sms);
+  p.form = choose_form(a, rows, plen, slen);
   if (p.form == FORM_JOINED) {
-    p.suffix_splits = dsv4_plan_splits(a->b, a->s_q, a->h_q, static_cast<int>(plen + slen < most ? plen + slen : most), 0, num_sms);
+    p.suffix_splits = dsv4_plan_splits(a->b, a->s_q, a->h_q, static_cast<int>(plen + slen < most ? plen + slen : most), 0, PLAN_SMS);
     p.suffix_bytes = (tokens * (plen + slen) + a->b) * 4;
     return p;
   }
@@ -379,17 +382,17 @@ static SharedPlan plan_shared(const Dsv4SharedPrefixArgs* a, int num_sms) {
     // 128 x 8, 32768, 64 to 512: 108 / 102).
     const int64_t most_own = a->s_q * a->h_q >= 16 ? 131072 : 49152;
     p.own = slen > 0 && a->b * ((slen + 127) / 128 * 128) <= most_own && dsv4::prefix_attn_fits(*a, true);
-    p.prefix_sets = dsv4::prefix_attn_sets(rows, num_sms);
+    p.prefix_sets = dsv4::prefix_attn_sets(rows, PLAN_SMS);
     p.prefix_bytes = dsv4::prefix_attn_workspace(*a, p.own);
     if (p.own) return p;
   } else if (plen > 0) {
     p.prefix_sets = a->prefix_splits > 0 ? a->prefix_splits
-                                         : dsv4_plan_splits(1, 1, static_cast<int>(rows), static_cast<int>(plen), 0, num_sms);
+                                         : dsv4_plan_splits(1, 1, static_cast<int>(rows), static_cast<int>(plen), 0, PLAN_SMS);
     p.prefix_bytes = (plen + 63) / 64 * 64 * 4;
   }
   if (slen > 0)
     p.suffix_splits = a->suffix_splits > 0 ? a->suffix_splits
-                                           : dsv4_plan_splits(a->b, a->s_q, a->h_q, static_cast<int>(slen), 0, num_sms);
+                                           : dsv4_plan_splits(a->b, a->s_q, a->h_q, static_cast<int>(slen), 0, PLAN_SMS);
   p.suffix_bytes = slen * tokens * 4;
   return p;
 }
@@ -416,7 +419,7 @@ int dsv4_shared_prefix_scratch(const Dsv4SharedPrefixArgs* a, int num_sms, int32
   if (rc) return rc;
   if (!sets || !bytes) return DSV4_ERR_NULL;
   if (num_sms < 2) return DSV4_ERR_SHAPE;
-  const SharedPlan p = plan_shared(a, num_sms);
+  const SharedPlan p = plan_shared(a);
   *sets = p.prefix_sets + p.suffix_splits;
   if (p.form == FORM_JOINED && p.suffix_splits == 1) *sets = 0;      // final at once
   *bytes = p.prefix_bytes + p.suffix_bytes;
@@ -440,7 +443,7 @@ int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* a, void* stream) {
   if (e) return cuda_fail(e);
   DevInfo info;
   if ((rc = device_info(dev, info))) return rc;
-  const SharedPlan plan = plan_shared(a, info.sms);
+  const SharedPlan plan = plan_shared(a);
   const int sets = plan.prefix_sets + plan.suffix_splits;
   if (sets > 0 && (plan.form != FORM_JOINED || sets > 1)) {
     if (!a->o_accum || !a->lse_accum) return DSV4_ERR_SCRATCH;
@@ -486,7 +489,7 @@ int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* a, void* stream) {
     d.stride_lse_b = a->stride_lse_b; d.stride_lse_s = a->stride_lse_s; d.stride_lse_h = a->stride_lse_h;
     return dsv4_sparse_decode(&d, stream);
   }
-  if (plan.form == FORM_DENSE && (e = dsv4::launch_prefix_attn(*a, setup, info.sms, st))) return cuda_fail(e);
+  if (plan.form == FORM_DENSE && (e = dsv4::launch_prefix_attn(*a, setup, plan.prefix_sets, info.sms, st))) return cuda_fail(e);
 
   dsv4::AttnParams p{};
   p.cluster = 1;

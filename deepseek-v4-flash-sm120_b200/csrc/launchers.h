@@ -62,14 +62,15 @@ cudaError_t launch_shared_setup(const Dsv4SharedPrefixArgs& a, const SharedSetup
 // Joins partial sets of BF16 outputs (like launch_combine, for few sets and many rows).
 cudaError_t launch_join_sets(const Dsv4CombineArgs& a, cudaStream_t st);
 
-// Attention of many rows over a shared prefix, into the first prefix_attn_sets partial sets
-// (shared_prefix_sm100.cu).
+// Attention of many rows over a shared prefix, into the first `sets` partial sets
+// (shared_prefix_sm100.cu); prefix_attn_sets says how many suit a number of SMs, and two or more
+// are enough for any.
 int prefix_attn_sets(int64_t rows, int num_sms);
 // `own`: with the requests' own tokens.  Do the sizes fit, and how many bytes of workspace?
 bool prefix_attn_fits(const Dsv4SharedPrefixArgs& a, bool own);
 int64_t prefix_attn_workspace(const Dsv4SharedPrefixArgs& a, bool own);
 void prefix_attn_place(const Dsv4SharedPrefixArgs& a, bool own, SharedSetup& out);
-cudaError_t launch_prefix_attn(const Dsv4SharedPrefixArgs& a, const SharedSetup& rows, int num_sms, cudaStream_t st);
+cudaError_t launch_prefix_attn(const Dsv4SharedPrefixArgs& a, const SharedSetup& rows, int sets, int num_sms, cudaStream_t st);
 cudaError_t read_prefix_error(int* value, bool reset);
 
 // Dense attention over packed sequences (dense_attn_sm100.cu).

@@ -1021,12 +1021,12 @@ cudaError_t launch_join_sets(const Dsv4CombineArgs& a, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, join_sets_kernel, a);
 }
 
-cudaError_t launch_prefix_attn(const Dsv4SharedPrefixArgs& a, const SharedSetup& setup, int num_sms, cudaStream_t st) {
+cudaError_t launch_prefix_attn(const Dsv4SharedPrefixArgs& a, const SharedSetup& setup, int sets, int num_sms, cudaStream_t st) {
   cudaError_t e;
   PrefixParams p;
   p.rows = a.b * a.s_q * a.h_q;
   p.blocks = (p.rows + 2 * ROWS - 1) / (2 * ROWS);
-  p.sets = prefix_attn_sets(p.rows, num_sms);
+  p.sets = sets;
   p.max_tokens = a.prefix_pages * a.page_block_size;
   p.padded = setup.padded;
   p.own_padded = setup.own_padded;

@@ -314,8 +314,9 @@ typedef struct Dsv4SharedPrefixArgs {
 
 int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* args, void* cuda_stream);
 
-/* Scratch of such a call (sizes and split counts of `args`; pointers are not looked at):
- * partial sets, and bytes of workspace.                                                    */
+/* Scratch of such a call (sizes, split counts and flags of `args`; pointers are not looked
+ * at): partial sets, and bytes of workspace.  They do not depend on num_sms (2 or more):
+ * the call plans for the 148 SMs of a B200 on every device.                                */
 int dsv4_shared_prefix_scratch(const Dsv4SharedPrefixArgs* args, int num_sms, int32_t* sets,
                                int64_t* workspace_bytes);
 

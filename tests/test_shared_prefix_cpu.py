@@ -69,3 +69,15 @@ def test_operator_refuses_host_tensors():
     q, kv = torch.zeros(2, 1, 16, 576, dtype=torch.bfloat16), torch.zeros(4, 64, 1, 644, dtype=torch.uint8)
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.shared_prefix_decode_fwd(q, kv, n, n[:1], t, n, None, 512, 0.04)
+
+
+@pytest.mark.parametrize("kw", [{}, dict(b=64, h_q=64, prefix_pages=512, max_pages=32), dict(b=16, h_q=64, prefix_pages=512, max_pages=1000),
+                                dict(b=1, s_q=1, prefix_pages=1100), dict(flags=N.FLAG_SHARED_JOINED), dict(flags=N.FLAG_SHARED_LISTS),
+                                dict(prefix_pages=0), dict(max_pages=0)])
+def test_scratch_is_what_the_call_uses_whatever_number_of_sms_is_named(kw):
+    """The call cannot know which number its scratch was sized with."""
+    def sized(num_sms):
+        sets, nbytes = C.c_int32(-1), C.c_int64(-1)
+        assert N.lib.dsv4_shared_prefix_scratch(C.byref(shared_args(**kw)), num_sms, C.byref(sets), C.byref(nbytes)) == 0
+        return sets.value, nbytes.value
+    assert len({sized(n) for n in (2, 3, 20, 74, 132, 148, 160, 1000)}) == 1
