@@ -419,6 +419,9 @@ int dsv4_shared_prefix_scratch(const Dsv4SharedPrefixArgs* a, int num_sms, int32
   if (rc) return rc;
   if (!sets || !bytes) return DSV4_ERR_NULL;
   if (num_sms < 2) return DSV4_ERR_SHAPE;
+  *sets = 0;
+  *bytes = 0;
+  if (a->b == 0) return DSV4_OK;         // (the plan divides by the rows' blocks)
   const SharedPlan p = plan_shared(a);
   *sets = p.prefix_sets + p.suffix_splits;
   if (p.form == FORM_JOINED && p.suffix_splits == 1) *sets = 0;      // final at once

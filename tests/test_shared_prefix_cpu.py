@@ -81,3 +81,10 @@ def test_scratch_is_what_the_call_uses_whatever_number_of_sms_is_named(kw):
         assert N.lib.dsv4_shared_prefix_scratch(C.byref(shared_args(**kw)), num_sms, C.byref(sets), C.byref(nbytes)) == 0
         return sets.value, nbytes.value
     assert len({sized(n) for n in (2, 3, 20, 74, 132, 148, 160, 1000)}) == 1
+
+
+@pytest.mark.parametrize("kw", [{}, dict(prefix_pages=100), dict(prefix_pages=5000), dict(max_pages=500), dict(flags=N.FLAG_SHARED_DENSE),
+                                dict(flags=N.FLAG_SHARED_LISTS), dict(prefix_splits=3)])
+def test_a_batch_of_no_request_needs_no_scratch(kw):
+    assert scratch(b=0, **kw) == (0, 0)
+    assert N.lib.dsv4_shared_prefix_decode(C.byref(shared_args(b=0, **kw)), None) in (0, 5, 6)      # (5, 6: no such device here)
