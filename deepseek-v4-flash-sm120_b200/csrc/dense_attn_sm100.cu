@@ -488,8 +488,10 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     tc_fence_after_sync();
   }
   const uint32_t tmem = ctrl.tmem;
-  // A role whose bounded wait gives up records it and ends; the others then run into their
-  // own limits, long after every copy and product in flight has finished.
+  // A lane whose bounded wait gives up records it, waits for nothing any more and issues nothing; but
+  // it walks on through the same loops, so that its warp stays together for what the whole warp has
+  // to execute (a phase may complete just as the first lanes give up).  The other roles then run into
+  // their own limits, long after every copy and product in flight has finished.
   auto gave_up = [&](int code) {
     atomicExch(&g_dense_error, code);
     *reinterpret_cast<volatile int*>(&ctrl.fail) = 1;
@@ -508,19 +510,26 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
                         w.q0 + w.t0 + s * p.tok_tile, bar(&ctrl.q_full[s]));
         };
         if (w.count[0] > 0) load_q(0);
-        bool ok = true;
+        bool ok = true;                  // (one lane alone: it may stop)
         int ks = 0, kphase = 0, vu = 0, vphase = 0;
-        for (int i = 0; i < n_tiles && ok; ++i) {
+        auto wait = [&](uint64_t* b, int parity) {
+          if (ok && !mbar_wait_fast(bar(b), parity)) {
+            gave_up(ERR_SLOT);
+            ok = false;
+          }
+          return ok;
+        };
+        for (int i = 0; i < n_tiles; ++i) {
           const int row = w.k0 + (w.first + i) * TILE_N;
           for (int c = 0; c < C::QB; c += C::K_STEP) {
-            if (!mbar_wait_fast(bar(&ctrl.k_empty[ks]), kphase ^ 1)) { gave_up(ERR_SLOT); ok = false; break; }
+            if (!wait(&ctrl.k_empty[ks], kphase ^ 1)) break;
             mbar_expect_tx(bar(&ctrl.k_full[ks]), C::K_STEP * BLOCK_BYTES);
             for (int d = 0; d < C::K_STEP; ++d)
               tma_load_3d(sK + (ks * C::K_STEP + d) * BLOCK_BYTES, &p.mk, 64 * (c + d), kvh, row, bar(&ctrl.k_full[ks]));
             if (++ks == C::K_RING) { ks = 0; kphase ^= 1; }
           }
           if (i == 0 && w.count[1] > 0 && !twin) load_q(1);
-          if (!ok || !mbar_wait_fast(bar(&ctrl.v_empty[vu]), vphase ^ 1)) { gave_up(ERR_SLOT); break; }
+          if (!wait(&ctrl.v_empty[vu], vphase ^ 1)) break;
           const uint32_t landed = bar(w.first + i >= w.look ? &ctrl.v_look[vu] : &ctrl.v_full[vu]);
           mbar_expect_tx(landed, C::V_UNIT_BYTES);
           for (int c = 0; c < C::VB; ++c)
@@ -546,21 +555,20 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
       bool ok = true;
       auto wait = [&](uint64_t* b, int parity, int code) {
         if (ok && !mbar_wait_fast(bar(b), parity)) {
-          if (lane == 0) gave_up(code);
+          if (elected) gave_up(code);
           ok = false;
         }
-        __syncwarp();
-      };
+      };                                 // (no lane needs another one here; a __syncwarp took 0.6 % more)
       if (warp == WARP_QK) {
         constexpr uint32_t idesc = make_idesc_16(BF16, TILE_M, TILE_N, 0, 0);
         const uint64_t dQ = make_smem_desc(sQ, 16, 1024, SWZ_128B);
         const uint64_t dK = make_smem_desc(sK, 16, 1024, SWZ_128B);
         int turn = 0;                                    // score tiles so far
 #pragma unroll 1
-        for (int i = 0; i < tiles && ok; ++i) {
+        for (int i = 0; i < tiles; ++i) {
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            if (!takes(s, i) || !ok) continue;
+            if (!takes(s, i)) continue;
             const bool last = twin || s == 1 || i >= count1;     // nobody reads the tile's K after this
             const int j = nth(i);
             if (j == 0) wait(&ctrl.q_full[twin ? 0 : s], 0, ERR_Q);
@@ -573,14 +581,15 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
 #pragma unroll
             for (int c = 0; c < C::QB; c += C::K_STEP) {
               wait(&ctrl.k_full[ks], kphase, ERR_K);
-              if (!ok) break;
               tc_fence_after_sync();
               const uint64_t d = dK + ((ks * C::K_STEP * BLOCK_BYTES) >> 4);
+              if (ok) {
 #pragma unroll
-              for (int k = 0; k < 4 * C::K_STEP; ++k)
-                umma_bf16_elect(tS, dQ + ((((twin ? 0 : s) * C::QB + c + (k >> 2)) * BLOCK_BYTES + (k & 3) * 32) >> 4),
-                                d + (((k >> 2) * BLOCK_BYTES + (k & 3) * 32) >> 4), idesc, (c | k) != 0, elected);
-              if (last) umma_commit_elect(bar(&ctrl.k_empty[ks]), elected);
+                for (int k = 0; k < 4 * C::K_STEP; ++k)
+                  umma_bf16_elect(tS, dQ + ((((twin ? 0 : s) * C::QB + c + (k >> 2)) * BLOCK_BYTES + (k & 3) * 32) >> 4),
+                                  d + (((k >> 2) * BLOCK_BYTES + (k & 3) * 32) >> 4), idesc, (c | k) != 0, elected);
+                if (last) umma_commit_elect(bar(&ctrl.k_empty[ks]), elected);
+              }
               if (++ks == C::K_RING) { ks = 0; kphase ^= 1; }
             }
             if (ok) umma_commit_elect(bar(&ctrl.s_full[s]), elected);
@@ -593,7 +602,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
         const int units = twin ? C::V_UNITS + 1 : C::V_UNITS;
         uint32_t clean_parity = 0;
 #pragma unroll 1
-        for (int i = 0; i < tiles && ok; ++i) {
+        for (int i = 0; i < tiles; ++i) {
           const int vu = i % units, vphase = (i / units) & 1;
           const uint64_t d = RANGES && vu == C::V_UNITS ? dV_more : dV + ((vu * C::V_UNIT_BYTES) >> 4);
           if (w.first + i >= w.look) {
@@ -607,8 +616,8 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
             if (!takes(s, i)) continue;
             const int j = nth(i);
             wait(&ctrl.p_full[s], j & 1, ERR_P);
-            if (!ok) break;
             tc_fence_after_sync();
+            if (!ok) continue;
 #pragma unroll
             for (int k = 0; k < TILE_N / 16; ++k)
               umma_ts_elect(t0 + C::COL_O + DV * s, t0 + C::COL_P + 64 * s + 8 * k, d + ((k * 2048) >> 4), idesc,
@@ -623,12 +632,14 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
       // keys the whole CTA sees (its last row sees the most)
       const int seen = reach_of(p, w, min(w.t0 + 2 * p.tok_tile, w.len_q) - 1);
       uint32_t parity = 0;
+      bool ok = true;
       for (int i = max(w.look - w.first, 0); i < n_tiles; ++i) {
         const int vu = i % v_units;
-        if (!mbar_wait_fast(bar(&ctrl.v_look[vu]), (parity >> vu) & 1)) {
-          if (lane == 0) gave_up(ERR_V);
-          break;
+        if (ok && !mbar_wait_fast(bar(&ctrl.v_look[vu]), (parity >> vu) & 1)) {
+          gave_up(ERR_V);
+          ok = false;
         }
+        __syncwarp();
         parity ^= 1u << vu;
         const int live = min(seen - (w.first + i) * TILE_N, TILE_N);   // rows of the tile that count
         // 32 chunks of 16 bytes (four rows of a block) at a time
@@ -704,15 +715,22 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
 
   float m_ref = -INFINITY, m_raw = -INFINITY, l = 0.f;
   bool ok = true;
+  auto wait = [&](uint64_t* b, int parity, int code) {
+    if (ok && !mbar_wait_fast(bar(b), parity)) {
+      gave_up(code);
+      ok = false;
+    }
+  };
 #pragma unroll 1
   for (int i = 0; i < n_mine; ++i) {
-    if (!mbar_wait_fast(bar(&ctrl.s_full[s]), i & 1)) { gave_up(ERR_S); ok = false; break; }
+    wait(&ctrl.s_full[s], i & 1, ERR_S);
     tc_fence_after_sync();
     if (idle) {
       if (lane == 0) mbar_arrive(bar(&ctrl.s_free[C::S_BUFS == 1 ? 0 : s]));
       // the same order as below: P of this tile is reported once P of the one before has been read,
       // or two reports of one warp could fall into one phase
-      if (i > 0 && !mbar_wait_fast(bar(&ctrl.o_done[s]), (i - 1) & 1)) { gave_up(ERR_O); ok = false; break; }
+      if (i > 0) wait(&ctrl.o_done[s], (i - 1) & 1, ERR_O);
+      __syncwarp();
       if (lane == 0) mbar_arrive(bar(&ctrl.p_full[s]));
       __syncwarp();
       continue;
@@ -747,7 +765,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     }
     // the product of the tile before has read P, and O is its result
     if (i > 0) {
-      if (!mbar_wait_fast(bar(&ctrl.o_done[s]), (i - 1) & 1)) { gave_up(ERR_O); ok = false; break; }
+      wait(&ctrl.o_done[s], (i - 1) & 1, ERR_O);
       tc_fence_after_sync();
     }
     if (i > 0 && __any_sync(0xffffffffu, raise)) {
@@ -791,7 +809,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   grid_launch_dependents();
 
   // ---- epilogue --------------------------------------------------------------------------
-  if (n_mine > 0 && ok && !mbar_wait_fast(bar(&ctrl.o_done[s]), (n_mine - 1) & 1)) { gave_up(ERR_O); ok = false; }
+  if (n_mine > 0) wait(&ctrl.o_done[s], (n_mine - 1) & 1, ERR_O);
   tc_fence_after_sync();
   const bool fail = !ok || *reinterpret_cast<volatile int*>(&ctrl.fail) != 0;
   const int64_t t = static_cast<int64_t>(w.q0) + tok;

@@ -274,8 +274,10 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
   const uint32_t tmem = ctrl.tmem;
   grid_dependency_wait();
   Share w(p, blockIdx.x >> 1, gridDim.x >> 1);
-  // A role whose bounded wait gives up records it and waits for nothing any more; what it does
-  // from then on is of no use, but every barrier of the CTA is still walked.
+  // A lane whose bounded wait gives up records it, waits for nothing any more and issues nothing; but
+  // it walks on through the same loops, so that its warp stays together for what the whole warp has
+  // to execute (a phase may complete just as the first lanes give up) and every barrier of the CTA
+  // is met.
   bool ok = true;
   auto gave_up = [&](int code) {
     atomicExch(&g_prefix_error, code);
@@ -284,16 +286,16 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
   };
 
   if (warp >= WARP_QK) {
+    const uint32_t elected = elect_one();          // the lane that loads or issues
     auto wait = [&](uint64_t* b, int parity, int code) {
       if (ok && !mbar_wait_fast(bar(b), parity)) {
-        if (lane == 0) gave_up(code);
+        if (elected) gave_up(code);
         ok = false;
       }
       __syncwarp();
     };
     if (warp == WARP_LOAD_K) {
       // ======================= Q and K ======================================================
-      const uint32_t elected = elect_one();
       int n = 0;
       while (__all_sync(0xffffffffu, ok) && w.next(p.starts)) {
         // Q is free once every product of the segment before is done
@@ -307,8 +309,7 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
           tok += rank * ROWS;
           for (int g = 0; g < C::GROUPS; ++g) {
             wait(&ctrl.k_empty[g], (n & 1) ^ 1, ERR_SLOT);
-            if (!ok) break;
-            if (elected) {
+            if (ok && elected) {
               if (rank == 0) mbar_expect_tx(bar(&ctrl.k_land[g]), 2 * C::PER * QK_BLOCK);
               for (int c = g * C::PER; c < (g + 1) * C::PER; ++c)
                 load_pair(sK + c * QK_BLOCK, &p.mk, 64 * c, 0, tok, of_leader(bar(&ctrl.k_land[g])));
@@ -317,10 +318,10 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
           ++n;
         };
         int i = 0;
-        for (; i < w.shared && ok; ++i) load((w.first + i) * TILE);
+        for (; i < w.shared; ++i) load((w.first + i) * TILE);
         if (i < w.count) {
           OwnTile tile(p, w.block, w.first + i - w.prefix_tiles);
-          for (; i < w.count && ok; ++i) {
+          for (; i < w.count; ++i) {
             load(tile.row(p));
             tile.step(p);
           }
@@ -328,14 +329,12 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
       }
     } else if (warp == WARP_LOAD_V) {
       // ======================= V ============================================================
-      const uint32_t elected = elect_one();
       int n = 0;
       while (__all_sync(0xffffffffu, ok) && w.next(p.starts)) {
         auto load = [&](int tok) {
           for (int h = 0; h < 2; ++h) {
             wait(&ctrl.v_empty[h], (n & 1) ^ 1, ERR_SLOT);
-            if (!ok) break;
-            if (elected) {
+            if (ok && elected) {
               if (rank == 0) mbar_expect_tx(bar(&ctrl.v_land[h]), 4 * V_BLOCK);
               for (int c = 0; c < 2; ++c)
                 load_pair(sV + (2 * h + c) * V_BLOCK, &p.mv, 256 * h + 128 * rank + 64 * c, 0, tok, of_leader(bar(&ctrl.v_land[h])));
@@ -344,10 +343,10 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
           ++n;
         };
         int i = 0;
-        for (; i < w.shared && ok; ++i) load((w.first + i) * TILE);
+        for (; i < w.shared; ++i) load((w.first + i) * TILE);
         if (i < w.count) {
           OwnTile tile(p, w.block, w.first + i - w.prefix_tiles);
-          for (; i < w.count && ok; ++i) {
+          for (; i < w.count; ++i) {
             load(tile.row(p));
             tile.step(p);
           }
@@ -360,21 +359,20 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
       constexpr uint32_t idesc = make_idesc_bf16(128, TILE, 0, 0);
       const uint64_t dQ = make_smem_desc(sQ, 16, 1024, SWZ_128B), dK = make_smem_desc(sK, 16, 1024, SWZ_128B);
       const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0) + COL_S;
-      const uint32_t elected = elect_one();
       int n = 0, seg = 0;
       while (__all_sync(0xffffffffu, ok) && w.next(p.starts)) {
         wait(&ctrl.q_land, seg & 1, ERR_Q);
         ++seg;
         const int count = __shfl_sync(0xffffffffu, w.count, 0);
 #pragma unroll 1
-        for (int i = 0; i < count && ok; ++i, ++n) {
+        for (int i = 0; i < count; ++i, ++n) {
           wait(&ctrl.s_free[n & 1], ((n >> 1) & 1) ^ 1, ERR_FREE);
           const uint32_t tS = t0 + 64 * (n & 1);
 #pragma unroll
           for (int g = 0; g < C::GROUPS; ++g) {
             wait(&ctrl.k_land[g], n & 1, ERR_K);
-            if (!ok) break;
             tc_fence_after_sync();
+            if (!ok) continue;
 #pragma unroll
             for (int k = 0; k < 4 * C::PER; ++k) {
               const uint32_t off = ((g * C::PER + (k >> 2)) * QK_BLOCK + (k & 3) * 32) >> 4;
@@ -391,20 +389,19 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
       const uint64_t dP = make_smem_desc(sP, 16, 1024, SWZ_128B);
       const uint64_t dV = make_smem_desc(sV, V_BLOCK, 1024, SWZ_128B);       // MN-major
       const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0) + COL_O;
-      const uint32_t elected = elect_one();
       int n = 0, seg = 0;
       while (__all_sync(0xffffffffu, ok) && w.next(p.starts)) {
         wait(&ctrl.o_free, (seg & 1) ^ 1, ERR_FREE);     // the segment before has been read out
         ++seg;
         const int count = __shfl_sync(0xffffffffu, w.count, 0);
 #pragma unroll 1
-        for (int i = 0; i < count && ok; ++i, ++n) {
+        for (int i = 0; i < count; ++i, ++n) {
           wait(&ctrl.p_full, n & 1, ERR_P);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             wait(&ctrl.v_land[h], n & 1, ERR_V);
-            if (!ok) break;
             tc_fence_after_sync();
+            if (!ok) continue;
 #pragma unroll
             for (int k = 0; k < TILE / 16; ++k)
               umma2(t0 + 128 * h, dP + (((k >> 2) * QK_BLOCK + (k & 3) * 32) >> 4),
