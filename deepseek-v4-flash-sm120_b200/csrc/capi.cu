@@ -331,6 +331,9 @@ int dsv4_sparse_prefill(const Dsv4PrefillArgs* a, void* stream) {
 // Scratch is sized by one call and used by another, so the plan depends on the sizes alone: it is
 // made for the 148 SMs of a B200 whatever the device has (the kernels take any number of sets).
 constexpr int PLAN_SMS = 148;
+// DENSE keeps 2 d_qk bytes of workspace for every token that the prefix table can hold, in each
+// captured graph too.
+constexpr int64_t DENSE_MOST_BYTES = 4ll << 30;
 enum SharedForm { FORM_JOINED, FORM_DENSE, FORM_LISTS };
 struct SharedPlan {
   SharedForm form;
@@ -355,7 +358,10 @@ static SharedForm choose_form(const Dsv4SharedPrefixArgs* a, int64_t rows, int64
   // rows once (1 x 16, 16000: 26 DENSE, 31 LISTS; 65536: 54 and 43; 262144: 154 and 98; two blocks of
   // rows, 2 x 64, 65536: 58 and 68).
   if (rows <= 64 && plen > 40000) return FORM_LISTS;
-  return dsv4::prefix_attn_fits(*a, false) ? FORM_DENSE : FORM_LISTS;
+  // DENSE for all others, unless its workspace passes what a caller can be expected to have: tables
+  // of more than 3.7 million tokens (d_qk 576) go by LISTS, 4 bytes a token (64 x 64 behind 4194304
+  // tokens: 29 ms DENSE with 4.8 GB, 72 LISTS with 17 MB; 16 x 64: 7.9 and 19).
+  return dsv4::prefix_attn_fits(*a, false) && dsv4::prefix_attn_workspace(*a, false) <= DENSE_MOST_BYTES ? FORM_DENSE : FORM_LISTS;
 }
 
 static SharedPlan plan_shared(const Dsv4SharedPrefixArgs* a) {

@@ -285,8 +285,9 @@ def shared_prefix_decode_fwd(q, kv, prefix_table, prefix_length, block_table, su
     Query token s sees the whole prefix and suffix_length - (s_q - 1 - s) own tokens.  A row
     that sees nothing gives out 0 and lse = its sink, or -inf.  Tokens on pages outside the
     cache are masked.  The lengths stay on the device, so a captured call can be replayed
-    with others; the scratch grows with what the two tables can hold, so they should be no
-    wider than needed.  `prefix_splits` / `suffix_splits` / `flags` are test hooks.  No counterpart
+    with others; the scratch grows with what the two tables can hold (2 * d_qk bytes a token
+    of the prefix table, 4 GiB at most, beyond which the call takes 2.5 times as long), so they
+    should be no wider than needed.  `prefix_splits` / `suffix_splits` / `flags` are test hooks.  No counterpart
     in the reference."""
     if not (q.is_cuda and kv.get_device() == q.get_device()):
         raise RuntimeError("q and kv must be CUDA tensors of one device")

@@ -316,7 +316,10 @@ int dsv4_shared_prefix_decode(const Dsv4SharedPrefixArgs* args, void* cuda_strea
 
 /* Scratch of such a call (sizes, split counts and flags of `args`; pointers are not looked
  * at): partial sets, and bytes of workspace.  They do not depend on num_sms (2 or more):
- * the call plans for the 148 SMs of a B200 on every device.                                */
+ * the call plans for the 148 SMs of a B200 on every device.  The workspace follows what the
+ * tables can hold, not the lengths: 2 d_qk bytes a token of the prefix table, 4 GiB at most
+ * (a wider one takes 4 bytes a token, and 2.5 times as long), and for the own tokens 2 d_qk
+ * bytes a token up to 131072 of them, or 4 s_q.                                            */
 int dsv4_shared_prefix_scratch(const Dsv4SharedPrefixArgs* args, int num_sms, int32_t* sets,
                                int64_t* workspace_bytes);
 

@@ -88,3 +88,13 @@ def test_scratch_is_what_the_call_uses_whatever_number_of_sms_is_named(kw):
 def test_a_batch_of_no_request_needs_no_scratch(kw):
     assert scratch(b=0, **kw) == (0, 0)
     assert N.lib.dsv4_shared_prefix_decode(C.byref(shared_args(b=0, **kw)), None) in (0, 5, 6)      # (5, 6: no such device here)
+
+
+@pytest.mark.parametrize("kw,per_token", [({}, 1152), (dict(d_qk=512, kv_format=N.KV_MODEL1, stride_kv_block=64 * 584), 1024)])
+def test_workspace_is_bounded_however_wide_the_table(kw, per_token):
+    batch = dict(b=64, s_q=1, h_q=64, num_blocks=1 << 16, max_pages=4, **kw)
+    most = (4 << 30) // (per_token * 64)                                    # pages whose tokens fill 4 GiB
+    for pages in (512, most // 2, most - 1000):
+        assert scratch(prefix_pages=pages, **batch)[1] >= pages * 64 * per_token
+    for pages in (most + 1, 1 << 17, 1 << 20, (1 << 25) - 2000):
+        assert scratch(prefix_pages=pages, **batch)[1] <= pages * 64 * 4 + (1 << 20)
