@@ -16,10 +16,12 @@
 // columns: the two tiles (s = 0, 1) share one score buffer (O_0, O_1, P_0 and P_1 fill the rest
 // of TMEM at d_v = 128), the scores of the next tile are formed while this one's exponentials
 // are, and the product with V waits for neither.  O is rescaled
-// only when a row's maximum has grown by more than 2^8 since its reference was set (the sums
-// are 32-bit and P has as many significant bits at any scale), by the same threads, so there
-// is no correction stage.  Q, K and V arrive by TMA; K's ring is recycled in blocks of 64
-// columns and V's in tiles, which is what the 227 KB allow at d_qk = 192.
+// only when a row's maximum has grown by more than 2^8 since its reference was set, by the same
+// threads, so there is no correction stage.  The sums are 32-bit; P has as many significant bits
+// at any scale in BF16, while FP16 weights are held 2^7 times as large (at most 2^15 then), which
+// moves what FP16 cannot hold from 2^-25 of the reference's weight to 2^-32 (of 120000 keys 18 nats
+// below another one, 0.2 % of the weight, nothing was left).  Q, K and V arrive by TMA; K's ring is
+// recycled in blocks of 64 columns and V's in tiles, which is what the 227 KB allow at d_qk = 192.
 //
 // Masked keys: scores are replaced, not added to, so nothing in a masked key's K row counts.
 // A product with weight zero would still let a NaN or an infinity of a masked V row through,
@@ -70,6 +72,7 @@ static_assert(THREADS * (LAUNCH_REGS + 8) > 65536, "LAUNCH_REGS is what the laun
 constexpr int WARP_QK = 8, WARP_PV = 9, WARP_TMA = 10, WARP_LOOK = 11;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float RESCALE_THRESHOLD = 8.0f;            // log2 units
+constexpr float FP16_LIFT = 7.0f;                    // log2 of the factor on FP16 weights
 constexpr uint32_t TMEM_COLS = 512;
 
 enum DenseErr { ERR_Q = 11, ERR_K = 12, ERR_V = 13, ERR_P = 14, ERR_S = 15, ERR_O = 16, ERR_SLOT = 17, ERR_LOOK = 18,
@@ -713,7 +716,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   // tiles below this one are seen whole by every row of this tile that exists
   const int whole = reach_of(p, w, row_t0) / TILE_N;
 
-  float m_ref = -INFINITY, m_raw = -INFINITY, l = 0.f;
+  float m_ref = -INFINITY, m_raw = -INFINITY, l = 0.f;    // l: times the factor on the weights
   bool ok = true;
   auto wait = [&](uint64_t* b, int parity, int code) {
     if (ok && !mbar_wait_fast(bar(b), parity)) {
@@ -781,7 +784,8 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     }
     const float ref = m_ref == -INFINITY ? 0.f : m_ref;
     if (!(top2 < INFINITY)) l = NAN;                 // a NaN or infinite score: the row shows it
-    const uint64_t c2 = pair(c, c), minus_ref = pair(-ref, -ref);
+    const float off = BF16 ? -ref : FP16_LIFT - ref;
+    const uint64_t c2 = pair(c, c), minus_ref = pair(off, off);
     uint64_t sum[2] = {0, 0};
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -816,7 +820,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
   float factor = 0.f;
   const int set = RANGES ? 2 * w.split + (twin ? s : 0) : 0;
   if (live) {
-    store_stats(p, set, t, h, m_raw, m_ref, l, fail, factor);
+    store_stats(p, set, t, h, m_raw, BF16 ? m_ref : m_ref - FP16_LIFT, l, fail, factor);
     float none;
     if (RANGES && !twin) store_stats(p, set + 1, t, h, -INFINITY, -INFINITY, 0.f, false, none);
     if (RANGES && (!twin || s == 0))
