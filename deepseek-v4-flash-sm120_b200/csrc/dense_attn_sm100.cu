@@ -921,7 +921,9 @@ dense_combine_kernel(const __grid_constant__ DenseParams p) {
   float w[4], sum = 0.f;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    w[k] = e[k] == -INFINITY ? 0.f : expf(e[k] - top);
+    // a set that holds anything weighs more than nothing, so that values in it that are not finite show;
+    // 2^-149 changes no other number
+    w[k] = e[k] == -INFINITY ? 0.f : expf(e[k] - top) + 1.4e-45f;
     sum += w[k];
   }
 #pragma unroll

@@ -122,3 +122,22 @@ def test_sparse_decode_of_one_token_that_is_not_finite(n_splits, simple):
     assert K.device_status() == 0
     assert torch.isnan(out[0]).all() and torch.isnan(lse[0]).all()
     assert (out[1] == 0).all() and (lse[1] == -float("inf")).all()
+
+
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("n_splits", [1, 2, 5, 16])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_values_far_below_the_largest_weight(dtype, n_splits, value):
+    """The token with the value that is not finite weighs e^-200 of the last one: still not nothing."""
+    n = 4000
+    q, k = torch.zeros(1, 2, 128, dtype=dtype, device="cuda"), torch.zeros(n, 1, 128, dtype=dtype, device="cuda")
+    v = torch.ones(n, 1, 128, dtype=dtype, device="cuda")
+    q[..., 0], k[n - 1, 0, 0], v[37, 0, 5] = 200.0, 1.0, value
+    cq, ck = (torch.tensor([0, m], dtype=torch.int32, device="cuda") for m in (1, n))
+    out, ml, lse = K.dense_prefill_fwd(q, k, v, cq, ck, 1.0, n_splits=n_splits)
+    torch.cuda.synchronize()
+    assert K.device_status() == 0
+    assert not torch.isfinite(out[..., 5]).any()
+    rest = torch.cat([out[..., :5], out[..., 6:]], -1)
+    assert ((rest.double() - 1).abs() <= torch.finfo(dtype).eps).all()
+    assert (ml == 200).all() and ((lse - 200).abs() <= 1e-3).all()
