@@ -53,6 +53,9 @@ int current_device_is_sm100() {
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Largest count that a kernel steps through: room for the strides that its 32-bit counters are
+// advanced and rounded by.
+constexpr int MOST_ITEMS = 0x7fffffff - 0xffff;
 bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 
 int check_paged(int kv_format, int d_qk, int page_block, int64_t stride_block, const void* kv) {
@@ -370,10 +373,9 @@ static SharedPlan plan_shared(const Dsv4SharedPrefixArgs* a) {
   const int64_t plen = static_cast<int64_t>(a->prefix_pages) * a->page_block_size;
   const int64_t slen = static_cast<int64_t>(a->max_pages) * a->page_block_size;
   const int64_t tokens = static_cast<int64_t>(a->b) * a->s_q;
-  const int64_t most = 0x7fffffff;
   p.form = choose_form(a, rows, plen, slen);
   if (p.form == FORM_JOINED) {
-    p.suffix_splits = dsv4_plan_splits(a->b, a->s_q, a->h_q, static_cast<int>(plen + slen < most ? plen + slen : most), 0, PLAN_SMS);
+    p.suffix_splits = dsv4_plan_splits(a->b, a->s_q, a->h_q, static_cast<int>(plen + slen), 0, PLAN_SMS);
     p.suffix_bytes = (tokens * (plen + slen) + a->b) * 4;
     return p;
   }
@@ -409,13 +411,16 @@ static int check_shared(const Dsv4SharedPrefixArgs* a) {
       !(a->sm_scale > 0.0f) || !(a->sm_scale <= 1.0e38f) || a->prefix_pages < 0 || a->max_pages < 0 || a->prefix_splits < 0 || a->suffix_splits < 0 ||
       a->prefix_splits > 64 || a->suffix_splits > 64)
     return DSV4_ERR_SHAPE;
-  const int64_t most = 0x7fffffff;
+  const int64_t most = MOST_ITEMS;
   if (static_cast<int64_t>(a->num_blocks) * a->page_block_size > most ||
       static_cast<int64_t>(a->prefix_pages) * a->page_block_size > most ||
       static_cast<int64_t>(a->max_pages) * a->page_block_size > most ||
       (static_cast<int64_t>(a->prefix_pages) + a->max_pages) * a->page_block_size > most ||
       static_cast<int64_t>(a->b) * a->s_q > most / a->h_q ||
       static_cast<int64_t>(a->b) * a->s_q * a->h_q > 64ll * 65535)
+    return DSV4_ERR_SHAPE;
+  // grid dimensions: heads of the combine, and rows as heads of the cross-check kernel
+  if (a->h_q > 65535 || (want_simple(a->flags) && static_cast<int64_t>(a->b) * a->s_q * a->h_q > 65535))
     return DSV4_ERR_SHAPE;
   return DSV4_OK;
 }
@@ -584,7 +589,7 @@ int dsv4_plan_dense_splits(int t_q, int t_k, int b, int h_q, int h_kv, int num_s
 
 int dsv4_dense_prefill(const Dsv4DensePrefillArgs* a, void* stream) {
   if (!a) return DSV4_ERR_NULL;
-  if (a->b < 0 || a->t_q < 0 || a->t_k < 0 || a->h_q < 1 || a->h_kv < 1 || a->h_q % a->h_kv ||
+  if (a->b < 0 || a->t_q < 0 || a->t_k < 0 || a->t_q > MOST_ITEMS || a->t_k > MOST_ITEMS || a->h_q < 1 || a->h_kv < 1 || a->h_q % a->h_kv ||
       a->n_splits < 1 || a->n_splits > dsv4::DENSE_MAX_SPLITS || !(a->sm_scale > 0.0f) ||
       !(a->sm_scale <= 1.0e38f) || dsv4::dense_ctas(a->t_q, a->b, a->h_q, a->h_kv) > (a->n_splits > 1 ? 1 << 24 : 0x7fffffff))
     return DSV4_ERR_SHAPE;
@@ -673,7 +678,7 @@ int dsv4_build_slot_maps(const Dsv4SlotMapArgs* a, void* stream) {
 
 int dsv4_page_indices(const Dsv4PageIndicesArgs* a, void* stream) {
   if (!a) return DSV4_ERR_NULL;
-  if (a->n_rows < 0 || a->topk < 0 || a->b < 0 || a->max_pages < 0 || a->page_block_size < 1 ||
+  if (a->n_rows < 0 || a->topk < 0 || a->n_rows > MOST_ITEMS || a->topk > MOST_ITEMS || a->b < 0 || a->max_pages < 0 || a->page_block_size < 1 ||
       a->s_q < 1 || a->stride_positions < 0 || a->stride_table < 0)
     return DSV4_ERR_SHAPE;
   if (a->n_rows == 0 || a->topk == 0) return DSV4_OK;

@@ -115,7 +115,7 @@ slot_maps_kernel(const Dsv4SlotMapArgs a) {
     *a.n_taken = total_need;
   }
   if (a.b == 0) {
-    for (int t = blockIdx.x * SLOT_THREADS + tid; t < a.n_slots; t += gridDim.x * SLOT_THREADS) {
+    for (long long t = blockIdx.x * SLOT_THREADS + tid; t < a.n_slots; t += gridDim.x * SLOT_THREADS) {
       a.slots[t] = -1;
       a.positions[t] = -1;
     }

@@ -22,6 +22,7 @@ from . import _native as N
 _DENSE_DTYPES = {torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_FP16}
 _KV_DTYPES = (torch.float8_e4m3fn, torch.uint8, torch.int8)
 _SCHED_META_INT32S = 8        # 32-byte record kept for FlashMLA binary parity
+_MOST = 2 ** 31 - 2 ** 16     # sizes are passed as 32-bit numbers, which ctypes would cut silently
 _sm_count = {}
 
 
@@ -300,6 +301,8 @@ def shared_prefix_decode_fwd(q, kv, prefix_table, prefix_length, block_table, su
     fmt = _kv_format(d_qk, token_bytes)
     if int(d_v) != 512:
         raise RuntimeError("Only d_v=512 supported")
+    if max(b, s_q, h_q, num_blocks, page_block, prefix_table.numel(), block_table.size(-1)) > _MOST:
+        raise RuntimeError("sizes of 2^31 and more are not supported")
     kv_strides = kv.stride()
     if (page_block > 1 and kv_strides[1] != token_bytes) or kv_strides[3] != 1:
         raise RuntimeError("kv pages must be dense (only the page stride may be padded)")
@@ -372,6 +375,8 @@ def dense_prefill_fwd(q, k, v, cu_seqlens_q, cu_seqlens_k, sm_scale, causal: boo
         raise RuntimeError(f"(d_qk, d_v) must be (64, 64), (128, 128) or (192, 128); got ({d_qk}, {d_v})")
     if k.shape != (t_k, h_kv, d_qk):
         raise RuntimeError("k must be [t_k, h_kv, d_qk], with v's tokens and heads")
+    if max(t_q, t_k, h_q) > _MOST:
+        raise RuntimeError("sizes of 2^31 and more are not supported")
     if h_kv < 1 or h_q < 1 or h_q % h_kv:
         raise RuntimeError(f"h_q ({h_q}) must be a multiple of h_kv ({h_kv})")
     sq, sk, sv = q.stride(), k.stride(), v.stride()
@@ -491,11 +496,14 @@ def build_slot_maps(block_table, cached_lens, new_lens, free_pages, page_block: 
         raise RuntimeError("page_block >= 1 and n_slots >= 0 expected")
     if b > 16384:
         raise RuntimeError("at most 16384 requests")
+    n_free = free_pages.numel()
+    if n_free > _MOST or max_pages > _MOST:
+        raise RuntimeError("sizes of 2^31 and more are not supported")
     slots = cached_lens.new_empty(n_slots, dtype=torch.int64)
     ints = cached_lens.new_empty(n_slots + 2 * b + 3)
     a = N.SlotMapArgs()
     a.b, a.max_pages, a.page_block_size, a.n_slots = b, max_pages, page_block, n_slots
-    a.n_free = free_pages.numel()
+    a.n_free = n_free
     a.block_table, a.stride_table = block_table.data_ptr(), block_table.stride(0) if b > 1 else max_pages
     a.cached_lens, a.new_lens, a.free_pages = cached_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr()
     a.slots, at = slots.data_ptr(), ints.data_ptr()
@@ -540,6 +548,8 @@ def page_indices(block_table, positions, page_block: int, cu_seqlens=None) -> to
             raise RuntimeError(f"cu_seqlens must have {b + 1} entries")
         if n_rows > 1:
             stride = positions.stride(0)
+    if n_rows > _MOST or topk > _MOST or max_pages > _MOST:
+        raise RuntimeError("sizes of 2^31 and more are not supported")
     out = positions.new_empty(*positions.shape)
     a = N.PageIndicesArgs()
     a.n_rows, a.topk, a.b, a.s_q = n_rows, topk, b, max(s_q, 1)

@@ -286,7 +286,8 @@ int dsv4_sparse_prefill(const Dsv4PrefillArgs* args, void* cuda_stream);
  * q rows are dense: stride_q_h = d_qk, [b, s_q, h_q] contiguous.  Scratch, sized by
  * dsv4_shared_prefix_scratch(args): o_accum fp32 [sets, b, s_q, h_q, 512], lse_accum fp32
  * [sets, b, s_q, h_q], workspace bytes (o_accum and workspace aligned to 32).  num_blocks * page_block_size and
- * (prefix_pages + max_pages) * page_block_size < 2^31; sm_scale is in (0, 1e38].            */
+ * (prefix_pages + max_pages) * page_block_size are at most 2^31 - 2^16, b * s_q * h_q at most
+ * 64 * 65535, h_q 65535; sm_scale is in (0, 1e38].                                         */
 typedef struct Dsv4SharedPrefixArgs {
   int32_t b, s_q, h_q, d_qk, d_v;
   int32_t kv_format;            /* DSV4_KV_MODEL1 or DSV4_KV_V32                 */
@@ -342,7 +343,7 @@ int dsv4_shared_prefix_scratch(const Dsv4SharedPrefixArgs* args, int num_sms, in
  * (d_qk, d_v) is (64, 64), (128, 128) or (192, 128); q, k, v, out of one type.  Strides are
  * in elements, multiples of 8, positive (k and v of several tokens or heads cannot be
  * broadcast views); pointers are 16-byte aligned; the last dimension is dense.  sm_scale is
- * positive and at most 1e38.  n_splits > 1 cuts the sequences' keys into ranges of about the
+ * positive and at most 1e38, t_q and t_k at most 2^31 - 2^16.  n_splits > 1 cuts the sequences' keys into ranges of about the
  * same length, no sequence into more than n_splits (64 at most), and needs o_accum
  * [2 n_splits, t_q, h_q, d_v] (32-byte aligned) and stat_accum [2 n_splits, t_q, h_q, 2].  */
 enum Dsv4Dtype { DSV4_DTYPE_BF16 = 0, DSV4_DTYPE_FP16 = 1 };
@@ -451,7 +452,8 @@ int dsv4_build_slot_maps(const Dsv4SlotMapArgs* args, void* cuda_stream);
  * pos = positions[i][j].  Row i belongs to request r = i / s_q, or, when cu_seqlens
  * [b + 1] is given, to the request with cu_seqlens[r] <= i < cu_seqlens[r + 1].  The result
  * is -1 for a negative position, a column >= max_pages, a negative page id, an index that
- * does not fit int32, and a row of no request.  Rows of indices are dense.                */
+ * does not fit int32, and a row of no request.  Rows of indices are dense.  n_rows and topk
+ * are at most 2^31 - 2^16.                                                                */
 typedef struct Dsv4PageIndicesArgs {
   int32_t n_rows, topk, b, s_q, max_pages, page_block_size;
   const int32_t* block_table;   /* [b, max_pages]                                 */
