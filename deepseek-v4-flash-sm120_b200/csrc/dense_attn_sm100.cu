@@ -1021,16 +1021,16 @@ int pack_of(int group) {
   return 1;
 }
 
+// CTAs of a launch with ranges: one for every SM, or twice the uncut ones where those alone are
+// more than half of the SMs.
+int64_t dense_range_ctas(int64_t ctas, int num_sms) { return 2 * ctas > num_sms ? 2 * ctas : num_sms; }
+
 }  // namespace
 
 int64_t dense_ctas(int t_q, int b, int h_q, int h_kv) {
   const int pack = pack_of(h_q / h_kv);
   return (static_cast<int64_t>(t_q) / (2 * (TILE_M / pack)) + b) * (h_q / pack);
 }
-
-// CTAs of a launch with ranges: one for every SM, or twice the uncut ones where those alone are
-// more than half of the SMs.
-int64_t dense_range_ctas(int64_t ctas, int num_sms) { return 2 * ctas > num_sms ? 2 * ctas : num_sms; }
 
 cudaError_t launch_dense_prefill(const Dsv4DensePrefillArgs& a, int num_sms, cudaStream_t st) {
   DenseParams p;

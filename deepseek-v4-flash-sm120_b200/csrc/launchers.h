@@ -76,7 +76,6 @@ cudaError_t read_prefix_error(int* value, bool reset);
 // Dense attention over packed sequences (dense_attn_sm100.cu).
 constexpr int DENSE_MAX_SPLITS = 64;
 int64_t dense_ctas(int t_q, int b, int h_q, int h_kv);      // CTAs of one key range, at most
-int64_t dense_range_ctas(int64_t ctas, int num_sms);       // CTAs of a launch with ranges
 cudaError_t launch_dense_prefill(const Dsv4DensePrefillArgs& a, int num_sms, cudaStream_t st);
 cudaError_t read_dense_error(int* value, bool reset);
 
