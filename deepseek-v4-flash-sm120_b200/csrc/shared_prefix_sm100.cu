@@ -292,8 +292,8 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
         if (elected) gave_up(code);
         ok = false;
       }
-      __syncwarp();
-    };
+    };                                 // (no lane needs another one until the next segment; a __syncwarp
+                                       // took 1 % more)
     if (warp == WARP_LOAD_K) {
       // ======================= Q and K ======================================================
       int n = 0;
