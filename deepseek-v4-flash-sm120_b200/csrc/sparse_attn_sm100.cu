@@ -114,7 +114,7 @@ struct Ctrl {
   uint32_t tmem;
   int resc;
   int fail;
-  int far;                               // some reference is too large for its BF16 rounding
+  int pad;
   alignas(16) float wred[4][MAX_HEADS];  // per-lane-group column partials (max, then sums)
   alignas(16) float mref[MAX_HEADS];     // reference max, log2-scaled units (read as float4)
   float alpha[MAX_HEADS];                // rescale factor / final output factor
@@ -208,6 +208,13 @@ __device__ __forceinline__ float warp_col_max_packed(uint32_t (&pk)[N / 2], int 
   }
   const uint32_t r = bf16x2_max(pk[0], __shfl_xor_sync(0xffffffffu, pk[0], 1));
   return __uint_as_float((lane & 1) ? (r & 0xffff0000u) : (r << 16));
+}
+
+// Largest of a warp's values; NaN is passed over, as by fmaxf.
+__device__ __forceinline__ float warp_max(float v) {
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
 }
 
 // Column-wise sum, over the 32 lanes of a warp, of N columns held one row per lane:
@@ -666,50 +673,12 @@ __device__ __noinline__ void cluster_merge(const MergeOut p, Ctrl& ctrl, const M
 }
 
 // ---------------------------------------------------------------------------
-// References beyond FAR_REFERENCE (all 512 workers; called by raise_references, which has left those
-// heads alone and their BF16-rounded column maxima in ctrl.aux).  The maxima of what is left above
-// or below those are small, so that BF16 loses nothing of them that matters.
-// ---------------------------------------------------------------------------
-template <int NH>
-__device__ __noinline__ void raise_far_references(Ctrl& ctrl, uint32_t tmem_lanes, bool masked, float cs) {
-  constexpr int CPW = NH / 4;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int lg = warp & 3, cg = warp >> 2;
-  uint32_t s[CPW];
-  tmem_ld_cols<CPW>(tmem_lanes + COL_S + cg * CPW, s);
-  tmem_ld_wait();
-  uint32_t pk[CPW / 2];
-#pragma unroll
-  for (int i = 0; i < CPW / 2; ++i) {
-    const float a = fmaf(__uint_as_float(s[2 * i]), cs, -ctrl.aux[cg * CPW + 2 * i]);
-    const float b = fmaf(__uint_as_float(s[2 * i + 1]), cs, -ctrl.aux[cg * CPW + 2 * i + 1]);
-    pk[i] = pack_bf16x2(masked ? -INFINITY : a, masked ? -INFINITY : b);
-  }
-  const float cm = warp_col_max_packed<CPW>(pk, lane);
-  if (lane < CPW) ctrl.wred[lg][cg * CPW + lane] = cm;
-  bar_sync(WORKER_BARRIER, WORKERS);
-  if (tid < NH) {
-    float tm = ctrl.aux[tid];
-    if (fabsf(tm) >= FAR_REFERENCE && fabsf(tm) < INFINITY) {
-      tm += fmaxf(fmaxf(ctrl.wred[0][tid], ctrl.wred[1][tid]), fmaxf(ctrl.wred[2][tid], ctrl.wred[3][tid]));
-      const float mr = ctrl.mref[tid];
-      if (tm > mr + RESCALE_THRESHOLD) {
-        ctrl.alpha[tid] = (mr <= NEG_HUGE) ? 0.f : ex2(mr - tm);
-        ctrl.mref[tid] = tm;
-        ctrl.resc = 1;
-      }
-    }
-  }
-  bar_sync(WORKER_BARRIER, WORKERS);
-}
-
-// ---------------------------------------------------------------------------
 // Raising the softmax references (all 512 workers; the first tile, and any tile in which
 // some score exceeds its head's reference by more than the threshold).  Column maxima of
-// S^T over the tile's rows (BF16-rounded: the reference only has to be the same for every
-// thread, not exact; raise_far_references deals with those that are too large for it), a new
-// reference where the maximum has grown by more than the threshold (also the first finite one), and O^T in TMEM scaled down to it; the factors
-// stay in ctrl.alpha (ctrl.resc says whether any differs from one) for the caller's
+// S^T over the tile's rows (rounded to BF16, unless FAR_REFERENCE forbids it: the reference only
+// has to be the same for every thread, not exact), a new reference where the maximum has grown by
+// more than the threshold (also the first finite one), and O^T in TMEM scaled down to it; the
+// factors stay in ctrl.alpha (ctrl.resc says whether any differs from one) for the caller's
 // denominators.  Out of line on purpose: it is rare, and the tile loop must stay small.
 // `tmem_lanes` is the TMEM base address with this warp's lane offset applied.
 // ---------------------------------------------------------------------------
@@ -723,35 +692,31 @@ __device__ __noinline__ void raise_references(Ctrl& ctrl, uint32_t tmem_lanes, b
     uint32_t s[CPW];
     tmem_ld_cols<CPW>(tmem_lanes + COL_S + cg * CPW, s);
     tmem_ld_wait();
-    uint32_t pk[CPW / 2];
+    float cm = -INFINITY;                     // of column `lane`
 #pragma unroll
-    for (int i = 0; i < CPW / 2; ++i) {
-      const float a = masked ? -INFINITY : __uint_as_float(s[2 * i]);
-      const float b = masked ? -INFINITY : __uint_as_float(s[2 * i + 1]);
-      pk[i] = pack_bf16x2(a, b);
+    for (int i = 0; i < CPW; ++i) {
+      const float m = warp_max(masked ? -INFINITY : __uint_as_float(s[i]));
+      if (lane == i) cm = m;
     }
-    const float cm = warp_col_max_packed<CPW>(pk, lane);
     if (lane < CPW) ctrl.wred[lg][cg * CPW + lane] = cm;
   }
-  if (tid == 0) ctrl.resc = ctrl.far = 0;
+  if (tid == 0) ctrl.resc = 0;
   bar_sync(WORKER_BARRIER, WORKERS);
   if (tid < NH) {
-    const float tm = fmaxf(fmaxf(ctrl.wred[0][tid], ctrl.wred[1][tid]),
-                           fmaxf(ctrl.wred[2][tid], ctrl.wred[3][tid])) * cs;
+    const float top = fmaxf(fmaxf(ctrl.wred[0][tid], ctrl.wred[1][tid]),
+                            fmaxf(ctrl.wred[2][tid], ctrl.wred[3][tid]));
+    float tm = __bfloat162float(__float2bfloat16_rn(top)) * cs;
+    if (fabsf(tm) >= FAR_REFERENCE) tm = top * cs;
     const float mr = ctrl.mref[tid];
     float alpha = 1.f;
-    if (fabsf(tm) >= FAR_REFERENCE && fabsf(tm) < INFINITY) {
-      ctrl.far = 1;
-    } else if (tm > mr + RESCALE_THRESHOLD) {
+    if (tm > mr + RESCALE_THRESHOLD) {
       alpha = (mr <= NEG_HUGE) ? 0.f : ex2(mr - tm);
       ctrl.mref[tid] = tm;
       ctrl.resc = 1;
     }
     ctrl.alpha[tid] = alpha;
-    ctrl.aux[tid] = tm;
   }
   bar_sync(WORKER_BARRIER, WORKERS);
-  if (ctrl.far) raise_far_references<NH>(ctrl, tmem_lanes, masked, cs);
   if (ctrl.resc && rescale_o) {
     // this warp rescales slice cg of O^T for its 32 TMEM lanes
 #pragma unroll 1
