@@ -44,9 +44,8 @@
 // with the joining launch.
 #include <cuda_fp16.h>
 
-#include <mutex>
-
 #include "attn_params.cuh"
+#include "launch_util.h"
 #include "launchers.h"
 #include "sm100_ptx.cuh"
 #include "tensor_map.h"
@@ -145,11 +144,6 @@ struct DenseParams {
   float *o_accum, *stat_accum;   // [2 splits][t][h][d_v], [2 splits][t][h][2] (max logit, log-sum-exp)
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // Pairs of 32-bit floats in one 64-bit register: one instruction for both.
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
   uint64_t d;
@@ -762,7 +756,7 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
     const bool raise = top2 > m_ref + RESCALE_THRESHOLD;       // also the first finite one
     float alpha = 1.f;
     if (raise) {
-      alpha = ex2(m_ref - top2);                               // 0 for the first
+      alpha = ex2_ftz(m_ref - top2);                               // 0 for the first
       m_ref = top2;
       l *= alpha;
     }
@@ -794,8 +788,8 @@ dense_attn_kernel(const __grid_constant__ DenseParams p) {
       for (int j = 0; j < 16; ++j) {
         float a, b;
         unpair(fma_pair(pair(__uint_as_float(x[32 * q + 2 * j]), __uint_as_float(x[32 * q + 2 * j + 1])), c2, minus_ref), a, b);
-        a = ex2(a);
-        b = ex2(b);
+        a = ex2_ftz(a);
+        b = ex2_ftz(b);
         sum[j & 1] = add_pair(sum[j & 1], pair(a, b));
         pk[j] = pack2<BF16>(a, b);
       }
@@ -972,26 +966,11 @@ dense_combine_kernel(const __grid_constant__ DenseParams p) {
   }
 }
 
-constexpr int MAX_DEVICES = 64;
-std::mutex g_dense_mu;
-
 template <int DQK, int DV, bool BF16, bool RANGES>
 cudaError_t launch_one(const DenseParams& p, cudaStream_t st) {
   constexpr size_t smem = dense_smem_bytes<DQK, DV>();
-  static bool configured[MAX_DEVICES] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  cudaError_t e = allow_shared_memory<dense_attn_kernel<DQK, DV, BF16, RANGES>>(smem);
   if (e) return e;
-  if (dev < 0 || dev >= MAX_DEVICES) return cudaErrorInvalidDevice;
-  {
-    std::lock_guard<std::mutex> lk(g_dense_mu);
-    if (!configured[dev]) {
-      e = cudaFuncSetAttribute(dense_attn_kernel<DQK, DV, BF16, RANGES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               static_cast<int>(smem));
-      if (e) return e;
-      configured[dev] = true;
-    }
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(RANGES ? p.ctas : p.items));
   cfg.blockDim = dim3(THREADS);

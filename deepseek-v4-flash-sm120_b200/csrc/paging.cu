@@ -19,9 +19,8 @@
 // out, bound by memory for prefill lists.  16-byte loads and stores where rows allow, the
 // division by a multiplication prepared on the host.  Measured: 8192 x 2048 entries 23.7 us,
 // 5.7 TB/s (0.87 of a copy's rate); 64 x 2048 entries 2.7 us in a graph.
-#include <mutex>
-
 #include "attn_params.cuh"
+#include "launch_util.h"
 #include "launchers.h"
 #include "paging.cuh"
 
@@ -203,27 +202,13 @@ page_indices_kernel(const Dsv4PageIndicesArgs a, const FastDiv page) {
   }
 }
 
-constexpr int MAX_DEVICES = 64;
-std::mutex g_paging_mu;
-
 }  // namespace
 
 cudaError_t launch_slot_maps(const Dsv4SlotMapArgs& a, cudaStream_t st) {
   const size_t smem = 2 * (static_cast<size_t>(a.b) + 1) * sizeof(int);
-  static bool configured[MAX_DEVICES] = {};
   int dev = 0, sms = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  cudaError_t e = allow_shared_memory<slot_maps_kernel>(2 * (SLOT_MAP_MAX_REQUESTS + 1) * sizeof(int), &dev);
   if (e) return e;
-  if (dev < 0 || dev >= MAX_DEVICES) return cudaErrorInvalidDevice;
-  {
-    std::lock_guard<std::mutex> lk(g_paging_mu);
-    if (!configured[dev]) {
-      e = cudaFuncSetAttribute(slot_maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               static_cast<int>(2 * (SLOT_MAP_MAX_REQUESTS + 1) * sizeof(int)));
-      if (e) return e;
-      configured[dev] = true;
-    }
-  }
   if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev))) return e;
   const long long want = (static_cast<long long>(a.n_slots) + a.b + SLOT_THREADS - 1) / SLOT_THREADS;
   cudaLaunchConfig_t cfg = {};

@@ -37,9 +37,8 @@
 // 1.5 PFLOP/s for the prefix alone, tensor pipe 86 % busy at an SM clock of 1.55 GHz that the power
 // limit sets.  Bound by the tensor cores at that clock; around it conversion 25 us (6.9 TB/s with
 // rows that stay in L2) and the join 12 us (2 KB a row and set read, 1 KB a row written).
-#include <mutex>
-
 #include "attn_params.cuh"
+#include "launch_util.h"
 #include "launchers.h"
 #include "paging.cuh"
 #include "sm100_ptx.cuh"
@@ -151,11 +150,6 @@ __device__ __forceinline__ void commit2(uint32_t bar, uint32_t elected) {
       "setp.ne.b32 q, %1, 0;\n\t"
       "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}"
       ::"r"(bar), "r"(elected) : "memory");
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
@@ -467,7 +461,7 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
           const float both = fmaxf(top2, ctrl.part[2 * group + (half ^ 1)][r]);
           float alpha = 1.f;
           if (both > ref + RESCALE_THRESHOLD) {
-            alpha = ex2(ref - both);               // 0 for the first
+            alpha = ex2_ftz(ref - both);               // 0 for the first
             ref = both;
           }
           bar_sync(BAR_GROUP + group, GROUP);      // both threads of a row have read the old one
@@ -491,7 +485,7 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
         }
         if (n + 1 < total_tiles) bar_arrive(BAR_DECIDED + group, SOFTMAX_THREADS);
         if (ref != m_ref) {                        // raised here or by the other group
-          l *= ex2(m_ref - ref);
+          l *= ex2_ftz(m_ref - ref);
           m_ref = ref;
         }
         const float sub = ref == -INFINITY ? 0.f : ref;
@@ -499,8 +493,8 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
         uint32_t pk[32];
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
-          const float a = ex2(fmaf(__uint_as_float(x[2 * k]), c, -sub));
-          const float b = ex2(fmaf(__uint_as_float(x[2 * k + 1]), c, -sub));
+          const float a = ex2_ftz(fmaf(__uint_as_float(x[2 * k]), c, -sub));
+          const float b = ex2_ftz(fmaf(__uint_as_float(x[2 * k + 1]), c, -sub));
           sum[(2 * k) & 3] += a;
           sum[(2 * k + 1) & 3] += b;
           pk[k] = pack_bf16x2(a, b);
@@ -559,7 +553,7 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
       // ---- the segment's partial ------------------------------------------------------------
       bar_sync(BAR_BOTH, SOFTMAX_THREADS);         // every decision has been made
       const float ref = ctrl.ref[r];
-      if (ref != m_ref) l *= ex2(m_ref - ref);
+      if (ref != m_ref) l *= ex2_ftz(m_ref - ref);
       ctrl.part[2 * group + half][r] = l;
       bar_sync(BAR_BOTH, SOFTMAX_THREADS);
       const float total = (ctrl.part[0][r] + ctrl.part[1][r]) + (ctrl.part[2][r] + ctrl.part[3][r]);
@@ -899,25 +893,11 @@ join_sets_kernel(const Dsv4CombineArgs a) {
   }
 }
 
-constexpr int MAX_DEVICES = 64;
-std::mutex g_prefix_mu;
-
 template <int DQK>
 cudaError_t launch_attn(const PrefixParams& p, int clusters, cudaStream_t st) {
   constexpr size_t smem = prefix_smem_bytes<DQK>();
-  static bool configured[MAX_DEVICES] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  cudaError_t e = allow_shared_memory<prefix_attn_kernel<DQK>>(smem);
   if (e) return e;
-  if (dev < 0 || dev >= MAX_DEVICES) return cudaErrorInvalidDevice;
-  {
-    std::lock_guard<std::mutex> lk(g_prefix_mu);
-    if (!configured[dev]) {
-      e = cudaFuncSetAttribute(prefix_attn_kernel<DQK>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-      if (e) return e;
-      configured[dev] = true;
-    }
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * clusters);
   cfg.blockDim = dim3(THREADS);

@@ -342,6 +342,13 @@ __device__ __forceinline__ void st_global_32(void* p, uint32_t a, uint32_t b, ui
                ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d), "r"(e), "r"(f), "r"(g), "r"(h) : "memory");
 }
 
+// 2^x; results below 2^-126 are zero.
+__device__ __forceinline__ float ex2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t pred;
   asm volatile(

@@ -46,10 +46,10 @@
 // g_attn_error, and the CTA walks on without waiting again, drops its outputs and
 // writes NaN into the log-sum-exp slots it owns so that the failure is visible
 // downstream without a host synchronisation.
-#include <mutex>
 #include <type_traits>
 
 #include "attn_params.cuh"
+#include "launch_util.h"
 #include "launchers.h"
 #include "sm100_ptx.cuh"
 
@@ -1372,28 +1372,11 @@ sm100_attn_kernel(const AttnParams p) {
   if (tid == 0) stamp_cta(p, 3);
 }
 
-// The dynamic shared-memory limit of a kernel is a per-device attribute: set once per
-// (instantiation, device).
-constexpr int MAX_DEVICES = 64;
-std::mutex g_configure_mu;
-
 template <int FMT, int DQK, int NH, bool EXTRA>
 cudaError_t launch_one(const AttnParams& p, cudaStream_t st) {
   constexpr size_t smem = smem_bytes<FMT, DQK, NH>();
-  static bool configured[MAX_DEVICES] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  cudaError_t e = allow_shared_memory<sm100_attn_kernel<FMT, DQK, NH, EXTRA>>(smem);
   if (e) return e;
-  if (dev < 0 || dev >= MAX_DEVICES) return cudaErrorInvalidDevice;
-  {
-    std::lock_guard<std::mutex> lk(g_configure_mu);
-    if (!configured[dev]) {
-      e = cudaFuncSetAttribute(sm100_attn_kernel<FMT, DQK, NH, EXTRA>,
-                               cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-      if (e) return e;
-      configured[dev] = true;
-    }
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.n_req, (p.h_q + NH - 1) / NH, p.n_splits);
   cfg.blockDim = dim3(THREADS);
