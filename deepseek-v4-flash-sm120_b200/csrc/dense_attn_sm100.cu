@@ -35,13 +35,15 @@
 // pipeline ("twin"), which halves its chain of products and softmaxes; a range therefore has
 // two partial sets.
 //
-// Measured.  One prompt of 8192, 16 heads, (192, 128), causal: 270 us from a cold clock, 1.27
-// PFLOP/s of the products that are not masked (0.76 of a matrix product's rate), 327 us under the
+// Measured.  One prompt of 8192, 16 heads, (192, 128), causal: 272 us from a cold clock, 1.26
+// PFLOP/s of the products that are not masked (0.75 of a matrix product's rate), 328 us under the
 // power limit; tensor pipe 64 % busy, bound by the 128 exponentials, sums and conversions of
-// each thread and tile beside it.  Packed prompts, 24 heads on 4, (128, 128): 253 us and 55 %.
-// Single tokens, 8 contexts of 1000 to 16383, 32 heads on 8: 18 us a CTA for 99 MB, of which 13 us
-// stream at memory's rate (with one unit of V less for twins 17) and 5 are its start and end; 31 us
-// with the joining launch.
+// each thread and tile beside it.  Packed prompts, 24 heads on 4, (128, 128): 255 to 276 us from a
+// cold clock, 302 under the power limit, tensor pipe 56 % busy: products and exponentials take equal
+// clocks there and overlap in part, and an SM's ten CTAs start and end one after the other.  (64, 64),
+// one prompt of 8192: 184 us, 119 of them for the exponentials alone.  Single tokens, 8 contexts of 1000
+// to 16383, 32 heads on 8: 18 us a CTA for 99 MB, of which 13 us stream at memory's rate (with one
+// unit of V less for twins 17) and 5 are its start and end; 31 us with the joining launch.
 #include <cuda_fp16.h>
 
 #include "attn_params.cuh"

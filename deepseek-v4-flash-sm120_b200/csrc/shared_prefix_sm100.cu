@@ -33,10 +33,10 @@
 // leaving a normalised 32-bit partial and its log-sum-exp.  The segments of a row block are its
 // sets 0, 1, ...; the last one marks the sets that are not used with -inf.
 //
-// Measured (64 requests x 64 heads, a prefix of 32768 of d_qk 576, 64 to 2048 own tokens): 194 us,
-// 1.5 PFLOP/s for the prefix alone, tensor pipe 86 % busy at an SM clock of 1.55 GHz that the power
-// limit sets.  Bound by the tensor cores at that clock; around it conversion 25 us (6.9 TB/s with
-// rows that stay in L2) and the join 12 us (2 KB a row and set read, 1 KB a row written).
+// Measured (64 requests x 64 heads, a prefix of 32768 of d_qk 576, 64 to 2048 own tokens): 191 us,
+// 1.5 PFLOP/s for the prefix alone, tensor pipe 91 % busy at an SM clock of 1.43 GHz (both from one
+// profile).  Bound by the tensor cores at that clock; around it conversion 26 us and the join 14 us
+// (2 KB a row and set read, 1 KB a row written).
 #include "attn_params.cuh"
 #include "launch_util.h"
 #include "launchers.h"
@@ -683,8 +683,9 @@ __device__ __forceinline__ void block_starts(const Dsv4SharedPrefixArgs& a, cons
 // of the prefix, and of every request's own tokens, -> BF16 rows [tokens, d_qk], and a bit per
 // token that says whether it exists; rows that do not are zero.  Whole tiles of 128 tokens are
 // written.  Bound by memory: 644 (584) B in and 1152 (1024) B out per token; a warp has four
-// tokens in flight (32768 tokens and 64 x 1000 own ones: 24 us, 7 TB/s with writes that stay in L2).  One CTA: where the row blocks' tiles start.  CTAs [row_ctas, +list_ctas):
-// token indices of the prefix.  The others: one query token's list each, of its own tokens or of
+// tokens in flight (32768 tokens and 64 x 1000 own ones: 26 us, writes that stay in L2 among them).
+// One CTA: where the row blocks' tiles start.  CTAs [row_ctas, +list_ctas): token indices of the
+// prefix.  The others: one query token's list each, of its own tokens or of
 // the prefix and those.  List entries behind a length are not written: nothing reads them.
 template <int FMT>
 __global__ void __launch_bounds__(256)
