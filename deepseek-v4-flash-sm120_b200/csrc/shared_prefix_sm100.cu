@@ -268,8 +268,9 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
   const uint32_t tmem = ctrl.tmem;
   grid_dependency_wait();
   Share w(p, blockIdx.x >> 1, gridDim.x >> 1);
-  // A lane whose bounded wait gives up records it, waits for nothing any more and issues nothing; but
-  // it walks on through the same loops, so that its warp stays together for what the whole warp has
+  // A lane whose bounded wait gives up records it, waits for nothing any more, and issues and reports
+  // nothing (its arrivals would stand in for the other CTA's, whose rows would be wrong and not know);
+  // but it walks on through the same loops, so that its warp stays together for what the whole warp has
   // to execute (a phase may complete just as the first lanes give up) and every barrier of the CTA
   // is met.
   bool ok = true;
@@ -439,7 +440,7 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
         tmem_ld_wait();
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) arrive_leader(bar(&ctrl.s_free[group]));
+        if (lane == 0 && ok) arrive_leader(bar(&ctrl.s_free[group]));
         if ((seen.x & seen.y) != 0xffffffffu) {
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
@@ -509,7 +510,7 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
         fence_async_smem();
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) arrive_leader(bar(&ctrl.p_full));
+        if (lane == 0 && ok) arrive_leader(bar(&ctrl.p_full));
       };
       // bits are fetched a tile ahead
       const uint2* bits = reinterpret_cast<const uint2*>(p.valid) + w.first * 2 + half;
@@ -583,7 +584,7 @@ prefix_attn_kernel(const __grid_constant__ PrefixParams p) {
         if (k == 3) {
           tc_fence_before_sync();
           __syncwarp();
-          if (lane == 0) arrive_leader(bar(&ctrl.o_free));
+          if (lane == 0 && ok) arrive_leader(bar(&ctrl.o_free));
         }
 #pragma unroll
         for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);

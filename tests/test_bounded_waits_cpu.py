@@ -38,3 +38,11 @@ def test_every_wait_is_skipped_after_one_has_given_up(name):
     text = source(name)
     for m in re.finditer(r"!mbar_wait_fast\(", text):
         assert text[:m.start()].rstrip().endswith("ok &&"), text[m.start() - 60:m.end() + 60]
+
+
+def test_a_lane_that_gave_up_reports_nothing_to_the_other_cta():
+    """The leader's barriers count arrivals of both CTAs: one that no longer waits could arrive in the other's place."""
+    text = source("shared_prefix_sm100.cu")
+    calls = re.findall(r"if \(([^\n]*)\) arrive_leader\(", text)
+    assert len(calls) == 3 and all(c == "lane == 0 && ok" for c in calls)
+    assert len(re.findall(r"arrive_leader\(bar\(", text)) == 3
