@@ -460,7 +460,8 @@ __device__ __forceinline__ void store_line(const uint4& v, uint32_t sK, int row,
 // with n_splits == cs there is no combine launch at all.  An empty split (no tile) takes
 // part with l = 0, m = "none" (weight 0) and stages zeros; a CTA
 // whose bounded wait gave up still walks every barrier (its peers must not be left
-// waiting) and only drops its own stores.
+// waiting), drops its own stores, and gives NaN for its sums, so that what the others write
+// says so too.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -584,8 +585,9 @@ __device__ __noinline__ void cluster_merge(const MergeOut p, Ctrl& ctrl, const M
   if (tid < MAX_HEADS) {
     const uint32_t a_l = smem_u32(&ctrl.wred[rank][tid]), a_m = smem_u32(&ctrl.wmax[rank][tid]);
     const float mv = (m_own <= NEG_HUGE) ? -INFINITY : m_own;
+    const float lv = ctrl.fail ? NAN : l_own;            // NaN in every CTA's part of the result
     for (int r = 0; r < cs; ++r) {
-      st_cluster_b32(map_to_rank(a_l, r), __float_as_uint(l_own));
+      st_cluster_b32(map_to_rank(a_l, r), __float_as_uint(lv));
       st_cluster_b32(map_to_rank(a_m, r), __float_as_uint(mv));
     }
   }

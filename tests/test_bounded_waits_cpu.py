@@ -46,3 +46,10 @@ def test_a_lane_that_gave_up_reports_nothing_to_the_other_cta():
     calls = re.findall(r"if \(([^\n]*)\) arrive_leader\(", text)
     assert len(calls) == 3 and all(c == "lane == 0 && ok" for c in calls)
     assert len(re.findall(r"arrive_leader\(bar\(", text)) == 3
+
+
+def test_a_cta_that_gave_up_makes_the_whole_cluster_s_result_nan():
+    """Each CTA of a cluster writes columns of the merged row, and one of them its log-sum-exp."""
+    body = re.search(r"void cluster_merge\(.*?\n\}", source("sparse_attn_sm100.cu"), re.S).group(0)
+    assert re.search(r"const float lv = ctrl\.fail \? NAN : l_own;", body)
+    assert "st_cluster_b32(map_to_rank(a_l, r), __float_as_uint(lv));" in body
