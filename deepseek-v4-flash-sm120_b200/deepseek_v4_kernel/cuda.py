@@ -284,8 +284,8 @@ def shared_prefix_decode_fwd(q, kv, prefix_table, prefix_length, block_table, su
       -> (out [b, s_q, h_q, 512] bf16, lse [b, h_q, s_q] fp32, sink-merged)
 
     Query token s sees the whole prefix and suffix_length - (s_q - 1 - s) own tokens.  A row
-    that sees nothing gives out 0 and lse = its sink, or -inf.  Tokens on pages outside the
-    cache are masked.  The lengths stay on the device, so a captured call can be replayed
+    that sees nothing gives out 0 and lse = its sink, or -inf; one that sees a NaN or +inf
+    score is NaN.  Tokens on pages outside the cache are masked.  The lengths stay on the device, so a captured call can be replayed
     with others; the scratch grows with what the two tables can hold (2 * d_qk bytes a token
     of the prefix table, 4 GiB at most, beyond which the call takes 2.5 times as long), so they
     should be no wider than needed.  `prefix_splits` / `suffix_splits` / `flags` are test hooks.  No counterpart

@@ -280,14 +280,14 @@ int dsv4_sparse_prefill(const Dsv4PrefillArgs* args, void* cuda_stream);
  * once for the rows of all requests together; the two parts are joined by their
  * log-sum-exps.  Layouts, out, lse (sink-merged) and strides as dsv4_sparse_decode's; a row
  * that sees nothing gives out 0 and lse = its sink, or -inf; one that sees a NaN or +inf
- * score is NaN.  Tokens of a page id outside [0, num_blocks) are masked; lengths are clamped to the tables.  The lengths live on the
- * device; launches depend on sizes only.
+ * score is NaN.  Tokens of a page id outside [0, num_blocks) are masked; lengths are clamped
+ * to the tables.  The lengths live on the device; launches depend on sizes only.
  *
  * q rows are dense: stride_q_h = d_qk, [b, s_q, h_q] contiguous.  Scratch, sized by
  * dsv4_shared_prefix_scratch(args): o_accum fp32 [sets, b, s_q, h_q, 512], lse_accum fp32
- * [sets, b, s_q, h_q], workspace bytes (o_accum and workspace aligned to 32).  num_blocks * page_block_size and
- * (prefix_pages + max_pages) * page_block_size are at most 2^31 - 2^16, b * s_q * h_q at most
- * 64 * 65535, h_q 65535; sm_scale is in (0, 1e38].                                         */
+ * [sets, b, s_q, h_q], workspace bytes (o_accum and workspace aligned to 32).
+ * num_blocks * page_block_size and (prefix_pages + max_pages) * page_block_size are at most
+ * 2^31 - 2^16, b * s_q * h_q at most 64 * 65535, h_q 65535; sm_scale is in (0, 1e38].       */
 typedef struct Dsv4SharedPrefixArgs {
   int32_t b, s_q, h_q, d_qk, d_v;
   int32_t kv_format;            /* DSV4_KV_MODEL1 or DSV4_KV_V32                 */
